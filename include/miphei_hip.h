@@ -166,6 +166,64 @@ MVIT_API int mvit_attention_fwd(const void* qkv, void* out, void* out_res, float
 MVIT_API int mvit_attention_bwd(const void* qkv, const void* out, const void* out_res, const void* d_out, const float* lse,
                                 float* dsum, void* dqkv, int B, int N, int H, int Dh, float scale, mvit_stream_t stream);
 
+/* ---------------------------------------------------------------- transformer-block operators (torch.ops.mvit.*) */
+/* Root-mean-square norm of a residual stream.  h = x + res (kept in res's type; what is normed is h as it is stored),
+ * y = h / sqrt(mean(h^2) + eps) * w, rstd(f32)[M] (optional) = 1 / sqrt(...) for the backward pass.  *_f32 != 0: that operand is f32,
+ * else 16-bit; row strides ldx, ldr in elements, h and y are dense [M, D].  res = NULL: h is x and is not written.
+ * x 16-bit: res 16-bit or f32, y 16-bit.  x f32: res f32, y 16-bit or f32.  1 <= D <= 16384, any D and any alignment (16-byte loads
+ * where D % 8 == 0 and all rows start on 16 bytes). */
+MVIT_API int mvit_rmsnorm_fwd(const void* x, int x_f32, long long ldx, const void* res, int res_f32, long long ldr, const void* w,
+                              int w_f32, void* h, void* y, int y_f32, float* rstd, int M, int D, float eps, mvit_stream_t stream);
+/* The same with y in 8 bits: scale(f32)[M] = max(max |y|, 1e-30) / 448, q(e4m3)[M, D] = y / scale rounded to nearest even.  A row with
+ * a NaN or an infinity in y reads back (q * scale) as NaN. */
+MVIT_API int mvit_rmsnorm_fp8_fwd(const void* x, int x_f32, long long ldx, const void* res, int res_f32, long long ldr, const void* w,
+                                  int w_f32, void* h, void* q, float* scale, int M, int D, float eps, mvit_stream_t stream);
+/* q, scale of the rows of x itself (no norm). */
+MVIT_API int mvit_quantize_rows_fp8(const void* x, int x_f32, long long ldx, void* q, float* scale, int M, int D, mvit_stream_t stream);
+/* Backward of mvit_rmsnorm_fwd: g = dh + rstd (w dy - xhat mean(w dy xhat)), xhat = h rstd, written to dx (dy's type) and / or dres
+ * (h's type), either may be NULL; dh (h's type) may be NULL; dw (w's type)[D] = sum over rows of dy xhat, NULL if not wanted.  x_f32:
+ * the type of dy and dx.  All rows dense.  scratch: mvit_rmsnorm_bwd_scratch_bytes(M, D) bytes of partial sums of dw (needed with dw
+ * only); ordered sums, bit-identical from run to run. */
+MVIT_API long long mvit_rmsnorm_bwd_scratch_bytes(int M, int D);
+MVIT_API int mvit_rmsnorm_bwd(const void* dy, int x_f32, const void* dh, const void* h, int h_f32, const void* w, int w_f32,
+                              const float* rstd, void* dx, void* dres, void* dw, void* scratch, long long scratch_bytes, int M, int D,
+                              mvit_stream_t stream);
+/* Rotary positions with 1 to 4 axes on x [B, N, H, Dh] (any batch / token / head strides, in elements; last one 1) -> y (its own strides;
+ * y = x with equal strides: in place).  Pair i of the first 2P values of a head, P = sum of sections, is (i, i + P), or (2i, 2i + 1)
+ * where interleaved, and turns by positions[n - prefix][axis of i] * inv_freq[i]; sections[a] consecutive pairs belong to axis a.
+ * Tokens before prefix, heads from rotate_heads on and values from 2P on pass through.  inverse != 0: by the negative angle (the
+ * gradient).  positions [N - prefix, axes], pos_b elements apart per batch entry (0: shared), pos_type 0 int32, 1 int64, 2 f32;
+ * inv_freq [P] f64 (freq_f64) or f32.  Dh even, <= 1024; H <= 1024; B <= 65535. */
+typedef struct mvit_rotary_args {
+  const void* x; void* y; const void* positions; const void* inv_freq;
+  long long xb, xn, xh, yb, yn, yh, pos_b;
+  int B, N, H, Dh, rotate_heads, prefix, axes;
+  int sections[4];
+  int x_f32, pos_type, freq_f64, interleaved, inverse;
+} mvit_rotary_args;
+MVIT_API int mvit_rotary(const mvit_rotary_args* args, mvit_stream_t stream);
+
+/* y[M,N] = res + act(x[M,K] W[N,K]^T + bias), f32 accumulation.  mvit_linear_act: 16-bit x, W; pre (optional, 16-bit, dense [M,N])
+ * receives the value in front of the activation for the backward pass.  mvit_linear_fp8: e4m3 x, W, the product times
+ * x_scale(f32)[m] * w_scale(f32)[n]; no pre.  bias [N] f32 or 16-bit, may be NULL.  y dense, f32 or 16-bit; res (may be NULL) has y's type
+ * and its own row stride ldr.  ldx, ldw, ldr in elements.  x, W rows start on 16 bytes and K is a multiple of 16 bytes (8 or 16 values);
+ * K and the row strides of x and W are at most 2^23 bytes.  M, N of any size. */
+enum mvit_activation { MVIT_ACT_NONE = 0, MVIT_ACT_RELU = 1, MVIT_ACT_SILU = 2, MVIT_ACT_GELU = 3, MVIT_ACT_GELU_TANH = 4 };
+typedef struct mvit_linear_args {
+  const void* x; const void* w; const void* bias; const void* res; void* y; void* pre; const float* x_scale; const float* w_scale;
+  long long ldx, ldw, ldr;
+  int M, N, K, act, bias_f32, y_f32;
+} mvit_linear_args;
+MVIT_API int mvit_linear_act(const mvit_linear_args* args, mvit_stream_t stream);
+MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_stream_t stream);
+/* Backward of the epilogue: dz(16-bit)[M,N] = dy * act'(pre) (pre NULL: act is none), dbias[N] (f32 or 16-bit) = its sum over the rows,
+ * taken before dz is rounded; dz or dbias may be NULL.  dy f32 or 16-bit, all dense.  scratch: mvit_act_bwd_scratch_bytes(M, N) bytes
+ * (needed with dbias only); ordered sums, bit-identical from run to run.  dx and dW are the products dz W and dz^T x
+ * (mvit_gemm_bf16, mvit_gemm_tn_bf16). */
+MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N);
+MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, void* dbias, int dbias_f32, void* scratch, int M,
+                          int N, mvit_stream_t stream);
+
 /* ---------------------------------------------------------------- decoder data movement (NHWC bf16) */
 /* dst[b,oy,ox,c] = sum_{ty,tx} ty_w[oy,ty]*tx_w[ox,tx] * f(src[b, ty_idx[oy,ty], tx_idx[ox,tx], c]),
  * f = identity or relu(v*scale[c]+shift[c]) (BatchNorm+ReLU of the producer fused into the gather).

@@ -58,6 +58,19 @@ class ConvUnpackDesc(C.Structure):
     _fields_ = [("dWt", vp), ("dW", vp), ("Cout", ci), ("Cin", ci), ("Cp", ci), ("rot", ci), ("accumulate", ci), ("n_major", ci)]
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = [("x", vp), ("y", vp), ("positions", vp), ("inv_freq", vp),
+                ("xb", ll), ("xn", ll), ("xh", ll), ("yb", ll), ("yn", ll), ("yh", ll), ("pos_b", ll),
+                ("B", ci), ("N", ci), ("H", ci), ("Dh", ci), ("rotate_heads", ci), ("prefix", ci), ("axes", ci),
+                ("sections", ci * 4), ("x_f32", ci), ("pos_type", ci), ("freq_f64", ci), ("interleaved", ci), ("inverse", ci)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [("x", vp), ("w", vp), ("bias", vp), ("res", vp), ("y", vp), ("pre", vp), ("x_scale", vp), ("w_scale", vp),
+                ("ldx", ll), ("ldw", ll), ("ldr", ll),
+                ("M", ci), ("N", ci), ("K", ci), ("act", ci), ("bias_f32", ci), ("y_f32", ci)]
+
+
 # name -> argtypes (restype is always int); mirrors include/miphei_hip.h
 SIGNATURES = {
     "mvit_gemm_bf16": [C.POINTER(GemmArgs), vp],
@@ -116,6 +129,16 @@ SIGNATURES = {
     "mvit_augment_draw": [ci, ci, ci, ci, C.c_ulonglong, C.c_ulonglong, cf, cf, cf, cf, vp],
     "mvit_cell_means": [vp, vp, vp, ci, ci, ci, ci, ci, cf, ci, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp],
     "mvit_adam_clip_step": [vp, vp, vp, vp, vp, ll, cf, cf, cf, cf, cf, cf, cf, vp, vp],
+    "mvit_rmsnorm_fwd": [vp, ci, ll, vp, ci, ll, vp, ci, vp, vp, ci, vp, ci, ci, cf, vp],
+    "mvit_rmsnorm_fp8_fwd": [vp, ci, ll, vp, ci, ll, vp, ci, vp, vp, vp, ci, ci, cf, vp],
+    "mvit_quantize_rows_fp8": [vp, ci, ll, vp, vp, ci, ci, vp],
+    "mvit_rmsnorm_bwd_scratch_bytes": [ci, ci],
+    "mvit_rmsnorm_bwd": [vp, ci, vp, vp, ci, vp, ci, vp, vp, vp, vp, vp, ll, ci, ci, vp],
+    "mvit_rotary": [C.POINTER(RotaryArgs), vp],
+    "mvit_linear_act": [C.POINTER(LinearArgs), vp],
+    "mvit_linear_fp8": [C.POINTER(LinearArgs), vp],
+    "mvit_act_bwd": [vp, ci, vp, ci, vp, vp, ci, vp, ci, ci, vp],
+    "mvit_act_bwd_scratch_bytes": [ci, ci],
     "mvit_occupy_cus": [ci, ci, vp],
 }
 

@@ -1,0 +1,478 @@
+// Root-mean-square norm of a residual stream, with its backward pass and its 8-bit form, and the 8-bit quantisation of rows.
+//
+//   h = x + residual                              kept in the residual stream's type: what the next layer reads is what is normed
+//   y = h * r * w,  r = 1 / sqrt(mean(h^2) + eps)
+//   8 bits: scale = max(max |y|, 1e-30) / 448 (one per row), q = e4m3(y / scale); 448 is the largest e4m3 value
+//   d h = d h_out + r (w dy - xhat mean(w dy xhat)),  xhat = h r;   d w = sum over rows of dy xhat
+//
+// All of it is bound by HBM: a row is read once, lives in registers (f32) while its sum of squares, its largest value and its outputs
+// are formed, and is written once.
+//  * A row belongs to TPR = 64 threads (one wave: no barrier) or, from D > 4096 on or where there are fewer rows than the chip has
+//    waves, to 256 (the row's latency then counts, and a quarter of the loads per thread is what shortens it).
+//  * Each thread holds NV pieces of VEC values; VEC = 8 (16-byte loads) where D, the row strides and the addresses allow it, else 1.
+//  * Rows are walked with a grid stride, so that w is loaded once per thread and not once per row.
+// Sums and statistics are f32; sums over the rows (d w) go row by row in registers, over the waves of a block in LDS, over the blocks
+// through a [blocks][D] f32 workspace that a second launch adds up: a fixed order, no atomics, bit-identical from run to run.
+#include "common.hpp"
+#include "../../include/miphei_hip.h"
+
+namespace {
+
+enum { T16 = 0, F32 = 1, NONE = 2, F8 = 3 };
+
+constexpr float E4M3_MAX = 448.f, AMAX_MIN = 1e-30f;
+
+// VEC values from element `i` of a 16-bit or f32 array
+template <int T, int VEC>
+__device__ __forceinline__ void load_vec(const void* p, size_t i, float* v) {
+  if constexpr (T == T16) {
+    if constexpr (VEC == 8) {
+      const uint4 u = *(const uint4*)((const bf16_t*)p + i);
+      v[0] = lo16f(u.x), v[1] = hi16f(u.x), v[2] = lo16f(u.y), v[3] = hi16f(u.y);
+      v[4] = lo16f(u.z), v[5] = hi16f(u.z), v[6] = lo16f(u.w), v[7] = hi16f(u.w);
+    } else {
+      v[0] = bf2f(((const bf16_t*)p)[i]);
+    }
+  } else {
+    if constexpr (VEC == 8) {
+      const float4 a = *(const float4*)((const float*)p + i), b = *(const float4*)((const float*)p + i + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      v[0] = ((const float*)p)[i];
+    }
+  }
+}
+template <int T, int VEC>
+__device__ __forceinline__ void store_vec(void* p, size_t i, const float* v) {
+  if constexpr (T == T16) {
+    if constexpr (VEC == 8)
+      *(uint4*)((bf16_t*)p + i) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+    else
+      ((bf16_t*)p)[i] = f2bf(v[0]);
+  } else if constexpr (T == F32) {
+    if constexpr (VEC == 8) {
+      *(float4*)((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+      *(float4*)((float*)p + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      ((float*)p)[i] = v[0];
+    }
+  } else {
+    if constexpr (VEC == 8) {
+      int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+      a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true), b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], b, true);
+      *(int2*)((uint8_t*)p + i) = make_int2(a, b);
+    } else {
+      ((uint8_t*)p)[i] = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[0], 0, false) & 0xff);
+    }
+  }
+}
+// the value as it reads back from the stream's own type (16-bit streams are normed as they are stored)
+template <int T>
+__device__ __forceinline__ float as_stored(float v) {
+  if constexpr (T == T16) return bf2f(f2bf(v));
+  return v;
+}
+
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+  return v;
+}
+
+// Sum and maximum over the TPR threads of a row.  TPR = 256: through 4 words of LDS, one set of them for each turn (`odd`), so that
+// the next reduction's writes never meet this one's reads: one barrier a reduction.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* lds, int& turn) {
+  v = wave_sum(v);
+  if constexpr (TPR > 64) {
+    float* s = lds + (turn & 1) * (TPR / 64);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < TPR / 64; ++k) v += s[k];
+  }
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ unsigned row_umax(unsigned v, float* lds, int& turn) {
+  v = wave_umax(v);
+  if constexpr (TPR > 64) {
+    unsigned* s = (unsigned*)lds + (turn & 1) * (TPR / 64);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int k = 0; k < TPR / 64; ++k) v = max(v, s[k]);
+  }
+  return v;
+}
+
+struct RowArgs {
+  const void *x, *res;
+  const void* w;
+  void *h, *y;
+  float *rstd, *scale;
+  long long ldx, ldr;
+  int M, D, w_f32;
+  float eps;
+};
+
+// NORM = false: y is x itself (the quantisation alone)
+template <int TPR, int NV, int VEC, int XT, int RT, int YT, bool NORM>
+__global__ __launch_bounds__(256) void rms_fwd(const RowArgs p) {
+  constexpr int RPB = 256 / TPR;
+  __shared__ float lds[2 * 4];
+  int turn = 0;
+  const int t = threadIdx.x % TPR;
+  float w[NV][VEC];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * TPR + t) * VEC;
+      if (c < p.D) {
+        if (p.w_f32)
+          load_vec<F32, VEC>(p.w, c, w[v]);
+        else
+          load_vec<T16, VEC>(p.w, c, w[v]);
+      }
+    }
+  }
+  const float inv_d = 1.f / (float)p.D;
+  for (int row = blockIdx.x * RPB + threadIdx.x / TPR; row < p.M; row += gridDim.x * RPB) {
+    float a[NV][VEC];
+    const size_t xo = (size_t)row * p.ldx, ro = (size_t)row * p.ldr, o = (size_t)row * p.D;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * TPR + t) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) a[v][e] = 0.f;
+      if (c < p.D) load_vec<XT, VEC>(p.x, xo + c, a[v]);
+    }
+    if constexpr (RT != NONE) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * TPR + t) * VEC;
+        if (c < p.D) {
+          float r[VEC];
+          load_vec<RT, VEC>(p.res, ro + c, r);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) a[v][e] = as_stored<RT>(a[v][e] + r[e]);
+          store_vec<RT, VEC>(p.h, o + c, a[v]);
+        }
+      }
+    }
+    if constexpr (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) ss += a[v][e] * a[v][e];
+      const float r = rsqrtf(row_sum<TPR>(ss, lds, turn) * inv_d + p.eps);
+      if (p.rstd && t == 0) p.rstd[row] = r;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * TPR + t) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a[v][e] = c < p.D ? a[v][e] * r * w[v][e] : 0.f;
+      }
+    }
+    if constexpr (YT == F8) {
+      // the largest |y| as the largest bit pattern without its sign: a NaN's is above every number's, so that a row with a NaN gets a
+      // NaN as its scale and reads back as NaN (fmaxf would drop it)
+      unsigned m = 0;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(a[v][e]) & 0x7fffffffu);
+      const float amax = __uint_as_float(row_umax<TPR>(m, lds, turn));
+      const float scale = (amax < AMAX_MIN ? AMAX_MIN : amax) / E4M3_MAX, inv = 1.f / scale;
+      if (t == 0) p.scale[row] = scale;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          // y / scale to the last bit by one correction of y * inv (Markstein): 16-bit values quantised by a power-of-two multiple of
+          // 7 lie exactly between two e4m3 values often enough that the last bit shows
+          const float q = a[v][e] * inv;
+          const float c = __builtin_fmaf(__builtin_fmaf(-q, scale, a[v][e]), inv, q);
+          a[v][e] = c;
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * TPR + t) * VEC;
+      if (c < p.D) store_vec<YT, VEC>(p.y, o + c, a[v]);
+    }
+  }
+}
+
+struct BwdArgs {
+  const void *dy, *dh, *h, *w;
+  const float* rstd;
+  void *dx, *dres;
+  float* part;   // [gridDim.x][D]
+  int M, D, w_f32;
+};
+
+// XT: the type of dy and dx; HT: the type of h, dh and dres.  One wave (TPR = 64) or 512 threads a row, 512 threads a block.
+template <int TPR, int NV, int VEC, int XT, int HT>
+__global__ __launch_bounds__(512) void rms_bwd(const BwdArgs p) {
+  constexpr int RPB = 512 / TPR;
+  extern __shared__ float lds[];   // TPR = 64: D floats (the block's sum of d w); 512: 2 * 8 words of the row sums
+  int turn = 0;
+  const int t = threadIdx.x % TPR;
+  float w[NV][VEC], acc[NV][VEC];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * TPR + t) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) w[v][e] = acc[v][e] = 0.f;
+    if (c < p.D) {
+      if (p.w_f32)
+        load_vec<F32, VEC>(p.w, c, w[v]);
+      else
+        load_vec<T16, VEC>(p.w, c, w[v]);
+    }
+  }
+  const float inv_d = 1.f / (float)p.D;
+  for (int row = blockIdx.x * RPB + threadIdx.x / TPR; row < p.M; row += gridDim.x * RPB) {
+    float g[NV][VEC], h[NV][VEC];
+    const size_t o = (size_t)row * p.D;
+    const float r = p.rstd[row];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * TPR + t) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) g[v][e] = h[v][e] = 0.f;
+      if (c < p.D) {
+        load_vec<HT, VEC>(p.h, o + c, h[v]);
+        load_vec<XT, VEC>(p.dy, o + c, g[v]);
+      }
+    }
+    float dot = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        h[v][e] *= r;
+        acc[v][e] += g[v][e] * h[v][e];
+        g[v][e] *= w[v][e];
+        dot += g[v][e] * h[v][e];
+      }
+    const float mean = row_sum<TPR>(dot, lds, turn) * inv_d;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * TPR + t) * VEC;
+      if (c < p.D) {
+        float d[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[e] = 0.f;
+        if (p.dh) load_vec<HT, VEC>(p.dh, o + c, d);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[e] += r * (g[v][e] - h[v][e] * mean);
+        if (p.dx) store_vec<XT, VEC>(p.dx, o + c, d);
+        if (p.dres) store_vec<HT, VEC>(p.dres, o + c, d);
+      }
+    }
+  }
+  if (!p.part) return;
+  float* out = p.part + (size_t)blockIdx.x * p.D;
+  if constexpr (TPR == 64) {
+    for (int c = threadIdx.x; c < p.D; c += 512) lds[c] = 0.f;
+    __syncthreads();
+    for (int k = 0; k < 8; ++k) {   // wave after wave: a fixed order
+      if ((int)(threadIdx.x >> 6) == k) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c = (v * TPR + t) * VEC;
+          if (c < p.D)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) lds[c + e] += acc[v][e];
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < p.D; c += 512) out[c] = lds[c];
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * TPR + t) * VEC;
+      if (c < p.D) store_vec<F32, VEC>(out, c, acc[v]);
+    }
+  }
+}
+
+// out[c] = sum over the parts, in order within 8 interleaved groups, then over the groups: 32 columns x 8 groups a block
+__global__ __launch_bounds__(256) void sum_parts(const float* part, void* out, int parts, int D, int out_f32) {
+  __shared__ float lds[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+  float s = 0.f;
+  if (c < D) {
+#pragma unroll 8
+    for (int k = g; k < parts; k += 8) s += part[(size_t)k * D + c];
+  }
+  lds[g][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (g == 0 && c < D) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += lds[k][threadIdx.x];
+    if (out_f32)
+      ((float*)out)[c] = s;
+    else
+      ((bf16_t*)out)[c] = f2bf(s);
+  }
+}
+
+constexpr int MAX_D = 16384;
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <int TPR, int NV, int VEC, int XT, int RT, int YT, bool NORM>
+int launch_fwd(const RowArgs& a, hipStream_t s) {
+  const int rpb = 256 / TPR;
+  const long long need = ((long long)a.M + rpb - 1) / rpb, most = (long long)mvit_num_cus() * 8;
+  hipLaunchKernelGGL((rms_fwd<TPR, NV, VEC, XT, RT, YT, NORM>), dim3((unsigned)(need < most ? need : most)), dim3(256), 0, s, a);
+  return MVIT_LAUNCH_CHECK();
+}
+
+template <int XT, int RT, int YT, bool NORM>
+int fwd_layout(const RowArgs& a, bool vec, hipStream_t s) {
+  const int D = a.D;
+  if (vec) {
+    if (D <= 4096 && a.M >= 4 * mvit_num_cus()) {
+      if (D <= 512) return launch_fwd<64, 1, 8, XT, RT, YT, NORM>(a, s);
+      if (D <= 1024) return launch_fwd<64, 2, 8, XT, RT, YT, NORM>(a, s);
+      if (D <= 1536) return launch_fwd<64, 3, 8, XT, RT, YT, NORM>(a, s);
+      if (D <= 2048) return launch_fwd<64, 4, 8, XT, RT, YT, NORM>(a, s);
+      return launch_fwd<64, 8, 8, XT, RT, YT, NORM>(a, s);
+    }
+    if (D <= 2048) return launch_fwd<256, 1, 8, XT, RT, YT, NORM>(a, s);
+    if (D <= 4096) return launch_fwd<256, 2, 8, XT, RT, YT, NORM>(a, s);
+    if (D <= 8192) return launch_fwd<256, 4, 8, XT, RT, YT, NORM>(a, s);
+    return launch_fwd<256, 8, 8, XT, RT, YT, NORM>(a, s);
+  }
+  if (D <= 512) return launch_fwd<64, 8, 1, XT, RT, YT, NORM>(a, s);
+  if (D <= 1024) return launch_fwd<64, 16, 1, XT, RT, YT, NORM>(a, s);
+  if (D <= 4096) return launch_fwd<256, 16, 1, XT, RT, YT, NORM>(a, s);
+  return launch_fwd<256, 64, 1, XT, RT, YT, NORM>(a, s);
+}
+
+// vector loads: every row of every operand starts on 16 bytes (8 for the e4m3 output, whose rows are D bytes)
+bool vec_ok(const RowArgs& a) {
+  return a.D % 8 == 0 && a.ldx % 8 == 0 && (!a.res || a.ldr % 8 == 0) && aligned16(a.x) && aligned16(a.res) && aligned16(a.h) && aligned16(a.y) &&
+         aligned16(a.w);
+}
+
+// (an empty tensor has no address: pointers are asked for where there are rows)
+bool rows_bad(const RowArgs& a) {
+  if (a.M < 0 || a.D <= 0 || a.D > MAX_D) return true;
+  return a.M > 0 && (!a.x || !a.y || a.ldx < a.D || (a.res && (!a.h || a.ldr < a.D)));
+}
+
+template <int TPR, int NV, int VEC, int XT, int HT>
+int launch_bwd(const BwdArgs& a, int grid, hipStream_t s) {
+  const size_t lds = TPR == 64 ? (size_t)a.D * 4 : 64;
+  hipLaunchKernelGGL((rms_bwd<TPR, NV, VEC, XT, HT>), dim3(grid), dim3(512), lds, s, a);
+  return MVIT_LAUNCH_CHECK();
+}
+
+template <int XT, int HT>
+int bwd_layout(const BwdArgs& a, bool vec, int grid, hipStream_t s) {
+  const int D = a.D;
+  if (vec) {
+    if (D <= 512) return launch_bwd<64, 1, 8, XT, HT>(a, grid, s);
+    if (D <= 1024) return launch_bwd<64, 2, 8, XT, HT>(a, grid, s);
+    if (D <= 1536) return launch_bwd<64, 3, 8, XT, HT>(a, grid, s);
+    if (D <= 2048) return launch_bwd<64, 4, 8, XT, HT>(a, grid, s);
+    if (D <= 4096) return launch_bwd<512, 1, 8, XT, HT>(a, grid, s);
+    if (D <= 8192) return launch_bwd<512, 2, 8, XT, HT>(a, grid, s);
+    return launch_bwd<512, 4, 8, XT, HT>(a, grid, s);
+  }
+  if (D <= 512) return launch_bwd<64, 8, 1, XT, HT>(a, grid, s);
+  if (D <= 1024) return launch_bwd<64, 16, 1, XT, HT>(a, grid, s);
+  if (D <= 4096) return launch_bwd<512, 8, 1, XT, HT>(a, grid, s);
+  return launch_bwd<512, 32, 1, XT, HT>(a, grid, s);
+}
+
+// blocks of the backward pass, which is also the number of partial sums of d w: two blocks of 512 threads a CU, no more than there are
+// rows for (8 rows a block where a wave has a row: D <= 2048 by vectors, D <= 1024 by elements; the smaller bound counts for both)
+int bwd_blocks(int M, int D) {
+  const long long rows = D <= 2048 ? 8 : 1, need = ((long long)M + rows - 1) / rows, most = (long long)mvit_num_cus() * 2;
+  return (int)(need < most ? need : most);
+}
+
+}  // namespace
+
+extern "C" MVIT_API int mvit_rmsnorm_fwd(const void* x, int x_f32, long long ldx, const void* res, int res_f32, long long ldr, const void* w,
+                                         int w_f32, void* h, void* y, int y_f32, float* rstd, int M, int D, float eps, mvit_stream_t stream) {
+  MVIT_CLEAR_ERROR();
+  const RowArgs a = {x, res, w, h, y, rstd, nullptr, ldx, ldr, M, D, w_f32, eps};
+  if (rows_bad(a) || !w || (!x_f32 && y_f32) || (x_f32 && res && !res_f32)) return MVIT_EINVAL;
+  if (M == 0) return MVIT_OK;
+  const bool v = vec_ok(a);
+  hipStream_t s = (hipStream_t)stream;
+  if (!x_f32) {
+    if (!res) return fwd_layout<T16, NONE, T16, true>(a, v, s);
+    return res_f32 ? fwd_layout<T16, F32, T16, true>(a, v, s) : fwd_layout<T16, T16, T16, true>(a, v, s);
+  }
+  if (!res) return y_f32 ? fwd_layout<F32, NONE, F32, true>(a, v, s) : fwd_layout<F32, NONE, T16, true>(a, v, s);
+  return y_f32 ? fwd_layout<F32, F32, F32, true>(a, v, s) : fwd_layout<F32, F32, T16, true>(a, v, s);
+}
+
+extern "C" MVIT_API int mvit_rmsnorm_fp8_fwd(const void* x, int x_f32, long long ldx, const void* res, int res_f32, long long ldr,
+                                             const void* w, int w_f32, void* h, void* q, float* scale, int M, int D, float eps,
+                                             mvit_stream_t stream) {
+  MVIT_CLEAR_ERROR();
+  const RowArgs a = {x, res, w, h, q, nullptr, scale, ldx, ldr, M, D, w_f32, eps};
+  if (rows_bad(a) || !w || (M > 0 && !scale) || (x_f32 && res && !res_f32)) return MVIT_EINVAL;
+  if (M == 0) return MVIT_OK;
+  const bool v = vec_ok(a);
+  hipStream_t s = (hipStream_t)stream;
+  if (!x_f32) {
+    if (!res) return fwd_layout<T16, NONE, F8, true>(a, v, s);
+    return res_f32 ? fwd_layout<T16, F32, F8, true>(a, v, s) : fwd_layout<T16, T16, F8, true>(a, v, s);
+  }
+  return res ? fwd_layout<F32, F32, F8, true>(a, v, s) : fwd_layout<F32, NONE, F8, true>(a, v, s);
+}
+
+extern "C" MVIT_API int mvit_quantize_rows_fp8(const void* x, int x_f32, long long ldx, void* q, float* scale, int M, int D,
+                                               mvit_stream_t stream) {
+  MVIT_CLEAR_ERROR();
+  const RowArgs a = {x, nullptr, nullptr, nullptr, q, nullptr, scale, ldx, 0, M, D, 0, 0.f};
+  if (rows_bad(a) || (M > 0 && !scale)) return MVIT_EINVAL;
+  if (M == 0) return MVIT_OK;
+  const bool v = vec_ok(a);
+  return x_f32 ? fwd_layout<F32, NONE, F8, false>(a, v, (hipStream_t)stream) : fwd_layout<T16, NONE, F8, false>(a, v, (hipStream_t)stream);
+}
+
+extern "C" MVIT_API long long mvit_rmsnorm_bwd_scratch_bytes(int M, int D) {
+  return M <= 0 || D <= 0 ? 0 : (long long)bwd_blocks(M, D) * D * 4;
+}
+
+extern "C" MVIT_API int mvit_rmsnorm_bwd(const void* dy, int x_f32, const void* dh, const void* h, int h_f32, const void* w, int w_f32,
+                                         const float* rstd, void* dx, void* dres, void* dw, void* scratch, long long scratch_bytes, int M,
+                                         int D, mvit_stream_t stream) {
+  MVIT_CLEAR_ERROR();
+  if (M < 0 || D <= 0 || D > MAX_D || !w || (M > 0 && (!dy || !h || !rstd)) || (x_f32 && !h_f32)) return MVIT_EINVAL;
+  if (dw && M > 0 && (!scratch || scratch_bytes < mvit_rmsnorm_bwd_scratch_bytes(M, D))) return MVIT_EINVAL;
+  hipStream_t s = (hipStream_t)stream;
+  const int grid = M > 0 ? bwd_blocks(M, D) : 0;
+  if (M > 0) {
+    const BwdArgs a = {dy, dh, h, w, rstd, dx, dres, dw ? (float*)scratch : nullptr, M, D, w_f32};
+    const bool v = D % 8 == 0 && aligned16(dy) && aligned16(dh) && aligned16(h) && aligned16(w) && aligned16(dx) && aligned16(dres) && aligned16(scratch);
+    int rc;
+    if (x_f32)
+      rc = bwd_layout<F32, F32>(a, v, grid, s);
+    else
+      rc = h_f32 ? bwd_layout<T16, F32>(a, v, grid, s) : bwd_layout<T16, T16>(a, v, grid, s);
+    if (rc) return rc;
+  }
+  if (dw) {
+    hipLaunchKernelGGL(sum_parts, dim3((D + 31) / 32), dim3(256), 0, s, (const float*)scratch, dw, grid, D, w_f32);
+    return MVIT_LAUNCH_CHECK();
+  }
+  return MVIT_OK;
+}

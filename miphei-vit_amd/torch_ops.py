@@ -247,4 +247,9 @@ def _wmse_bwd(ctx, grad_loss, _grad_d):
 
 weighted_mse_forward.register_autograd(_wmse_bwd, setup_context=_wmse_setup)
 
-__all__ = ["linear", "layer_norm", "attention", "weighted_mse"]
+# ------------------------------------------------------------------ the further operators of a transformer block
+from .block_ops import (add_rms_norm, add_rms_norm_fp8, grid_positions, linear_act, linear_fp8, quantize_fp8, rms_norm, rms_norm_fp8, rotary, rotary_,  # noqa: E402
+                        rotary_frequencies)
+
+__all__ = ["linear", "layer_norm", "attention", "weighted_mse", "rms_norm", "add_rms_norm", "rms_norm_fp8", "add_rms_norm_fp8", "quantize_fp8",
+           "rotary", "rotary_", "rotary_frequencies", "grid_positions", "linear_act", "linear_fp8"]
