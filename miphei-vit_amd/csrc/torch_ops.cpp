@@ -1,0 +1,721 @@
+// torch.ops.mvit.*: the transformer-block operators (RMS norm, row quantisation, rotary positions, linear with activation and residual)
+// on the C-ABI of miphei_hip.h -- argument checks, output allocation, autograd formulas and the choice of library, in C++.
+//
+// Why C++ here: the calls on one token take the GPU 4 to 8 us, and the same host work in Python (checks, allocations, ctypes) took
+// 18 to 22 us a call and 190 us for a forward and backward, 60 of them Python run by autograd's device thread.
+//
+// Conventions: the work goes to the tensors' device, on its current stream; 16-bit operands are bf16 (libmiphei_hip.so) or fp16
+// (libmiphei_hip_f16.so, the same sources), never a mixture; scratch memory comes from torch's allocator on the same stream, so that a
+// captured graph owns its own.  Wrong arguments raise ValueError in the GPU and in the meta (shape) implementation alike.
+#include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <dlfcn.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <array>
+#include <optional>
+#include <string>
+
+#include "../../include/miphei_hip.h"
+
+namespace {
+
+using at::ScalarType;
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// ---------------------------------------------------------------- the two libraries
+struct Lib {
+#define MVIT_FN(name) decltype(&::name) name = nullptr
+  MVIT_FN(mvit_rmsnorm_fwd);
+  MVIT_FN(mvit_rmsnorm_fp8_fwd);
+  MVIT_FN(mvit_quantize_rows_fp8);
+  MVIT_FN(mvit_rmsnorm_bwd_scratch_bytes);
+  MVIT_FN(mvit_rmsnorm_bwd);
+  MVIT_FN(mvit_rotary);
+  MVIT_FN(mvit_linear_act);
+  MVIT_FN(mvit_linear_fp8);
+  MVIT_FN(mvit_act_bwd_scratch_bytes);
+  MVIT_FN(mvit_act_bwd);
+  MVIT_FN(mvit_transpose_bf16);
+#undef MVIT_FN
+};
+std::array<Lib, 2> libs;   // [0] bf16, [1] fp16: filled by mvit_torch_bind before the first call
+bool bound = false;
+
+const Lib& lib(bool f16) {
+  TORCH_CHECK(bound, "libmiphei_hip.so is not bound: import miphei_vit_amd.torch_ops");
+  return libs[f16];
+}
+
+void ok(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
+
+// ---------------------------------------------------------------- checks
+#define REQUIRE(cond, op, ...) TORCH_CHECK_VALUE(cond, "mvit::", op, ": ", ##__VA_ARGS__)
+
+bool is_half(ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+// The one 16-bit type among the operands; a mixture is refused, and so is any type but bf16, fp16 and f32
+struct HalfType {
+  const char* op;
+  std::optional<ScalarType> t;
+  void add(ScalarType d) {
+    if (d == at::kFloat) return;
+    REQUIRE(is_half(d), op, "operands are bfloat16, float16 or float32, got ", d);
+    REQUIRE(!t || *t == d, op, "bfloat16 and float16 operands in one call");
+    t = d;
+  }
+  void add(const OptTensor& x) {
+    if (x) add(x->scalar_type());
+  }
+  bool f16() const { return t && *t == at::kHalf; }
+};
+
+void same_place(const char* op, const Tensor& x, const OptTensor& y) {
+  REQUIRE(!y || y->device() == x.device(), op, "tensors on ", x.device(), " and ", y->device());
+}
+
+void no_grad(const char* op, std::initializer_list<OptTensor> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const auto& t : ts)
+    TORCH_CHECK(!t || !t->requires_grad(), "mvit::", op, " has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+
+constexpr int64_t ROWS_MAX = 0x7fffffff;
+
+// ---------------------------------------------------------------- tensors as the kernels take them
+// [rows, last] view whose rows are dense, any row stride of at least their length; a copy only where there is none
+Tensor rows(const Tensor& t) {
+  const int64_t d = t.size(-1);
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, d});
+  if ((d > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < d)) r = r.contiguous();
+  return r;
+}
+int64_t ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }   // (the stride of a single row says nothing)
+
+// the same for the matrix kernels: rows start on 16 bytes and are at most 2^23 bytes apart
+Tensor operand(const Tensor& t) {
+  Tensor r = rows(t);
+  const int64_t es = r.element_size(), step = r.size(0) > 1 ? r.stride(0) * es : 0;
+  if (reinterpret_cast<uintptr_t>(r.const_data_ptr()) % 16 || step % 16 || step > (1 << 23)) r = r.clone(at::MemoryFormat::Contiguous);
+  return r;
+}
+
+const void* ptr(const OptTensor& t) { return t ? t->const_data_ptr() : nullptr; }
+int f32(const OptTensor& t) { return t && t->scalar_type() == at::kFloat; }
+void* stream(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
+Tensor scratch(const Tensor& x, int64_t bytes) { return at::empty({bytes}, x.options().dtype(at::kByte)); }
+Tensor none(const Tensor& x, ScalarType t) { return at::empty({0}, x.options().dtype(t)); }
+
+std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
+  auto s = x.sizes().vec();
+  s.back() = n;
+  return s;
+}
+
+// ================================================================ RMS norm
+HalfType norm_check(const char* op, const Tensor& x, const OptTensor& residual, const Tensor& weight, std::optional<ScalarType> out) {
+  REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, op, "the last dimension must be 1 .. 16384");
+  const int64_t d = x.size(-1);
+  REQUIRE(x.numel() / d <= ROWS_MAX, op, "more than 2^31 - 1 rows");
+  REQUIRE(weight.dim() == 1 && weight.size(0) == d, op, "weight ", weight.sizes(), " does not match input ", x.sizes());
+  REQUIRE(!residual || residual->sizes() == x.sizes(), op, "residual ", residual->sizes(), " and input ", x.sizes(), " differ (it is not broadcast)");
+  same_place(op, x, residual);
+  same_place(op, x, weight);
+  HalfType h{op};
+  h.add(x), h.add(residual), h.add(weight);
+  if (out) h.add(*out);
+  const bool xf = x.scalar_type() == at::kFloat;
+  REQUIRE(!xf || !residual || f32(residual), op, "a float32 input needs a float32 residual");
+  REQUIRE(!out || *out == x.scalar_type() || xf, op, "out_dtype ", *out, " of a ", x.scalar_type(), " input");
+  return h;
+}
+
+struct NormOut {
+  Tensor y, h, row;   // row: one f32 a row (rstd, scale)
+};
+NormOut norm_out(const Tensor& x, const OptTensor& residual, ScalarType y) {
+  return {at::empty(x.sizes(), x.options().dtype(y)), residual ? at::empty(x.sizes(), x.options().dtype(residual->scalar_type())) : none(x, x.scalar_type()),
+          at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat))};
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps,
+                                                    std::optional<ScalarType> out_dtype) {
+  const HalfType h = norm_check("rms_norm", x, residual, weight, out_dtype);
+  c10::DeviceGuard guard(x.device());
+  NormOut o = norm_out(x, residual, out_dtype.value_or(x.scalar_type()));
+  const Tensor x2 = rows(x), w = weight.contiguous();
+  const OptTensor r2 = residual ? OptTensor(rows(*residual)) : std::nullopt;
+  ok(lib(h.f16()).mvit_rmsnorm_fwd(x2.const_data_ptr(), f32(x2), ld(x2), ptr(r2), f32(r2), r2 ? ld(*r2) : 0, w.const_data_ptr(), f32(w),
+                                   residual ? o.h.mutable_data_ptr() : nullptr, o.y.mutable_data_ptr(), f32(o.y), o.row.mutable_data_ptr<float>(),
+                                   (int)x2.size(0), (int)x2.size(1), (float)eps, stream(x)),
+     "mvit_rmsnorm_fwd");
+  return {o.y, o.h, o.row};
+}
+std::tuple<Tensor, Tensor, Tensor> rms_norm_forward_meta(const Tensor& x, const OptTensor& residual, const Tensor& weight, double,
+                                                         std::optional<ScalarType> out_dtype) {
+  norm_check("rms_norm", x, residual, weight, out_dtype);
+  NormOut o = norm_out(x, residual, out_dtype.value_or(x.scalar_type()));
+  return {o.y, o.h, o.row};
+}
+
+// (dx, dresidual, dweight), empty where not wanted; where x and the stream have one type the two gradients are one tensor, dx
+struct NormBwd {
+  Tensor dx, dres, dw;
+  bool x, res;
+};
+NormBwd norm_bwd_out(const Tensor& h, const Tensor& weight, ScalarType x_dtype, bool need_x, bool need_residual, bool need_weight) {
+  const bool one = x_dtype == h.scalar_type(), x = need_x || (one && need_residual), res = need_residual && !one;
+  return {x ? at::empty(h.sizes(), h.options().dtype(x_dtype)) : none(h, x_dtype), res ? at::empty(h.sizes(), h.options()) : none(h, h.scalar_type()),
+          need_weight ? at::empty_like(weight, at::MemoryFormat::Contiguous) : none(weight, weight.scalar_type()), x, res};
+}
+std::tuple<Tensor, Tensor, Tensor> rms_norm_backward(const Tensor& dy, const OptTensor& dh, const Tensor& h, const Tensor& weight, const Tensor& rstd,
+                                                     ScalarType x_dtype, bool need_x, bool need_residual, bool need_weight) {
+  c10::DeviceGuard guard(h.device());
+  NormBwd o = norm_bwd_out(h, weight, x_dtype, need_x, need_residual, need_weight);
+  const int64_t d = h.size(-1), m = h.numel() / d;
+  // the kernel's dx has dy's type: the gradient of a 16-bit output of an f32 x is widened first
+  const Tensor h2 = h.contiguous(), dy2 = dy.to(x_dtype).contiguous(), w = weight.contiguous();
+  const OptTensor dh2 = dh ? OptTensor(dh->to(h.scalar_type()).contiguous()) : std::nullopt;
+  HalfType half{"rms_norm"};
+  half.add(dy2), half.add(h2), half.add(w);
+  const Lib& l = lib(half.f16());
+  const long long bytes = need_weight ? l.mvit_rmsnorm_bwd_scratch_bytes((int)m, (int)d) : 0;
+  const Tensor s = scratch(h, bytes);
+  ok(l.mvit_rmsnorm_bwd(dy2.const_data_ptr(), f32(dy2), ptr(dh2), h2.const_data_ptr(), f32(h2), w.const_data_ptr(), f32(w), rstd.const_data_ptr<float>(),
+                        o.x ? o.dx.mutable_data_ptr() : nullptr, o.res ? o.dres.mutable_data_ptr() : nullptr,
+                        need_weight ? o.dw.mutable_data_ptr() : nullptr, bytes ? s.mutable_data_ptr() : nullptr, bytes, (int)m, (int)d, stream(h)),
+     "mvit_rmsnorm_bwd");
+  return {o.dx, o.dres, o.dw};
+}
+std::tuple<Tensor, Tensor, Tensor> rms_norm_backward_meta(const Tensor&, const OptTensor&, const Tensor& h, const Tensor& weight, const Tensor&,
+                                                          ScalarType x_dtype, bool need_x, bool need_residual, bool need_weight) {
+  NormBwd o = norm_bwd_out(h, weight, x_dtype, need_x, need_residual, need_weight);
+  return {o.dx, o.dres, o.dw};
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps) {
+  no_grad("rms_norm_fp8", {x, residual, weight});
+  const HalfType h = norm_check("rms_norm_fp8", x, residual, weight, std::nullopt);
+  c10::DeviceGuard guard(x.device());
+  NormOut o = norm_out(x, residual, at::kFloat8_e4m3fn);
+  const Tensor x2 = rows(x), w = weight.contiguous();
+  const OptTensor r2 = residual ? OptTensor(rows(*residual)) : std::nullopt;
+  ok(lib(h.f16()).mvit_rmsnorm_fp8_fwd(x2.const_data_ptr(), f32(x2), ld(x2), ptr(r2), f32(r2), r2 ? ld(*r2) : 0, w.const_data_ptr(), f32(w),
+                                       residual ? o.h.mutable_data_ptr() : nullptr, o.y.mutable_data_ptr(), o.row.mutable_data_ptr<float>(),
+                                       (int)x2.size(0), (int)x2.size(1), (float)eps, stream(x)),
+     "mvit_rmsnorm_fp8_fwd");
+  return {o.y, o.row, o.h};
+}
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8_meta(const Tensor& x, const OptTensor& residual, const Tensor& weight, double) {
+  norm_check("rms_norm_fp8", x, residual, weight, std::nullopt);
+  NormOut o = norm_out(x, residual, at::kFloat8_e4m3fn);
+  return {o.y, o.row, o.h};
+}
+
+HalfType quantize_check(const Tensor& x) {
+  REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "quantize_fp8", "the last dimension must be 1 .. 16384");
+  REQUIRE(x.numel() / x.size(-1) <= ROWS_MAX, "quantize_fp8", "more than 2^31 - 1 rows");
+  HalfType h{"quantize_fp8"};
+  h.add(x);
+  return h;
+}
+std::tuple<Tensor, Tensor> quantize_fp8(const Tensor& x) {
+  no_grad("quantize_fp8", {x});
+  const HalfType h = quantize_check(x);
+  c10::DeviceGuard guard(x.device());
+  NormOut o = norm_out(x, std::nullopt, at::kFloat8_e4m3fn);
+  const Tensor x2 = rows(x);
+  ok(lib(h.f16()).mvit_quantize_rows_fp8(x2.const_data_ptr(), f32(x2), ld(x2), o.y.mutable_data_ptr(), o.row.mutable_data_ptr<float>(),
+                                         (int)x2.size(0), (int)x2.size(1), stream(x)),
+     "mvit_quantize_rows_fp8");
+  return {o.y, o.row};
+}
+std::tuple<Tensor, Tensor> quantize_fp8_meta(const Tensor& x) {
+  quantize_check(x);
+  NormOut o = norm_out(x, std::nullopt, at::kFloat8_e4m3fn);
+  return {o.y, o.row};
+}
+
+// ================================================================ rotary positions
+HalfType rotary_check(const char* op, const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
+                      int64_t num_prefix) {
+  REQUIRE(x.dim() == 4, op, "x must be [B, N, heads, head_dim], got ", x.sizes());
+  const int64_t B = x.size(0), N = x.size(1), H = x.size(2), Dh = x.size(3), axes = (int64_t)sections.size();
+  REQUIRE(Dh % 2 == 0 && Dh >= 2 && Dh <= 1024 && H >= 1 && H <= 1024 && B <= 65535 && N <= ROWS_MAX, op,
+          "head_dim must be even and at most 1024, heads 1 .. 1024, batch at most 65535");
+  int64_t pairs = 0;
+  bool good = axes >= 1 && axes <= 4;
+  for (const int64_t s : sections) good = good && s >= 0 && s <= Dh, pairs += good ? s : 0;
+  REQUIRE(good && pairs >= 1 && pairs <= Dh / 2, op, "sections ", sections, ": 1 to 4 axes, together 1 .. head_dim / 2 pairs");
+  REQUIRE(rotate_heads >= 0 && rotate_heads <= H && num_prefix >= 0 && num_prefix <= N, op, "rotate_heads ", rotate_heads, " of ", H, ", num_prefix ",
+          num_prefix, " of ", N);
+  const int64_t want[3] = {B, N - num_prefix, axes};
+  REQUIRE(positions.sizes() == at::IntArrayRef(want + 1, 2) || positions.sizes() == at::IntArrayRef(want, 3), op, "positions must be ",
+          at::IntArrayRef(want + 1, 2), " or ", at::IntArrayRef(want, 3), ", got ", positions.sizes());
+  const ScalarType pt = positions.scalar_type(), ft = inv_freq.scalar_type();
+  REQUIRE(pt == at::kInt || pt == at::kLong || pt == at::kFloat, op, "positions are int32, int64 or float32, got ", pt);
+  REQUIRE(inv_freq.dim() == 1 && inv_freq.size(0) == pairs && (ft == at::kFloat || ft == at::kDouble), op, "inv_freq must be float32 or float64 [", pairs,
+          "], got ", ft, " ", inv_freq.sizes());
+  same_place(op, x, positions);
+  same_place(op, x, inv_freq);
+  HalfType h{op};
+  h.add(x);
+  return h;
+}
+
+void rotary_into(const HalfType& half, const Tensor& x, const Tensor& y, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections,
+                 int64_t rotate_heads, int64_t num_prefix, bool interleaved, bool inverse) {
+  if (x.numel() == 0) return;
+  const Tensor pos = positions.contiguous(), freq = inv_freq.contiguous();
+  mvit_rotary_args a = {};
+  a.x = x.const_data_ptr(), a.y = y.mutable_data_ptr(), a.positions = pos.const_data_ptr(), a.inv_freq = freq.const_data_ptr();
+  a.xb = x.stride(0), a.xn = x.stride(1), a.xh = x.stride(2), a.yb = y.stride(0), a.yn = y.stride(1), a.yh = y.stride(2);
+  a.pos_b = pos.dim() == 3 ? pos.stride(0) : 0;
+  a.B = (int)x.size(0), a.N = (int)x.size(1), a.H = (int)x.size(2), a.Dh = (int)x.size(3);
+  a.rotate_heads = (int)rotate_heads, a.prefix = (int)num_prefix, a.axes = (int)sections.size();
+  for (size_t i = 0; i < sections.size(); ++i) a.sections[i] = (int)sections[i];
+  const ScalarType pt = pos.scalar_type();
+  a.x_f32 = f32(x), a.pos_type = pt == at::kInt ? 0 : pt == at::kLong ? 1 : 2, a.freq_f64 = freq.scalar_type() == at::kDouble;
+  a.interleaved = interleaved, a.inverse = inverse;
+  ok(lib(half.f16()).mvit_rotary(&a, stream(x)), "mvit_rotary");
+}
+
+Tensor rotary_forward(const Tensor& x0, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
+                      int64_t num_prefix, bool interleaved, bool inverse) {
+  const HalfType h = rotary_check("rotary", x0, positions, inv_freq, sections, rotate_heads, num_prefix);
+  c10::DeviceGuard guard(x0.device());
+  const Tensor x = x0.stride(3) == 1 ? x0 : x0.contiguous();
+  Tensor y = at::empty_like(x);
+  rotary_into(h, x, y, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
+  return y;
+}
+Tensor rotary_forward_meta(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
+                           int64_t num_prefix, bool, bool) {
+  rotary_check("rotary", x, positions, inv_freq, sections, rotate_heads, num_prefix);
+  return at::empty_like(x.stride(3) == 1 ? x : x.contiguous());
+}
+
+Tensor& rotary_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix,
+                bool interleaved) {
+  no_grad("rotary_", {x});
+  const HalfType h = rotary_check("rotary_", x, positions, inv_freq, sections, rotate_heads, num_prefix);
+  bool dense = x.stride(3) == 1;
+  for (int64_t i = 0; i < 4; ++i) dense = dense && (x.stride(i) != 0 || x.size(i) == 1);
+  REQUIRE(dense, "rotary_", "x must have dense heads and no expanded dimension to be turned in place");
+  c10::DeviceGuard guard(x.device());
+  rotary_into(h, x, x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, false);
+  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+  return x;
+}
+Tensor& rotary_meta_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix, bool) {
+  rotary_check("rotary_", x, positions, inv_freq, sections, rotate_heads, num_prefix);
+  return x;
+}
+
+// ================================================================ linear
+int activation(const char* op, c10::string_view a) {
+  static constexpr std::pair<const char*, int> names[] = {
+      {"none", MVIT_ACT_NONE}, {"relu", MVIT_ACT_RELU}, {"silu", MVIT_ACT_SILU}, {"gelu", MVIT_ACT_GELU}, {"gelu_tanh", MVIT_ACT_GELU_TANH}};
+  for (const auto& [name, code] : names)
+    if (a == name) return code;
+  REQUIRE(false, op, "activation '", std::string(a), "': one of none, relu, silu, gelu, gelu_tanh");
+}
+
+int linear_check(const char* op, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, c10::string_view act,
+                 int64_t multiple) {
+  REQUIRE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(1) % multiple == 0 && weight.numel() > 0, op, "weight ",
+          weight.sizes(), " does not match input ", x.sizes(), " (K must be a multiple of ", multiple, ")");
+  const int64_t K = weight.size(1), N = weight.size(0);
+  REQUIRE(K * (int64_t)weight.element_size() <= (1 << 23) && N <= ROWS_MAX && x.numel() / K <= ROWS_MAX, op,
+          "K is at most 2^23 bytes, N and the rows of x at most 2^31 - 1");
+  const int code = activation(op, act);
+  REQUIRE(!bias || (bias->dim() == 1 && bias->size(0) == N), op, "bias ", bias->sizes(), ", expected [", N, "]");
+  REQUIRE(!residual || residual->sizes() == at::IntArrayRef(with_last(x, N)), op, "residual ", residual->sizes(), ", expected ", with_last(x, N),
+          " (it is not broadcast)");
+  same_place(op, x, weight);
+  same_place(op, x, bias);
+  same_place(op, x, residual);
+  return code;
+}
+HalfType linear_half(const char* op, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual) {
+  REQUIRE(is_half(x.scalar_type()) && weight.scalar_type() == x.scalar_type(), op, "x and weight are both bfloat16 or both float16, got ",
+          x.scalar_type(), " and ", weight.scalar_type());
+  HalfType h{op};
+  h.add(x), h.add(bias), h.add(residual);
+  return h;
+}
+
+// y = res + act(x w^T + b) of [M, K] and [N, K] operands that operand() made fit
+void product(const Lib& l, const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& res, const Tensor& y, void* pre, int act,
+             const float* xs, const float* ws, int64_t M, int64_t N, void* st) {
+  mvit_linear_args a = {};
+  a.x = x.const_data_ptr(), a.w = w.const_data_ptr(), a.bias = ptr(bias), a.res = ptr(res), a.y = y.mutable_data_ptr(), a.pre = pre;
+  a.x_scale = xs, a.w_scale = ws, a.ldx = ld(x), a.ldw = ld(w), a.ldr = res ? ld(*res) : 0;
+  a.M = (int)M, a.N = (int)N, a.K = (int)x.size(1), a.act = act, a.bias_f32 = f32(bias), a.y_f32 = f32(y);
+  if (xs)
+    ok(l.mvit_linear_fp8(&a, st), "mvit_linear_fp8");
+  else
+    ok(l.mvit_linear_act(&a, st), "mvit_linear_act");
+}
+
+Tensor linear_out(const Tensor& x, const Tensor& weight, const OptTensor& residual, ScalarType t) {
+  return at::empty(with_last(x, weight.size(0)), x.options().dtype(residual ? residual->scalar_type() : t));
+}
+
+std::tuple<Tensor, Tensor> linear_act_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                                              c10::string_view act, bool save_pre) {
+  const int code = linear_check("linear_act", x, weight, bias, residual, act, 8);
+  const HalfType h = linear_half("linear_act", x, weight, bias, residual);
+  c10::DeviceGuard guard(x.device());
+  Tensor y = linear_out(x, weight, residual, x.scalar_type());
+  Tensor pre = save_pre ? at::empty(y.sizes(), x.options()) : none(x, x.scalar_type());
+  if (y.numel())
+    product(lib(h.f16()), operand(x), operand(weight), bias ? OptTensor(bias->contiguous()) : std::nullopt,
+            residual ? OptTensor(rows(*residual)) : std::nullopt, y, save_pre ? pre.mutable_data_ptr() : nullptr, code, nullptr, nullptr,
+            x.numel() / x.size(-1), weight.size(0), stream(x));
+  return {y, pre};
+}
+std::tuple<Tensor, Tensor> linear_act_forward_meta(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                                                   c10::string_view act, bool save_pre) {
+  linear_check("linear_act", x, weight, bias, residual, act, 8);
+  linear_half("linear_act", x, weight, bias, residual);
+  Tensor y = linear_out(x, weight, residual, x.scalar_type());
+  return {y, save_pre ? at::empty(y.sizes(), x.options()) : none(x, x.scalar_type())};
+}
+
+// t^T with its rows padded by zeros to whole 16-byte pieces: an operand whose K axis is t's rows
+Tensor transposed(const Lib& l, const Tensor& t, void* st) {
+  const int64_t r = t.size(0), c = t.size(1), pad = (r + 7) / 8 * 8;
+  Tensor out = pad == r ? at::empty({c, r}, t.options()) : at::zeros({c, pad}, t.options());
+  ok(l.mvit_transpose_bf16(t.const_data_ptr(), out.mutable_data_ptr(), (int)r, (int)c, (int)ld(t), pad, st), "mvit_transpose_bf16");
+  return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& pre, c10::string_view act,
+                                                       bool need_x, bool need_w, bool need_b, ScalarType bias_dtype) {
+  const int code = activation("linear_act", act);
+  c10::DeviceGuard guard(x.device());
+  const ScalarType t = x.scalar_type();
+  const int64_t N = weight.size(0), K = weight.size(1), M = x.numel() / K;
+  Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : none(x, t);
+  Tensor dw = need_w ? at::empty({N, K}, x.options()) : none(x, t);
+  Tensor db = need_b ? at::empty({N}, x.options().dtype(bias_dtype)) : none(x, bias_dtype);
+  if (M == 0) return {dx, dw.zero_(), db.zero_()};
+  const Lib& l = lib(t == at::kHalf);
+  void* st = stream(x);
+  const Tensor dy2 = dy.reshape({M, N}).contiguous();
+  Tensor dz = dy2;
+  const bool products = need_x || need_w, rounded = code != MVIT_ACT_NONE || dy2.scalar_type() != t;
+  if ((products && rounded) || need_b) {
+    if (products && rounded) dz = at::empty({M, N}, x.options());
+    const Tensor s = scratch(x, need_b ? l.mvit_act_bwd_scratch_bytes((int)M, (int)N) : 0);
+    ok(l.mvit_act_bwd(dy2.const_data_ptr(), f32(dy2), code == MVIT_ACT_NONE ? nullptr : pre.const_data_ptr(), code,
+                      products && rounded ? dz.mutable_data_ptr() : nullptr, need_b ? db.mutable_data_ptr() : nullptr, f32(db),
+                      need_b ? s.mutable_data_ptr() : nullptr, (int)M, (int)N, st),
+       "mvit_act_bwd");
+  }
+  if (need_x) {   // dx = dz W: its K axis is N
+    const Tensor wt = transposed(l, rows(weight), st);
+    Tensor a = dz;
+    if (wt.size(1) != N) {
+      a = at::zeros({M, wt.size(1)}, dz.options());
+      a.narrow(1, 0, N).copy_(dz);
+    }
+    product(l, operand(a), wt, std::nullopt, std::nullopt, dx, nullptr, MVIT_ACT_NONE, nullptr, nullptr, M, K, st);
+  }
+  if (need_w)     // dW = dz^T x: its K axis is M
+    product(l, transposed(l, dz, st), transposed(l, rows(x), st), std::nullopt, std::nullopt, dw, nullptr, MVIT_ACT_NONE, nullptr, nullptr, N, K, st);
+  return {dx, dw, db};
+}
+std::tuple<Tensor, Tensor, Tensor> linear_act_backward_meta(const Tensor&, const Tensor& x, const Tensor& weight, const Tensor&, c10::string_view,
+                                                            bool need_x, bool need_w, bool need_b, ScalarType bias_dtype) {
+  const ScalarType t = x.scalar_type();
+  return {need_x ? at::empty(x.sizes(), x.options()) : none(x, t), need_w ? at::empty(weight.sizes(), x.options()) : none(x, t),
+          need_b ? at::empty({weight.size(0)}, x.options().dtype(bias_dtype)) : none(x, bias_dtype)};
+}
+
+int linear_fp8_check(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& w_scale, const OptTensor& bias,
+                     const OptTensor& residual, c10::string_view act, ScalarType out_dtype, HalfType& h) {
+  const char* op = "linear_fp8";
+  REQUIRE(x.scalar_type() == at::kFloat8_e4m3fn && weight.scalar_type() == at::kFloat8_e4m3fn, op, "x and weight are float8_e4m3fn, got ",
+          x.scalar_type(), " and ", weight.scalar_type());
+  const int code = linear_check(op, x, weight, bias, residual, act, 16);
+  REQUIRE(x_scale.scalar_type() == at::kFloat && w_scale.scalar_type() == at::kFloat && x_scale.sizes() == x.sizes().slice(0, x.dim() - 1) &&
+              w_scale.sizes() == weight.sizes().slice(0, 1),
+          op, "float32 scales ", x.sizes().slice(0, x.dim() - 1), " and ", weight.sizes().slice(0, 1), ", got ", x_scale.scalar_type(), " ",
+          x_scale.sizes(), " and ", w_scale.scalar_type(), " ", w_scale.sizes());
+  same_place(op, x, x_scale);
+  same_place(op, x, w_scale);
+  REQUIRE(is_half(out_dtype) || out_dtype == at::kFloat, op, "out_dtype ", out_dtype);
+  h.add(bias), h.add(residual);
+  if (!residual) h.add(out_dtype);
+  return code;
+}
+Tensor linear_fp8(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& w_scale, const OptTensor& bias, const OptTensor& residual,
+                  c10::string_view act, ScalarType out_dtype) {
+  no_grad("linear_fp8", {x_scale, w_scale, bias, residual});
+  HalfType h{"linear_fp8"};
+  const int code = linear_fp8_check(x, x_scale, weight, w_scale, bias, residual, act, out_dtype, h);
+  c10::DeviceGuard guard(x.device());
+  Tensor y = linear_out(x, weight, residual, out_dtype);
+  if (y.numel()) {
+    const Tensor xs = x_scale.contiguous(), ws = w_scale.contiguous();
+    product(lib(h.f16()), operand(x), operand(weight), bias ? OptTensor(bias->contiguous()) : std::nullopt,
+            residual ? OptTensor(rows(*residual)) : std::nullopt, y, nullptr, code, xs.const_data_ptr<float>(), ws.const_data_ptr<float>(),
+            x.numel() / x.size(-1), weight.size(0), stream(x));
+  }
+  return y;
+}
+Tensor linear_fp8_meta(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& w_scale, const OptTensor& bias,
+                       const OptTensor& residual, c10::string_view act, ScalarType out_dtype) {
+  HalfType h{"linear_fp8"};
+  linear_fp8_check(x, x_scale, weight, w_scale, bias, residual, act, out_dtype, h);
+  return linear_out(x, weight, residual, out_dtype);
+}
+
+// ================================================================ autograd
+template <class Sig>
+c10::TypedOperatorHandle<Sig> op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+}
+const auto& rms_forward_op() {
+  static const auto h = op<decltype(rms_norm_forward)>("mvit::rms_norm_forward");
+  return h;
+}
+const auto& rms_backward_op() {
+  static const auto h = op<decltype(rms_norm_backward)>("mvit::rms_norm_backward");
+  return h;
+}
+const auto& rotary_op() {
+  static const auto h = op<decltype(rotary_forward)>("mvit::rotary_forward");
+  return h;
+}
+const auto& linear_forward_op() {
+  static const auto h = op<decltype(linear_act_forward)>("mvit::linear_act_forward");
+  return h;
+}
+const auto& linear_backward_op() {
+  static const auto h = op<decltype(linear_act_backward)>("mvit::linear_act_backward");
+  return h;
+}
+
+bool wants_grad(std::initializer_list<OptTensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const auto& t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps,
+                               std::optional<ScalarType> out_dtype) {
+    at::AutoDispatchBelowAutograd below;
+    auto [y, h, rstd] = rms_forward_op().call(x, residual, weight, eps, out_dtype);
+    ctx->save_for_backward({residual ? h : x, weight, rstd});
+    ctx->saved_data["x_dtype"] = (int64_t)x.scalar_type();
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->set_materialize_grads(false);
+    if (residual)
+      ctx->mark_non_differentiable({rstd});
+    else
+      ctx->mark_non_differentiable({h, rstd});
+    return {y, h, rstd};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &weight = saved[1], &rstd = saved[2];
+    const auto x_dtype = (ScalarType)ctx->saved_data["x_dtype"].toInt();
+    const bool res = ctx->saved_data["residual"].toBool();   // (edges are counted over the tensors that were given)
+    const bool need_x = ctx->needs_input_grad(0), need_res = res && ctx->needs_input_grad(1), need_w = ctx->needs_input_grad(1 + res);
+    const Tensor &dy = g[0], &dh = g[1];
+    Tensor dx, dres, dw;
+    if (dy.defined()) {
+      std::tie(dx, dres, dw) = rms_backward_op().call(dy, given(dh), h, weight, rstd, x_dtype, need_x, need_res, need_w);
+      if (x_dtype == h.scalar_type()) dres = dx;
+    } else if (dh.defined()) {   // y was not used: the stream's gradient alone
+      dx = dh.to(x_dtype), dres = dh;
+      if (need_w) dw = at::zeros_like(weight);
+    }
+    return {need_x ? dx : Tensor(), need_res ? dres : Tensor(), need_w ? dw : Tensor(), Tensor(), Tensor()};
+  }
+};
+std::tuple<Tensor, Tensor, Tensor> rms_norm_forward_autograd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps,
+                                                             std::optional<ScalarType> out_dtype) {
+  if (wants_grad({x, residual, weight})) {
+    auto o = RmsNorm::apply(x, residual, weight, eps, out_dtype);
+    return {o[0], o[1], o[2]};
+  }
+  at::AutoDispatchBelowAutograd below;
+  return rms_forward_op().call(x, residual, weight, eps, out_dtype);
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections,
+                        int64_t rotate_heads, int64_t num_prefix, bool interleaved, bool inverse) {
+    at::AutoDispatchBelowAutograd below;
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["sections"] = sections.vec();
+    ctx->saved_data["heads"] = rotate_heads;
+    ctx->saved_data["prefix"] = num_prefix;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    return rotary_op().call(x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {   // the turn back, differentiable again by itself
+    const auto saved = ctx->get_saved_variables();
+    const auto sections = ctx->saved_data["sections"].toIntVector();
+    variable_list out(8);
+    if (g[0].defined())
+      out[0] = rotary_op().call(g[0], saved[0], saved[1], sections, ctx->saved_data["heads"].toInt(), ctx->saved_data["prefix"].toInt(),
+                                ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool());
+    return out;
+  }
+};
+Tensor rotary_forward_autograd(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
+                               int64_t num_prefix, bool interleaved, bool inverse) {
+  if (wants_grad({x})) return Rotary::apply(x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
+  at::AutoDispatchBelowAutograd below;
+  return rotary_op().call(x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
+}
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                               std::string act) {
+    at::AutoDispatchBelowAutograd below;
+    const bool keep = act != "none" && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
+    auto [y, pre] = linear_forward_op().call(x, weight, bias, residual, act, keep);
+    ctx->save_for_backward({x, weight, pre});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias_dtype"] = (int64_t)(bias ? bias->scalar_type() : x.scalar_type());
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->mark_non_differentiable({pre});
+    ctx->set_materialize_grads(false);
+    return {y, pre};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(5);
+    if (!g[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const bool bias = ctx->saved_data["bias"].toBool(), res = ctx->saved_data["residual"].toBool();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias && ctx->needs_input_grad(2);
+    if (need_x || need_w || need_b) {
+      const std::string act = ctx->saved_data["act"].toStringRef();
+      auto [dx, dw, db] = linear_backward_op().call(g[0], saved[0], saved[1], saved[2], act, need_x, need_w, need_b,
+                                                    (ScalarType)ctx->saved_data["bias_dtype"].toInt());
+      if (need_x) out[0] = dx;
+      if (need_w) out[1] = dw;
+      if (need_b) out[2] = db;
+    }
+    if (res && ctx->needs_input_grad(2 + bias)) out[3] = g[0];
+    return out;
+  }
+};
+std::tuple<Tensor, Tensor> linear_act_forward_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                                                       c10::string_view act, bool save_pre) {
+  if (wants_grad({x, weight, bias, residual})) {
+    auto o = LinearAct::apply(x, weight, bias, residual, std::string(act));
+    return {o[0], o[1]};
+  }
+  at::AutoDispatchBelowAutograd below;
+  return linear_forward_op().call(x, weight, bias, residual, act, save_pre);
+}
+
+// the backward operators are not differentiable themselves: a gradient of a gradient is refused, not silently zero
+std::tuple<Tensor, Tensor, Tensor> rms_norm_backward_autograd(const Tensor& dy, const OptTensor& dh, const Tensor& h, const Tensor& weight,
+                                                              const Tensor& rstd, ScalarType x_dtype, bool need_x, bool need_residual,
+                                                              bool need_weight) {
+  TORCH_CHECK(!wants_grad({dy, dh, h, weight}), "mvit::rms_norm is differentiable once");
+  at::AutoDispatchBelowAutograd below;
+  return rms_backward_op().call(dy, dh, h, weight, rstd, x_dtype, need_x, need_residual, need_weight);
+}
+std::tuple<Tensor, Tensor, Tensor> linear_act_backward_autograd(const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& pre,
+                                                                c10::string_view act, bool need_x, bool need_w, bool need_b, ScalarType bias_dtype) {
+  TORCH_CHECK(!wants_grad({dy, x, weight}), "mvit::linear_act is differentiable once");
+  at::AutoDispatchBelowAutograd below;
+  return linear_backward_op().call(dy, x, weight, pre, act, need_x, need_w, need_b, bias_dtype);
+}
+
+}  // namespace
+
+// The two libraries' entry points, from the paths that the Python host names (it has loaded torch's HIP runtime by then); 0, or 1 with
+// the reason in dlerror()
+extern "C" __attribute__((visibility("default"))) const char* mvit_torch_bind(const char* bf16_path, const char* f16_path) {
+  const char* paths[2] = {bf16_path, f16_path};
+  std::array<Lib, 2> got;
+  for (int i = 0; i < 2; ++i) {
+    void* h = dlopen(paths[i], RTLD_NOW | RTLD_LOCAL);
+    if (!h) return dlerror();
+#define MVIT_FN(name) \
+  if (!(got[i].name = reinterpret_cast<decltype(&::name)>(dlsym(h, #name)))) return dlerror()
+    MVIT_FN(mvit_rmsnorm_fwd);
+    MVIT_FN(mvit_rmsnorm_fp8_fwd);
+    MVIT_FN(mvit_quantize_rows_fp8);
+    MVIT_FN(mvit_rmsnorm_bwd_scratch_bytes);
+    MVIT_FN(mvit_rmsnorm_bwd);
+    MVIT_FN(mvit_rotary);
+    MVIT_FN(mvit_linear_act);
+    MVIT_FN(mvit_linear_fp8);
+    MVIT_FN(mvit_act_bwd_scratch_bytes);
+    MVIT_FN(mvit_act_bwd);
+    MVIT_FN(mvit_transpose_bf16);
+#undef MVIT_FN
+  }
+  libs = got;
+  bound = true;
+  return nullptr;
+}
+
+TORCH_LIBRARY_FRAGMENT(mvit, m) {
+  m.def("rms_norm_forward(Tensor x, Tensor? residual, Tensor weight, float eps, ScalarType? out_dtype) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_norm_backward(Tensor dy, Tensor? dh, Tensor h, Tensor weight, Tensor rstd, ScalarType x_dtype, bool need_x, bool need_residual, "
+        "bool need_weight) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("quantize_fp8(Tensor x) -> (Tensor, Tensor)");
+  m.def("rotary_forward(Tensor x, Tensor positions, Tensor inv_freq, int[] sections, int rotate_heads, int num_prefix, bool interleaved, "
+        "bool inverse) -> Tensor");
+  m.def("rotary_(Tensor(a!) x, Tensor positions, Tensor inv_freq, int[] sections, int rotate_heads, int num_prefix, bool interleaved) -> "
+        "Tensor(a!)");
+  m.def("linear_act_forward(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation, bool save_pre) -> (Tensor, Tensor)");
+  m.def("linear_act_backward(Tensor dy, Tensor x, Tensor weight, Tensor pre, str activation, bool need_x, bool need_w, bool need_b, "
+        "ScalarType bias_dtype) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_fp8(Tensor x, Tensor x_scale, Tensor weight, Tensor w_scale, Tensor? bias, Tensor? residual, str activation, "
+        "ScalarType out_dtype) -> Tensor");
+}
+TORCH_LIBRARY_IMPL(mvit, CUDA, m) {   // (torch's name for the ROCm device)
+  m.impl("rms_norm_forward", rms_norm_forward);
+  m.impl("rms_norm_backward", rms_norm_backward);
+  m.impl("rms_norm_fp8", rms_norm_fp8);
+  m.impl("quantize_fp8", quantize_fp8);
+  m.impl("rotary_forward", rotary_forward);
+  m.impl("rotary_", rotary_);
+  m.impl("linear_act_forward", linear_act_forward);
+  m.impl("linear_act_backward", linear_act_backward);
+  m.impl("linear_fp8", linear_fp8);
+}
+TORCH_LIBRARY_IMPL(mvit, Meta, m) {
+  m.impl("rms_norm_forward", rms_norm_forward_meta);
+  m.impl("rms_norm_backward", rms_norm_backward_meta);
+  m.impl("rms_norm_fp8", rms_norm_fp8_meta);
+  m.impl("quantize_fp8", quantize_fp8_meta);
+  m.impl("rotary_forward", rotary_forward_meta);
+  m.impl("rotary_", rotary_meta_);
+  m.impl("linear_act_forward", linear_act_forward_meta);
+  m.impl("linear_act_backward", linear_act_backward_meta);
+  m.impl("linear_fp8", linear_fp8_meta);
+}
+TORCH_LIBRARY_IMPL(mvit, AutogradCUDA, m) {
+  m.impl("rms_norm_forward", rms_norm_forward_autograd);
+  m.impl("rms_norm_backward", rms_norm_backward_autograd);
+  m.impl("rotary_forward", rotary_forward_autograd);
+  m.impl("linear_act_forward", linear_act_forward_autograd);
+  m.impl("linear_act_backward", linear_act_backward_autograd);
+  for (const char* name : {"rms_norm_fp8", "quantize_fp8", "rotary_", "linear_fp8"}) m.impl(name, torch::CppFunction::makeFallthrough());
+}

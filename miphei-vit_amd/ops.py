@@ -249,94 +249,6 @@ def layernorm_bwd(dh, x, w, dx, gamma_next=None, dy=None, eps=1e-6, accumulate=T
           _p(rowscale_next))
 
 
-def _f32(t):
-    return int(t.dtype == torch.float32)
-
-
-def _ld(t):
-    """row stride of a [rows, D] operand; that of a single row says nothing"""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def rmsnorm_fwd(x, res, w, h, y, rstd, eps):
-    """h = x + res; y = h * rstd * w (mvit_rmsnorm_fwd): x, res [M, D] rows of any stride, h, y dense; res / h / rstd may be None"""
-    M, D = x.shape
-    _call("mvit_rmsnorm_fwd", _p(x), _f32(x), _ld(x), _p(res), 0 if res is None else _f32(res), 0 if res is None else _ld(res),
-          _p(w), _f32(w), _p(h), _p(y), _f32(y), _p(rstd), M, D, eps)
-
-
-def rmsnorm_fp8_fwd(x, res, w, h, q, scale, eps):
-    """the same with y as e4m3 rows q and one f32 scale a row (mvit_rmsnorm_fp8_fwd)"""
-    M, D = x.shape
-    _call("mvit_rmsnorm_fp8_fwd", _p(x), _f32(x), _ld(x), _p(res), 0 if res is None else _f32(res),
-          0 if res is None else _ld(res), _p(w), _f32(w), _p(h), _p(q), _p(scale), M, D, eps)
-
-
-def quantize_rows_fp8(x, q, scale):
-    M, D = x.shape
-    _call("mvit_quantize_rows_fp8", _p(x), _f32(x), _ld(x), _p(q), _p(scale), M, D)
-
-
-def rmsnorm_bwd(dy, dh, h, w, rstd, dx, dres, dw):
-    """dx / dres / dw of rmsnorm_fwd (any of them None: not wanted); all [M, D] dense"""
-    M, D = h.shape
-    nbytes = int(L.lib().mvit_rmsnorm_bwd_scratch_bytes(M, D)) if dw is not None else 0
-    scratch = torch.empty(nbytes // 4, device=h.device, dtype=torch.float32) if nbytes else None
-    _call("mvit_rmsnorm_bwd", _p(dy), _f32(dy), _p(dh), _p(h), _f32(h), _p(w), _f32(w), _p(rstd), _p(dx), _p(dres), _p(dw), _p(scratch),
-          nbytes, M, D)
-
-
-_POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
-
-
-def rotary(x, y, positions, inv_freq, sections, rotate_heads, prefix, interleaved, inverse):
-    """y = x [B, N, H, Dh] with the pairs of the leading heads turned by positions * inv_freq (mvit_rotary); y is x: in place"""
-    a = L.RotaryArgs()
-    a.x, a.y, a.positions, a.inv_freq = x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr()
-    a.B, a.N, a.H, a.Dh = x.shape
-    a.xb, a.xn, a.xh, _ = x.stride()
-    a.yb, a.yn, a.yh, _ = y.stride()
-    a.pos_b = positions.stride(0) if positions.dim() == 3 else 0
-    a.rotate_heads, a.prefix, a.axes = rotate_heads, prefix, len(sections)
-    a.sections[:len(sections)] = sections
-    a.x_f32, a.pos_type, a.freq_f64 = _f32(x), _POS_TYPES[positions.dtype], int(inv_freq.dtype == torch.float64)
-    a.interleaved, a.inverse = int(interleaved), int(inverse)
-    L.check(L.lib().mvit_rotary(C.byref(a), _stream()), "mvit_rotary")
-    return y
-
-
-ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
-
-
-def linear_act(x, w, bias, res, y, pre, act, x_scale=None, w_scale=None):
-    """y = res + act(x @ w^T + bias) (mvit_linear_act; with scales: e4m3 operands, mvit_linear_fp8).  x [M, K], w [N, K], res [M, N] rows of
-    any stride, y and pre dense; bias / res / pre may be None"""
-    a = L.LinearArgs()
-    a.M, a.K = x.shape
-    a.N = w.shape[0]
-    a.x, a.w, a.y, a.ldx, a.ldw = x.data_ptr(), w.data_ptr(), y.data_ptr(), _ld(x), _ld(w)
-    if bias is not None:
-        a.bias, a.bias_f32 = bias.data_ptr(), _f32(bias)
-    if res is not None:
-        a.res, a.ldr = res.data_ptr(), _ld(res)
-    if pre is not None:
-        a.pre = pre.data_ptr()
-    a.act, a.y_f32 = ACTIVATIONS[act], _f32(y)
-    name = "mvit_linear_act"
-    if x_scale is not None:
-        a.x_scale, a.w_scale, name = x_scale.data_ptr(), w_scale.data_ptr(), "mvit_linear_fp8"
-    L.check(getattr(L.lib(), name)(C.byref(a), _stream()), name)
-    return y
-
-
-def act_bwd(dy, pre, act, dz, dbias):
-    """dz = dy * act'(pre) (pre None: dz = dy), dbias[n] = sum over rows of dy * act'(pre); dz or dbias may be None (mvit_act_bwd)"""
-    M, N = dy.shape
-    nbytes = int(L.lib().mvit_act_bwd_scratch_bytes(M, N)) if dbias is not None else 0
-    scratch = torch.empty(nbytes // 4, device=dy.device, dtype=torch.float32) if nbytes else None
-    _call("mvit_act_bwd", _p(dy), _f32(dy), _p(pre), ACTIVATIONS[act], _p(dz), _p(dbias), 0 if dbias is None else _f32(dbias), _p(scratch), M, N)
-
-
 def skinny_xw(X, W, out, *, ldx=None, ldw=None, ldo=None, M=None, K=None, R=None):
     """out[M,R] = X[M,K] @ W[R,K]^T (bf16 operands, R <= 16)."""
     _chk_bf16(X, "X")

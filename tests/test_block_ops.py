@@ -110,7 +110,6 @@ def refusals():
         "norm empty rows": lambda o: o.rms_norm(fake(4, 0), fake(0)),
         "norm wide": lambda o: o.rms_norm(fake(4, 16385), fake(16385)),
         "norm scalar": lambda o: o.rms_norm(fake(()), w),
-        "norm device": lambda o: o.rms_norm(x, fake(48, device="cpu")),
         "norm8 weight": lambda o: o.rms_norm_fp8(x, fake(47, dtype=f32)),
         "quantise wide": lambda o: o.quantize_fp8(fake(4, 16385)),
         "quantise integers": lambda o: o.quantize_fp8(fake(4, 8, dtype=i32)),
@@ -142,7 +141,7 @@ def refusals():
 
 
 @pytest.mark.parametrize("name", ["norm weight", "norm residual broadcast", "norm mixed halves", "norm f32 with half residual", "norm f64",
-                                  "norm integers", "norm out dtype", "norm empty rows", "norm wide", "norm scalar", "norm device", "norm8 weight",
+                                  "norm integers", "norm out dtype", "norm empty rows", "norm wide", "norm scalar", "norm8 weight",
                                   "quantise wide", "quantise integers", "rotary 3-d", "rotary odd head", "rotary sections", "rotary no sections",
                                   "rotary five axes", "rotary heads", "rotary prefix", "rotary positions", "rotary positions type",
                                   "rotary frequencies", "rotary_ expanded", "linear K", "linear weight", "linear types", "linear f32",
@@ -153,6 +152,60 @@ def test_refused(name):
     with FakeTensorMode():
         with pytest.raises(ValueError, match="mvit::"):
             refusals()[name](T())
+
+
+@pytest.mark.gpu
+def test_refused_on_two_devices():
+    ops = T()
+    x = torch.zeros(4, 48, device="cuda", dtype=torch.bfloat16)
+    q, s = ops.quantize_fp8(x)
+    for call in (lambda: ops.rms_norm(x, torch.ones(48)), lambda: ops.add_rms_norm(x, x.cpu(), torch.ones(48, device="cuda")),
+                 lambda: ops.rotary(x.view(1, 4, 3, 16), torch.zeros(4, 1, dtype=torch.int32), torch.ones(8, device="cuda"), [8]),
+                 lambda: ops.linear_act(x, torch.zeros(8, 48, dtype=torch.bfloat16)), lambda: ops.linear_fp8(q, s.cpu(), q, s)):
+        with pytest.raises(ValueError, match="mvit::"):
+            call()
+
+
+def test_c_entries_refuse_what_they_cannot_do():
+    """the C-ABI by itself: bad sizes, types and strides come back as -1 before anything is launched (addresses are never read here)"""
+    import ctypes as C
+    from miphei_vit_amd import _lib as L
+    lib, p = L.lib(), 4096
+    norm = lambda M, D, ldx=None, x_f32=0, res=None, res_f32=0, y_f32=0: lib.mvit_rmsnorm_fwd(  # noqa: E731
+        p, x_f32, D if ldx is None else ldx, res, res_f32, D, p, 1, p, p, y_f32, None, M, D, 1e-6, None)
+    assert norm(-1, 8) == norm(4, 0) == norm(4, 16385) == norm(4, 8, ldx=7) == norm(4, 8, y_f32=1) == norm(4, 8, x_f32=1, res=p) == -1
+    assert lib.mvit_rmsnorm_fwd(None, 0, 8, None, 0, 0, p, 1, None, p, 0, None, 4, 8, 1e-6, None) == -1
+    assert norm(0, 8) == 0
+    assert lib.mvit_quantize_rows_fp8(p, 0, 8, p, None, 4, 8, None) == -1
+    assert lib.mvit_rmsnorm_bwd(p, 0, None, p, 0, p, 1, p, p, None, p, None, 0, 4, 8, None) == -1          # dw without scratch
+    a = L.RotaryArgs(x=p, y=p, positions=p, inv_freq=p, B=1, N=2, H=2, Dh=8, rotate_heads=2, axes=1)
+    a.sections[0] = 4
+
+    def rot(**kw):
+        b = L.RotaryArgs.from_buffer_copy(a)
+        for k, v in kw.items():
+            if k == "sections":
+                b.sections[0] = v
+            else:
+                setattr(b, k, v)
+        return lib.mvit_rotary(C.byref(b), None)
+    assert all(rot(**kw) == -1 for kw in (dict(Dh=7), dict(Dh=1026), dict(H=1025), dict(rotate_heads=3), dict(prefix=3), dict(axes=0), dict(axes=5),
+                                          dict(sections=5), dict(sections=0), dict(sections=-1), dict(pos_type=3), dict(x=None), dict(B=-1)))
+    assert rot(N=0) == rot(B=0) == 0
+    a = L.LinearArgs(x=p, w=p, y=p, x_scale=p, w_scale=p, ldx=16, ldw=16, M=4, N=4, K=16)
+
+    def lin(fn, **kw):
+        b = L.LinearArgs.from_buffer_copy(a)
+        for k, v in kw.items():
+            setattr(b, k, v)
+        return fn(C.byref(b), None)
+    for fn in (lib.mvit_linear_act, lib.mvit_linear_fp8):
+        assert all(lin(fn, **kw) == -1 for kw in (dict(K=12), dict(K=0), dict(N=0), dict(M=-1), dict(ldx=8), dict(ldx=20), dict(ldw=17), dict(act=5),
+                                                  dict(act=-1), dict(x=p + 8), dict(w=p + 2), dict(y=None), dict(res=p, ldr=3), dict(ldx=1 << 24)))
+        assert lin(fn, M=0) == 0
+    assert lin(lib.mvit_linear_fp8, pre=p) == lin(lib.mvit_linear_fp8, x_scale=None) == -1
+    assert lib.mvit_act_bwd(p, 0, None, 3, p, None, 0, None, 4, 4, None) == -1                              # an activation without pre
+    assert lib.mvit_act_bwd(p, 0, p, 3, p, p, 0, None, 4, 4, None) == -1                                    # dbias without scratch
 
 
 def test_frequencies_and_grid():
