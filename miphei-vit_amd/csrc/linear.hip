@@ -1,55 +1,85 @@
 // The linear layer with activation and residual in its epilogue (kernels in linear_kernel.hpp), 16-bit and 8-bit operands.
-#include <type_traits>
+#include <cmath>
 #include "linear_kernel.hpp"
 
 using namespace mvit_linear;
 
 namespace {
 
-template <int MODE, int BM, int BN, int WM, int WN, int BKB, int NST>
+template <int MODE, class E, int BM, int BN, int WM, int WN, int BKB, int NST>
 int launch_tile(const Args& a, hipStream_t s) {
   using T = Tile<MODE, BM, BN, WM, WN, BKB, NST>;
   const long long nt = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
   if (nt > 0x7fffffff) return MVIT_EINVAL;
   static mvit_per_device_size raised;
-  const auto fn = linear_tile<MODE, BM, BN, WM, WN, BKB, NST>;
+  const auto fn = linear_tile<MODE, E, BM, BN, WM, WN, BKB, NST>;
   if (const int rc = mvit_ensure_dynamic_lds((const void*)fn, T::LDS, raised)) return rc;
-  hipLaunchKernelGGL(fn, dim3((unsigned)nt), dim3(T::NT), T::LDS, s, a);
+  const long long slots = (long long)mvit_num_cus() * T::BLOCKS_PER_CU;
+  hipLaunchKernelGGL(fn, dim3((unsigned)(nt < slots ? nt : slots)), dim3(T::NT), T::LDS, s, a);
   return MVIT_LAUNCH_CHECK();
 }
 
-template <bool OP8, int MT>
+template <bool OP8, class E, int MT>
 int launch_rows(const Args& a, hipStream_t s) {
-  hipLaunchKernelGGL((linear_rows<OP8, MT>), dim3((a.N + 15) / 16), dim3(512), 0, s, a);
+  hipLaunchKernelGGL((linear_rows<OP8, E, MT>), dim3((a.N + 15) / 16), dim3(512), 0, s, a);
   return MVIT_LAUNCH_CHECK();
 }
 
-template <int MODE>
-int dispatch(const Args& a, hipStream_t s) {
-  if (a.M <= 16) return launch_rows<MODE != H16, 1>(a, s);
-  if (a.M <= 32) return launch_rows<MODE != H16, 2>(a, s);
-  const long long t128 = (long long)((a.M + 127) / 128) * ((a.N + 127) / 128);
-  if (t128 >= mvit_num_cus()) return launch_tile<MODE, 128, 128, 2, 2, 128, 2>(a, s);
-  return launch_tile<MODE, 64, 64, 2, 2, 128, 4>(a, s);
+// Rows or tiles, and which: by what a round of blocks costs.  A round is every CU's share at once (one 256 x 256 tile, two of the others);
+// measured at K = 1536, bf16, it takes 40 us with tiles of 256 x 256, 27 of 128 x 128 (20 with one a CU) and 12 of 64 x 64, and the
+// ratios hold for e4m3 and other K within some per cent.  Large tiles read less of x and W; small ones leave less of the chip idle in the
+// last round: [5264, 1536] x [4608, 1536]: 75 / 79 / 130 us, [5264, 4096] x [1536, 4096]: 80 / 62 / 104, [1301, 1536] x [4608, 1536]:
+// 36 / 26 / 35, [329, 1536] x [4608, 1536]: 34 / 20 / 13.
+template <int MODE, class E>
+int by_size(const Args& a, hipStream_t s) {
+  using Any = End<E::out32, A_ANY, E::vec>;   // (the row kernels' epilogue is not unrolled)
+  const long long cus = mvit_num_cus();
+  // few rows: [1, 1536] x [1536, 1536] bf16 5.8 us against 9.0 with tiles, [17, ..] 6.7 / 9.1, [32, 4096] x [1536, 4096] 14 / 18; from 33
+  // rows on (9.0 / 9.2) and, from 17 on, with more than one block a CU (N > 4096) the tiles are as fast or faster
+  if (a.M <= 16) return launch_rows<MODE != H16, Any, 1>(a, s);
+  if (a.M <= 32 && a.N <= 16 * cus) return launch_rows<MODE != H16, Any, 2>(a, s);
+  auto rounds = [&](long long edge, long long at_once) {
+    const long long t = ((a.M + edge - 1) / edge) * ((a.N + edge - 1) / edge);
+    return (t + at_once - 1) / at_once;
+  };
+  const long long c256 = 40 * rounds(256, cus), c128 = rounds(128, cus) == 1 ? 20 : 27 * rounds(128, 2 * cus), c64 = 12 * rounds(64, 2 * cus);
+  if (c256 < c128 && c256 < c64) return launch_tile<MODE, E, 256, 256, 2, 4, 128, 2>(a, s);
+  if (c128 < c64) return launch_tile<MODE, E, 128, 128, 2, 2, 128, 2>(a, s);
+  return launch_tile<MODE, E, 64, 64, 2, 2, 128, 4>(a, s);
+}
+
+template <int MODE, bool OUT32>
+int dispatch(Args& a, bool vec, hipStream_t s) {
+  if (!vec) return by_size<MODE, End<OUT32, A_ANY, false>>(a, s);
+  switch (a.act) {
+    case MVIT_ACT_NONE:
+    case MVIT_ACT_RELU:
+      return by_size<MODE, End<OUT32, A_CLIP, true>>(a, s);
+    case MVIT_ACT_GELU:
+      return by_size<MODE, End<OUT32, A_ERF, true>>(a, s);
+    default:
+      return by_size<MODE, End<OUT32, A_SIGMOID, true>>(a, s);
+  }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // 0: go on, 1: nothing to do, < 0: refused.  es: bytes of an operand's value.
-int check(const mvit_linear_args* g, int es, Args& a) {
+int check(const mvit_linear_args* g, int es, Args& a, bool& vec) {
   if (!g || g->M < 0 || g->N <= 0 || g->K <= 0) return MVIT_EINVAL;
   if (g->M == 0) return 1;   // (an empty tensor has no address)
   if (!g->x || !g->w || !g->y) return MVIT_EINVAL;
   if (g->act < MVIT_ACT_NONE || g->act > MVIT_ACT_GELU_TANH) return MVIT_EINVAL;
   const long long kb = (long long)g->K * es, lx = g->ldx * es, lw = g->ldw * es;
-  // 16-byte pieces of K; the offsets inside a block's 128 rows are 31-bit
+  // 16-byte pieces of K; the offsets inside a block's 256 rows are 31-bit
   if (kb % 16 || lx % 16 || lw % 16 || lx < kb || lw < kb || !aligned16(g->x) || !aligned16(g->w)) return MVIT_EINVAL;
   if (kb > (1 << 23) || lx > (1 << 23) || lw > (1 << 23)) return MVIT_EINVAL;
   if (g->res && g->ldr < g->N) return MVIT_EINVAL;
   const int ye = g->y_f32 ? 4 : 2;
   a = {(const char*)g->x, (const char*)g->w, g->bias, g->res, g->y, g->pre, g->x_scale, g->w_scale, g->res ? g->ldr : 0, (unsigned)lx, (unsigned)lw,
-       g->M, g->N, (int)kb, g->act, g->bias_f32, g->y_f32, 0};
-  a.vec = g->N % 8 == 0 && aligned16(g->y) && aligned16(g->pre) && aligned16(g->res) && (!g->res || g->ldr * ye % 16 == 0);
+       g->M, g->N, (int)kb, g->act, g->bias_f32, g->act == MVIT_ACT_RELU ? 0.f : -INFINITY, g->act == MVIT_ACT_SILU ? 1.f : TANH_K,
+       g->act == MVIT_ACT_SILU ? 0.f : TANH_K * 0.044715f};
+  vec = g->N % 8 == 0 && aligned16(g->y) && aligned16(g->pre) && aligned16(g->res) && (!g->res || g->ldr * ye % 16 == 0);
   return 0;
 }
 
@@ -58,16 +88,18 @@ int check(const mvit_linear_args* g, int es, Args& a) {
 extern "C" MVIT_API int mvit_linear_act(const mvit_linear_args* args, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
   Args a;
-  if (const int rc = check(args, 2, a)) return rc < 0 ? rc : MVIT_OK;
-  return dispatch<H16>(a, (hipStream_t)stream);
+  bool vec;
+  if (const int rc = check(args, 2, a, vec)) return rc < 0 ? rc : MVIT_OK;
+  return args->y_f32 ? dispatch<H16, true>(a, vec, (hipStream_t)stream) : dispatch<H16, false>(a, vec, (hipStream_t)stream);
 }
 
 extern "C" MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
   Args a;
-  if (const int rc = check(args, 1, a)) return rc < 0 ? rc : MVIT_OK;
+  bool vec;
+  if (const int rc = check(args, 1, a, vec)) return rc < 0 ? rc : MVIT_OK;
   if (!a.xs || !a.ws || a.pre) return MVIT_EINVAL;
-  return a.y_f32 ? dispatch<F8X>(a, (hipStream_t)stream) : dispatch<F8>(a, (hipStream_t)stream);
+  return args->y_f32 ? dispatch<F8X, true>(a, vec, (hipStream_t)stream) : dispatch<F8, false>(a, vec, (hipStream_t)stream);
 }
 
 // ---------------------------------------------------------------- backward of the epilogue

@@ -10,6 +10,8 @@
 // widens the e4m3 values to 16 bits in registers (exact) for the 16-bit instructions, at half the rate.  Few rows are bound by reading
 // W, not by the matrix cores, and always take F8X.
 #pragma once
+#include <type_traits>
+#include <utility>
 #include "common.hpp"
 #include "../../include/miphei_hip.h"
 
@@ -29,7 +31,17 @@ struct Args {
   long long ldr;     // residual's row stride in elements
   unsigned ldx, ldw; // row strides in bytes
   int M, N, kb;      // kb: bytes of a row of x and W
-  int act, bias_f32, y_f32, vec;   // vec: rows of y, pre and res start on 16 bytes and N % 8 == 0
+  int act, bias_f32;
+  float act_lo, act_a, act_b;   // constants of the activation's class, see activate()
+};
+
+// What a tile kernel is compiled for besides its operands.  The epilogue is unrolled over the accumulators: with every activation and
+// output in one kernel it was 9800 instructions, more than the instruction cache holds, and cost 3 us a tile instead of 1.
+enum Act { A_CLIP, A_SIGMOID, A_ERF, A_ANY };
+template <bool OUT32, int ACT, bool VEC>   // VEC: rows of y, pre and res start on 16 bytes and N % 8 == 0; else by elements
+struct End {
+  static constexpr bool out32 = OUT32, vec = VEC;
+  static constexpr int act = ACT;
 };
 
 constexpr unsigned OOB = 0x80000000u;   // beyond every descriptor's range: the load returns zeros
@@ -54,90 +66,91 @@ __device__ __forceinline__ float normal_cdf(float z) {
   return z >= 0.f ? 1.f - q : q;
 }
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504089f * z)); }
-constexpr float TANH_K = 1.5957691216f;   // 2 sqrt(2 / pi): (1 + tanh u) / 2 = sigmoid(2 u)
+constexpr float TANH_K = 1.5957691216f;   // 2 sqrt(2 / pi)
 
-template <int V>
-__device__ __forceinline__ void activate(float (&v)[V], int act) {
-  switch (act) {
-    case MVIT_ACT_RELU:
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];   // (a NaN stays one, as the definition has it)
-      break;
-    case MVIT_ACT_SILU:
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = v[e] * sigmoid(v[e]);
-      break;
-    case MVIT_ACT_GELU:
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = v[e] * normal_cdf(v[e]);
-      break;
-    case MVIT_ACT_GELU_TANH:
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = v[e] * sigmoid(TANH_K * (v[e] + 0.044715f * v[e] * v[e] * v[e]));
-      break;
-    default:
-      break;
-  }
+// Three classes: none and relu clip at act_lo (-inf, 0; a NaN stays one); silu and gelu_tanh are z sigmoid(z (a + b z^2)) with
+// (1, 0) and 2 sqrt(2 / pi) (1, 0.044715) -- (1 + tanh u) / 2 = sigmoid(2 u); gelu is z Phi(z).
+template <int ACT>
+__device__ __forceinline__ float activated(const Args& p, float z) {
+  if constexpr (ACT == A_CLIP) return z < p.act_lo ? p.act_lo : z;
+  if constexpr (ACT == A_SIGMOID) return z * sigmoid(z * __builtin_fmaf(z * z, p.act_b, p.act_a));
+  if constexpr (ACT == A_ERF) return z * normal_cdf(z);
+  return p.act == MVIT_ACT_GELU ? z * normal_cdf(z)
+         : p.act == MVIT_ACT_SILU || p.act == MVIT_ACT_GELU_TANH ? z * sigmoid(z * __builtin_fmaf(z * z, p.act_b, p.act_a))
+                                                                  : z < p.act_lo ? p.act_lo : z;
 }
 
 __device__ __forceinline__ float value_of(const void* p, size_t i, bool f32) { return f32 ? ((const float*)p)[i] : bf2f(((const bf16_t*)p)[i]); }
 
-// The end of 8 columns of one row: column constants cs (w_scale) and cb (bias) of the lane's columns
-template <bool OP8>
-__device__ __forceinline__ void finish8(const Args& p, float (&v)[8], int row, int col, const float (&cs)[8], const float (&cb)[8]) {
-  if (row >= p.M || col >= p.N) return;
-  if constexpr (OP8) {
-    const float s = p.xs[row];
+// A piece is what a lane finishes at once: 16 bytes of y, W = 8 columns of a row (4 where y is f32).
+// Column constants of a piece: the weight's scales and the bias
+template <bool OP8, int W>
+struct Columns {
+  float s[W], b[W];
+  __device__ __forceinline__ void load(const Args& p, int col) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * s * cs[e];
+    for (int e = 0; e < W; ++e) {
+      const int c = min(col + e, p.N - 1);
+      s[e] = OP8 ? p.ws[c] : 1.f;
+      b[e] = p.bias ? value_of(p.bias, c, p.bias_f32) : 0.f;
+    }
   }
+};
+// The residual's piece, raw: loaded ahead of use, because a load that is waited for behind stores waits for these too
+template <class E>
+__device__ __forceinline__ uint4 residual_piece(const Args& p, int row, int col) {
+  if (!E::vec || !p.res || row >= p.M || col >= p.N) return make_uint4(0, 0, 0, 0);
+  return *(const uint4*)((const char*)p.res + ((size_t)row * p.ldr + col) * (E::out32 ? 4 : 2));
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+}
+
+// The end of a piece but for its store: v (products, times their row's scale) -> the bits of y (E::vec), or all of it (not E::vec)
+template <bool OP8, class E, int W>
+__device__ __forceinline__ uint4 finish(const Args& p, float (&v)[W], int row, int col, const Columns<OP8, W>& c, const uint4& res) {
+  static_assert(W == (E::out32 ? 4 : 8), "16 bytes of y");
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] += cb[e];
-  const size_t o = (size_t)row * p.N + col, r = (size_t)row * p.ldr + col;
-  if (p.vec) {
-    if (!OP8 && p.pre)
-      *(uint4*)((bf16_t*)p.pre + o) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
-    activate(v, p.act);
-    if (p.y_f32) {
-      if (p.res) {
-        const float4 a = *(const float4*)((const float*)p.res + r), b = *(const float4*)((const float*)p.res + r + 4);
-        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-      }
-      *(float4*)((float*)p.y + o) = make_float4(v[0], v[1], v[2], v[3]);
-      *(float4*)((float*)p.y + o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  for (int e = 0; e < W; ++e) v[e] = OP8 ? __builtin_fmaf(v[e], c.s[e], c.b[e]) : v[e] + c.b[e];
+  if constexpr (E::vec) {
+    if (!OP8 && p.pre && row < p.M && col < p.N) {
+      bf16_t* o = (bf16_t*)p.pre + (size_t)row * p.N + col;
+      if constexpr (W == 8)
+        *(uint4*)o = pack8(v);
+      else
+        *(uint2*)o = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
+    }
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = activated<E::act>(p, v[e]);
+    if constexpr (W == 4) {
+      if (p.res) v[0] += __uint_as_float(res.x), v[1] += __uint_as_float(res.y), v[2] += __uint_as_float(res.z), v[3] += __uint_as_float(res.w);
+      return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     } else {
       if (p.res) {
-        const uint4 a = *(const uint4*)((const bf16_t*)p.res + r);
-        v[0] += lo16f(a.x), v[1] += hi16f(a.x), v[2] += lo16f(a.y), v[3] += hi16f(a.y);
-        v[4] += lo16f(a.z), v[5] += hi16f(a.z), v[6] += lo16f(a.w), v[7] += hi16f(a.w);
+        v[0] += lo16f(res.x), v[1] += hi16f(res.x), v[2] += lo16f(res.y), v[3] += hi16f(res.y);
+        v[4] += lo16f(res.z), v[5] += hi16f(res.z), v[6] += lo16f(res.w), v[7] += hi16f(res.w);
       }
-      *(uint4*)((bf16_t*)p.y + o) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+      return pack8(v);
     }
   } else {
-    const int n = min(8, p.N - col);
-    if (!OP8 && p.pre)
+    const size_t o = (size_t)row * p.N + col, r = (size_t)row * p.ldr + col;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) ((bf16_t*)p.pre)[o + e] = f2bf(v[e]);
-    activate(v, p.act);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) {
-        if (p.res) v[e] += value_of(p.res, r + e, p.y_f32);
-        if (p.y_f32)
-          ((float*)p.y)[o + e] = v[e];
+    for (int e = 0; e < W; ++e)
+      if (row < p.M && col + e < p.N) {
+        if (!OP8 && p.pre) ((bf16_t*)p.pre)[o + e] = f2bf(v[e]);
+        float u = activated<E::act>(p, v[e]);
+        if (p.res) u += value_of(p.res, r + e, E::out32);
+        if constexpr (E::out32)
+          ((float*)p.y)[o + e] = u;
         else
-          ((bf16_t*)p.y)[o + e] = f2bf(v[e]);
+          ((bf16_t*)p.y)[o + e] = f2bf(u);
       }
+    return make_uint4(0, 0, 0, 0);
   }
 }
-template <bool OP8>
-__device__ __forceinline__ void column_constants(const Args& p, int col, float (&cs)[8], float (&cb)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    cs[e] = OP8 && col + e < p.N ? p.ws[col + e] : 0.f;
-    cb[e] = p.bias && col + e < p.N ? value_of(p.bias, col + e, p.bias_f32) : 0.f;
-  }
+template <class E>
+__device__ __forceinline__ void store_piece(const Args& p, int row, int col, const uint4& u) {
+  if (E::vec && row < p.M && col < p.N) *(uint4*)((char*)p.y + ((size_t)row * p.N + col) * (E::out32 ? 4 : 2)) = u;
 }
 
 // 16 e4m3 values -> two fragments of 8 16-bit ones (order kept; exact)
@@ -161,116 +174,145 @@ __device__ __forceinline__ void widen(const i32x4& v, bf16x8 (&out)[2]) {
 }
 
 // ---------------------------------------------------------------- tiles
-// A block of WM x WN waves forms BM x BN of y.  K goes by in tiles of BKB bytes a row; NST of them live in LDS, filled by DMA
-// (buffer_load ... lds, 16 bytes a lane), NST - 1 ahead of the one being multiplied.  LDS rows are BKB bytes; the 16-byte piece c of row r
-// lies at place c ^ (r / (256 / BKB) mod pieces), which puts the 16 rows that a fragment read touches on all 64 banks once.
-// The fragments of the next sub-step are read into registers while the current one's matrix instructions run; the hand-over of a
-// K tile (this wave's reads are back, its DMA of the next tile has landed, barrier, refill of the tile just read) stands in front of the
-// last sub-step's instructions.
+// WM x WN waves form BM x BN of y at a time.  K goes by in tiles of BKB bytes a row; NST of them live in LDS, filled by DMA
+// (buffer_load ... lds, 16 bytes a lane).  LDS rows are BKB bytes; the 16-byte piece c of row r lies at place
+// c ^ (r / (256 / BKB) mod pieces), which puts the 16 rows that a fragment read touches on all 64 banks once.
+//  * The fragments of the next sub-step (64 bytes of K) are read into registers behind the current one's matrix instructions; the
+//    hand-over of a K tile (this wave's reads are back, its DMA of the next tile has landed, barrier) stands in front of the last
+//    sub-step, and the refill of the tile just read is issued behind it.
+//  * Blocks are persistent: a block walks output tiles, and the refill runs on into the next output tile's K tiles, so that neither
+//    its first loads nor a launch stand between two tiles; they land while the epilogue runs.
+//  * The products are formed as W x^T: a lane then holds groups of 4 consecutive columns of one row of y.  Which row of W is which row of
+//    a fragment is free, and is chosen so that a lane's groups make up whole pieces of 16 bytes and the lanes of a row 64 bytes in a
+//    line: y leaves from the registers.  (Through panels in LDS, whole lines a store, the epilogue took 6 to 8 us of a 256 x 256 tile:
+//    a chain of LDS writes, reads and waits with two waves a SIMD to hide it.)
 template <int MODE, int BM, int BN, int WM, int WN, int BKB, int NST>
 struct Tile {
   static constexpr int NW = WM * WN, NT = NW * 64;
   static constexpr int WTM = BM / WM, WTN = BN / WN;
   static constexpr int FR = MODE == F8 ? 32 : 16;       // rows of a fragment
   static constexpr int TM = WTM / FR, TN = WTN / FR;
-  static constexpr int NSUB = BKB / 64;                 // sub-steps: 64 bytes of K each
   static constexpr int PIECES = BKB / 16;
   static constexpr int ROWS_PER_DMA = 1024 / BKB;       // rows of one wave's DMA instruction
   static constexpr int A_DMA = BM / ROWS_PER_DMA / NW, B_DMA = BN / ROWS_PER_DMA / NW, LPT = A_DMA + B_DMA;
   static constexpr int STAGE = (BM + BN) * BKB;
-  static constexpr int PLD = WTN + 4;                   // floats in a row of the epilogue panel
-  static constexpr size_t LDS = (size_t)NST * STAGE;
+  static constexpr int NSUB = BKB / 64;                 // sub-steps of a K tile: 64 bytes each
+  static constexpr int TABLE = MODE == F8 ? 2 * WTN : 0;   // floats of a wave's table of column constants
+  static constexpr size_t LDS = (size_t)NST * STAGE + (size_t)NW * TABLE * 4;
+  static constexpr int BLOCKS_PER_CU = 160 * 1024 / LDS < 512 / NT ? 160 * 1024 / LDS : 512 / NT;   // two waves a SIMD
   static_assert(A_DMA >= 1 && B_DMA >= 1 && TM >= 1 && TN >= 1, "tile too small");
-  static_assert((size_t)NW * 16 * PLD * 4 <= LDS, "the panels fit the stages");
+  static_assert((BKB == 64 || BKB == 128) && NW * ROWS_PER_DMA % 32 == 0, "LDS places repeat every 32 rows");
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
 
-template <int MODE, int BM, int BN, int WM, int WN, int BKB, int NST>
-__global__ __launch_bounds__(64 * WM * WN) void linear_tile(const Args p) {
+template <int MODE, class E, int BM, int BN, int WM, int WN, int BKB, int NST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   using T = Tile<MODE, BM, BN, WM, WN, BKB, NST>;
   constexpr bool OP8 = MODE != H16, WIDE = MODE == F8;   // WIDE: 32 x 32 instructions
   using frag = std::conditional_t<WIDE, i32x8, i32x4>;
   using acc_t = std::conditional_t<WIDE, f32x16, f32x4>;
-  constexpr int AR = WIDE ? 16 : 4;
+  constexpr int AR = WIDE ? 16 : 4, NR = T::TM + T::TN;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-
-  // block -> tile: blocks go to the eight XCDs in turn, so the ids of one XCD are put on one contiguous run of tiles, and runs go down
-  // 8 rows of tiles before the next column: the ~32 to 64 blocks that share an L2 share rows of x and of W
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, nt = tm * tn;
-  int id;
-  {
-    const int q = nt >> 3, r = nt & 7, xcd = blockIdx.x & 7;
-    id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
-  }
-  const int per = 8 * tn, g0 = id / per * 8, gsz = min(tm - g0, 8), in = id % per;
-  const int m0 = (g0 + in % gsz) * BM, n0 = in / gsz * BN;
+  const int nk = (p.kb + 127) / 128;            // turns of the main loop: 128 bytes of K each
 
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + (size_t)m0 * p.ldx), rw = make_rsrc(p.w + (size_t)n0 * p.ldw);
-  // this lane's part of a wave's DMA instruction: one 16-byte piece of row `dr`, at place lane % PIECES
-  const int dr = lane / T::PIECES, dp = lane % T::PIECES;
+  // tile number -> place: blocks go to the eight XCDs in turn, so the numbers of one XCD are put on one contiguous run of tiles, and runs
+  // go down 8 rows of tiles before the next column: the blocks that share an L2 share rows of x and of W
+  auto place = [&](int v, int& m0, int& n0) __attribute__((always_inline)) {
+    const int q = nt >> 3, r = nt & 7, xcd = v & 7;
+    const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (v >> 3);
+    const int per = 8 * tn, g0 = id / per * 8, gsz = min(tm - g0, 8), in = id % per;
+    m0 = (g0 + in % gsz) * BM, n0 = in / gsz * BN;
+  };
+
+  // the place of piece c of LDS row r is c ^ x_place(r), c ^ w_place(r): 16 lanes read 16 rows, for x 16 in a line, for W (H16 with 16-bit
+  // y) those of bit 2 alike among 32
+  constexpr bool PAIRED = MODE == H16 && !E::out32;
+  auto x_place = [](int r) __attribute__((always_inline)) { return BKB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  auto w_place = [](int r) __attribute__((always_inline)) { return BKB == 128 ? (PAIRED ? ((r >> 1) & 1) | ((r >> 2) & 6) : (r >> 1) & 7) : PAIRED ? (r >> 3) & 3 : (r >> 2) & 3; };
+
+  // ---- the DMA side: output tile `dv`, K tile `dk` of it come next
+  const int dr = lane / T::PIECES;   // this lane's part of a wave's DMA instruction: one 16-byte piece of row `dr`
+  const int drow = wave * T::ROWS_PER_DMA + dr;   // (further instructions of the wave are a multiple of 32 rows on: the same places)
+  const int x_piece = (lane % T::PIECES ^ x_place(drow)) * 16, w_piece = (lane % T::PIECES ^ w_place(drow)) * 16;
+  __amdgpu_buffer_rsrc_t rx, rw;
   unsigned off[T::LPT];
-  int src_piece;
-  {
-    // the places repeat every 16 rows, and a wave's instructions are a multiple of 16 rows apart: one piece for all of them
-    static_assert(T::NW * T::ROWS_PER_DMA % 16 == 0, "places repeat every 16 rows");
-    src_piece = (dp ^ (((wave * T::ROWS_PER_DMA + dr) / (256 / BKB)) % T::PIECES)) * 16;
+  int dv = blockIdx.x, dk = 0;
+  auto aim = [&](auto) __attribute__((always_inline)) {
+    int m0 = 0, n0 = 0;
+    const bool any = dv < nt;
+    if (any) place(dv, m0, n0);
+    rx = make_rsrc(p.x + (size_t)m0 * p.ldx), rw = make_rsrc(p.w + (size_t)n0 * p.ldw);
 #pragma unroll
     for (int j = 0; j < T::LPT; ++j) {
       const bool a = j < T::A_DMA;
       const int row = ((a ? j : j - T::A_DMA) * T::NW + wave) * T::ROWS_PER_DMA + dr;
-      const bool ok = a ? m0 + row < p.M : n0 + row < p.N;
-      off[j] = ok ? (unsigned)row * (a ? p.ldx : p.ldw) + (unsigned)src_piece : OOB;
+      const bool in = any && (a ? m0 + row < p.M : n0 + row < p.N);
+      off[j] = in ? (unsigned)row * (a ? p.ldx : p.ldw) + (unsigned)(a ? x_piece : w_piece) : OOB;
     }
-  }
-  auto issue = [&](int t, auto) __attribute__((always_inline)) {   // K tile t into its stage; beyond the end: zeros
-    char* s = smem + (t % NST) * T::STAGE;
-    const int k = t * BKB;
-    const bool ok = k + src_piece < p.kb;
-#pragma unroll
-    for (int j = 0; j < T::LPT; ++j) {
-      const bool a = j < T::A_DMA;
-      char* to = s + (a ? 0 : BM * BKB) + ((a ? j : j - T::A_DMA) * T::NW + wave) * 1024;
-      unsigned o = ok ? off[j] : OOB;
-      asm volatile("" : "+v"(o));   // one unconditional instruction a piece: the waits count them
-      if (a)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)to, 16, o, k, 0, 0);
-      else
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)to, 16, o, k, 0, 0);
+  };
+  auto issue = [&](int stage, int j, auto) __attribute__((always_inline)) {   // piece j of the next K tile; beyond K or M, N: zeros
+    const bool a = j < T::A_DMA;
+    char* to = smem + stage * T::STAGE + (a ? 0 : BM * BKB) + ((a ? j : j - T::A_DMA) * T::NW + wave) * 1024;
+    const int k = dk * BKB;
+    unsigned o = k + (a ? x_piece : w_piece) < p.kb ? off[j] : OOB;
+    asm volatile("" : "+v"(o));   // one unconditional instruction a piece: the waits count them
+    if (a)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)to, 16, o, k, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)to, 16, o, k, 0, 0);
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    if (++dk == nk * (128 / BKB)) {
+      dk = 0;
+      dv += gridDim.x;
+      aim(0);
     }
   };
 
-  // fragment addresses.  A lane holds piece lane / 16 (of the sub-step's four) of row lane % 16; F8: pieces 2 (lane / 32) and the next
-  // of row lane % 32.  Which K values those are does not matter as long as x and W agree.
+  // ---- fragments.  A lane holds piece lane / 16 (of the sub-step's four) of row lane % 16; F8: pieces 2 (lane / 32) and the next of row
+  // lane % 32.  Which K values those are does not matter as long as x and W agree.
   const int fr = lane % T::FR, fh = lane / T::FR;
-  auto read = [&](const char* base, int rows0, int s) __attribute__((always_inline)) {
-    const int sw = (fr / (256 / BKB)) % T::PIECES;   // rows0 is a multiple of 16
-    const char* row = base + (rows0 + fr) * BKB;
+  frag fa[2][T::TM], fb[2][T::TN];
+  auto read = [&](const char* base, int row, int place, int s) __attribute__((always_inline)) {
+    const char* at = base + row * BKB;
     if constexpr (WIDE) {
       const int c = s * 4 + fh * 2;
-      const i32x4 lo = *(const i32x4*)(row + ((c ^ sw) << 4)), hi = *(const i32x4*)(row + (((c + 1) ^ sw) << 4));
+      const i32x4 lo = *(const i32x4*)(at + ((c ^ place) << 4)), hi = *(const i32x4*)(at + (((c + 1) ^ place) << 4));
       return (frag){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     } else {
-      return *(const frag*)(row + (((s * 4 + fh) ^ sw) << 4));
+      return *(const frag*)(at + (((s * 4 + fh) ^ place) << 4));
     }
   };
-  frag fa[2][T::TM], fb[2][T::TN];
-  acc_t acc[T::TM][T::TN];
-#pragma unroll
-  for (int i = 0; i < T::TM; ++i)
-#pragma unroll
-    for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-      for (int r = 0; r < AR; ++r) acc[i][j][r] = 0.f;
-  auto load = [&](int t, int s, int f) __attribute__((always_inline)) {
-    const char* st = smem + (t % NST) * T::STAGE;
-#pragma unroll
-    for (int j = 0; j < T::TN; ++j) fb[f][j] = read(st + BM * BKB, wn * T::WTN + j * T::FR, s);
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) fa[f][i] = read(st, wm * T::WTM + i * T::FR, s);
+  // row of W (of the wave's WTN) that is row fr of fragment j.  A lane's results are, by row of the fragment, 4 fh .. + 3 (F8: + 8 g):
+  //   H16, 16-bit y: of fragments 2 q and 2 q + 1 together the 8 columns from 32 q + 8 fh on
+  //   F8:            of groups 2 k and 2 k + 1 together the 8 columns from 32 j + 16 k + 8 fh on
+  //   f32 y:         the 4 columns from 16 j + 4 fh on
+  const int w_row = PAIRED ? (fr >> 2) * 8 + (fr & 3) : WIDE ? (fr & 0x13) | (fr & 4) << 1 | (fr & 8) >> 1 : fr;
+  auto w_row_of = [&](int j) __attribute__((always_inline)) { return w_row + (PAIRED ? (j >> 1) * 32 + (j & 1) * 4 : j * T::FR); };
+  // fragment r of sub-step s of a stage into set f, in the order the products take them: x 0, all of W, x 1 ...
+  auto load1 = [&](int stage, int s, int f, int r) __attribute__((always_inline)) {
+    const char* st = smem + stage * T::STAGE;
+    if (r >= 1 && r <= T::TN)   // (the places of rows 32 or 4 apart agree where w_row_of() steps by them)
+      fb[f][r - 1] = read(st + BM * BKB + wn * T::WTN * BKB, w_row_of(r - 1), w_place(w_row), s);
+    else
+      fa[f][r ? r - T::TN : 0] = read(st + wm * T::WTM * BKB, fr + (r ? r - T::TN : 0) * T::FR, x_place(fr), s);
   };
-  auto multiply = [&](int f) __attribute__((always_inline)) {
+  acc_t acc[T::TM][T::TN];
+  // One sub-step: the products of fragment set f, and behind each of them its share of the reads of the next set (sub-step s of a stage)
+  // and of the DMA into stage d (d < 0: none).  Left to itself the compiler gathers the reads into bursts that the next products wait for.
+  auto sub_step = [&](int f, int stage, int s, int d, auto dma) __attribute__((always_inline)) {
+    constexpr int ND = decltype(dma)::value ? T::LPT : 0;
+    auto behind = [&](int m, int NM) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = m * NR / NM; r < (m + 1) * NR / NM; ++r) load1(stage, s, f ^ 1, r);
+#pragma unroll
+      for (int j = m * ND / NM; j < (m + 1) * ND / NM; ++j) issue(d, j, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    };
     if constexpr (MODE == F8X) {
       bf16x8 b[T::TN][2];
 #pragma unroll
@@ -282,7 +324,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile(const Args p) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < T::TN; ++j) acc[i][j] = mvit_mfma16(a[h], b[j][h], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < T::TN; ++j) {
+            acc[i][j] = mvit_mfma16(b[j][h], a[h], acc[i][j], 0, 0, 0);
+            behind((i * 2 + h) * T::TN + j, T::TM * T::TN * 2);
+          }
       }
     } else {
 #pragma unroll
@@ -291,81 +336,146 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile(const Args p) {
         for (int jj = 0; jj < T::TN; ++jj) {
           const int j = i & 1 ? T::TN - 1 - jj : jj;   // neighbours share an operand
           if constexpr (WIDE)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[f][i], fb[f][j], acc[i][j], 0, 0, 0, 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[f][j], fa[f][i], acc[i][j], 0, 0, 0, 0, 0, 0);
           else
-            acc[i][j] = mvit_mfma16(__builtin_bit_cast(bf16x8, fa[f][i]), __builtin_bit_cast(bf16x8, fb[f][j]), acc[i][j], 0, 0, 0);
+            acc[i][j] = mvit_mfma16(__builtin_bit_cast(bf16x8, fb[f][j]), __builtin_bit_cast(bf16x8, fa[f][i]), acc[i][j], 0, 0, 0);
+          behind(i * T::TN + jj, T::TM * T::TN);
         }
     }
   };
-  auto hand_over = [&](int t, auto tag) __attribute__((always_inline)) {   // tile t is read, tile t + 1 comes
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * T::LPT) : "memory");
+  auto barrier = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    issue(t + NST, tag);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  const int nk = (p.kb + BKB - 1) / BKB;
+  aim(0);
 #pragma unroll
-  for (int t = 0; t < NST; ++t) issue(t, 0);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * T::LPT) : "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  load(0, 0, 0);
-  if constexpr (T::NSUB == 2) {
-    for (int t = 0; t < nk; ++t) {
-      load(t, 1, 1);
-      multiply(0);
-      hand_over(t, 0);
-      load(t + 1, 0, 0);
-      multiply(1);
-    }
-  } else {
-    for (int t = 0; t < nk; t += 2) {   // an odd last tile is followed by one of zeros
-      hand_over(t, 0);
-      load(t + 1, 0, 1);
-      multiply(0);
-      hand_over(t + 1, 0);
-      load(t + 2, 0, 0);
-      multiply(1);
-    }
+  for (int t = 0; t < NST; ++t) {
+#pragma unroll
+    for (int j = 0; j < T::LPT; ++j) issue(t, j, 0);
+    advance();
   }
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing of anybody's is on its way to or from the stages
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * T::LPT) : "memory");
+  barrier();
+#pragma unroll
+  for (int r = 0; r < NR; ++r) load1(0, 0, 0, r);
 
-  // ---- epilogue: 16 rows at a time through a panel of this wave's own, so that a lane ends up with 8 columns of one row
-  float* panel = (float*)smem + wave * 16 * T::PLD;
-  constexpr int LPR = T::WTN / 8, RPP = 64 / LPR;   // lanes a row, rows a pass
-  const int pr = lane / LPR, pc = lane % LPR * 8;
-  const int col = n0 + wn * T::WTN + pc;
-  float cs[8], cb[8];
-  column_constants<OP8>(p, col, cs, cb);
+  int stage = 0, landed = 0;   // landed: K tiles behind the current one whose DMA has been waited for already
+  for (int v = blockIdx.x; v < nt; v += gridDim.x) {
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i)
-#pragma unroll
-    for (int h = 0; h < T::FR / 16; ++h) {
+    for (int i = 0; i < T::TM; ++i)
 #pragma unroll
       for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-        for (int r = 0; r < AR / (T::FR / 16); ++r) {
-          const int row = WIDE ? (r >> 2) * 8 + fh * 4 + (r & 3) : fh * 4 + r;
-          panel[row * T::PLD + j * T::FR + fr] = acc[i][j][(WIDE ? h * 8 : 0) + r];
-        }
-#pragma unroll
-      for (int q = 0; q < 16 / RPP; ++q) {
-        const float* s = panel + (q * RPP + pr) * T::PLD + pc;
-        const float4 a = *(const float4*)s, b = *(const float4*)(s + 4);
-        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        finish8<OP8>(p, v, m0 + wm * T::WTM + i * T::FR + h * 16 + q * RPP + pr, col, cs, cb);
+        for (int r = 0; r < AR; ++r) acc[i][j][r] = 0.f;
+    auto wait_next = [&]() __attribute__((always_inline)) {   // this wave's reads are back, its DMA of the next K tile has landed
+      if (landed > 0)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * T::LPT) : "memory");
+      --landed;
+      barrier();
+    };
+    for (int t = 0; t < nk; ++t) {
+      const int next = stage + 1 == NST ? 0 : stage + 1;
+      if constexpr (T::NSUB == 2) {
+        sub_step(0, stage, 1, -1, std::false_type{});
+        wait_next();
+        sub_step(1, next, 0, stage, std::true_type{});
+        advance();
+        stage = next;
+      } else {   // two K tiles a turn
+        const int after = next + 1 == NST ? 0 : next + 1;
+        wait_next();
+        sub_step(0, next, 0, stage, std::true_type{});
+        advance();
+        wait_next();
+        sub_step(1, after, 0, next, std::true_type{});
+        advance();
+        stage = after;
       }
     }
+    // ---- epilogue, from the registers.  The DMA of the next tile's first K tiles is waited for in front of its stores: loads, DMA and
+    // stores share one counter, and behind the stores it could not be told any more.
+    int m0, n0;
+    place(v, m0, n0);
+    constexpr int W = E::out32 ? 4 : 8, NP = T::TN * AR / W;   // pieces of a lane in one row of fragments
+    const int row0 = m0 + wm * T::WTM + fr, col0 = n0 + wn * T::WTN;
+    auto col_of = [&](int q) __attribute__((always_inline)) {
+      return col0 + (PAIRED ? q * 32 + fh * 8 : WIDE ? (q >> 1) * 32 + (q & 1) * 16 + fh * 8 : q * 16 + fh * 4);
+    };
+    // column constants: in registers, or (F8: 64 of them, beside 128 accumulators) in a table of the wave's own
+    Columns<OP8, W> cols[NP];
+    float rs[T::TM];
+    float* table = (float*)(smem + NST * T::STAGE) + wave * T::TABLE;
+    if constexpr (WIDE) {
+      const int c = min(col0 + lane, p.N - 1);
+      if (lane < T::WTN) {
+        table[lane] = p.ws[c];
+        table[T::WTN + lane] = p.bias ? value_of(p.bias, c, p.bias_f32) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < NP; ++q) cols[q].load(p, col_of(q));
+    }
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) rs[i] = OP8 ? p.xs[min(row0 + i * T::FR, p.M - 1)] : 1.f;
+    uint4 res[2][NP];   // of this row of fragments and the next
+#pragma unroll
+    for (int q = 0; q < NP; ++q) res[0][q] = residual_piece<E>(p, row0, col_of(q));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    landed = NST - 1;
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+      const int row = row0 + i * T::FR;
+      if (i + 1 < T::TM)
+#pragma unroll
+        for (int q = 0; q < NP; ++q) res[(i + 1) & 1][q] = residual_piece<E>(p, row + T::FR, col_of(q));
+      uint4 out[NP];
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        if constexpr (WIDE) {
+          const float* t = table + (col_of(q) - col0);
+#pragma unroll
+          for (int e = 0; e < W; ++e) cols[q].s[e] = t[e], cols[q].b[e] = t[T::WTN + e];
+        }
+        float o[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          o[e] = (WIDE ? acc[i][q >> 1][(q & 1) * 8 + e] : PAIRED ? acc[i][q * 2 + (e >> 2)][e & 3] : acc[i][q][e & 3]) * (OP8 ? rs[i] : 1.f);
+        out[q] = finish<OP8, E, W>(p, o, row, col_of(q), cols[q], res[i & 1][q]);
+        if constexpr (!WIDE) store_piece<E>(p, row, col_of(q), out[q]);
+      }
+      if constexpr (WIDE && E::vec) {
+        // two lanes of a row, 32 bytes a store: trade pieces between rows r and r + 16, so that four lanes have 64 bytes of one row
+#pragma unroll
+        for (int q = 0; q < NP; q += 2) {
+          uint32_t *a = (uint32_t*)&out[q], *b = (uint32_t*)&out[q + 1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const auto s = __builtin_amdgcn_permlane16_swap(a[e], b[e], false, false);
+            a[e] = s[0], b[e] = s[1];
+          }
+          const int r = row - fr + (lane & 15), c = col0 + (q >> 1) * 32 + ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;
+          store_piece<E>(p, r, c, out[q]);
+          store_piece<E>(p, r + 16, c, out[q + 1]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (rows of fragments pulled together cost registers that are not there)
+    }
+    // the next tile's first fragments again: read once more, they need no registers during the epilogue
+#pragma unroll
+    for (int r = 0; r < NR; ++r) load1(stage, 0, 0, r);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the zeros behind the last tile: nothing of this block's is on its way to LDS)
 }
 
 // ---------------------------------------------------------------- few rows
 // M <= 16 MT: what counts is to have W on its way at once.  A block forms 16 columns of all rows; its 8 waves share K in pieces of
 // 128 bytes a row (wave w takes pieces w, w + 8, ...), load their fragments straight from memory into registers -- W is read by nobody
 // else -- and join through LDS in wave order.
-template <bool OP8, int MT>
+template <bool OP8, class E, int MT>
 __global__ __launch_bounds__(512) void linear_rows(const Args p) {
   constexpr int NWV = 8, U = 4;   // U pieces in flight
   __shared__ float part[NWV][MT * 16][17];
@@ -416,18 +526,22 @@ __global__ __launch_bounds__(512) void linear_rows(const Args p) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) part[wave][m * 16 + fh * 4 + r][fr] = acc[m][r];
   __syncthreads();
-  for (int i = tid; i < MT * 16 * 2; i += 512) {   // 8 columns of a row each
-    const int row = i >> 1, c0 = (i & 1) * 8, col = n0 + c0;
+  constexpr int W = E::out32 ? 4 : 8;
+  for (int i = tid; i < MT * 16 * (16 / W); i += 512) {   // a piece each
+    const int row = i / (16 / W), c0 = i % (16 / W) * W, col = n0 + c0;
     if (row >= p.M || col >= p.N) continue;
-    float v[8], cs[8], cb[8];
+    Columns<OP8, W> cols;
+    cols.load(p, col);
+    const uint4 res = residual_piece<E>(p, row, col);
+    float v[W];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < W; ++e) {
       v[e] = part[0][row][c0 + e];
 #pragma unroll
       for (int k = 1; k < NWV; ++k) v[e] += part[k][row][c0 + e];
+      if constexpr (OP8) v[e] *= p.xs[row];
     }
-    column_constants<OP8>(p, col, cs, cb);
-    finish8<OP8>(p, v, row, col, cs, cb);
+    store_piece<E>(p, row, col, finish<OP8, E, W>(p, v, row, col, cols, res));
   }
 }
 
