@@ -216,13 +216,17 @@ typedef struct mvit_linear_args {
 } mvit_linear_args;
 MVIT_API int mvit_linear_act(const mvit_linear_args* args, mvit_stream_t stream);
 MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_stream_t stream);
-/* Backward of the epilogue: dz(16-bit)[M,N] = dy * act'(pre) (pre NULL: act is none), dbias[N] (f32 or 16-bit) = its sum over the rows,
- * taken before dz is rounded; dz or dbias may be NULL.  dy f32 or 16-bit, all dense.  scratch: mvit_act_bwd_scratch_bytes(M, N) bytes
- * (needed with dbias only); ordered sums, bit-identical from run to run.  dx and dW are the products dz W and dz^T x
- * (mvit_gemm_bf16, mvit_gemm_tn_bf16). */
+/* Backward of the epilogue: dz(16-bit) = dy * act'(pre), rows [M, ld_dz] and transposed [N, ld_dzt], dbias[N] (f32 or 16-bit) = its sum
+ * over the rows, taken before dz is rounded; each of them may be NULL (dzt only beside dz).  dy [M, N] f32 or 16-bit and pre (16-bit; may be
+ * NULL where act is none) dense; ld_dz, ld_dzt are multiples of 8 with ld_dz >= N, M <= ld_dzt < M + 8, dz and dzt start on 16 bytes; what
+ * pads a row of dzt, and a row of dz up to ld_dz where N is no multiple of 8, is zero.  scratch: mvit_act_bwd_scratch_bytes(M, N) bytes
+ * (needed with dbias only); ordered sums, bit-identical from run to run.  dx and dW are the products dz W and dz^T x (mvit_linear_act). */
 MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N);
-MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, void* dbias, int dbias_f32, void* scratch, int M,
-                          int N, mvit_stream_t stream);
+MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dzt, long long ld_dzt,
+                          void* dbias, int dbias_f32, void* scratch, int M, int N, mvit_stream_t stream);
+/* dst[c][r] = src[r][c] (16-bit), rows of dst padded by zeros to ld_dst, R <= ld_dst < R + 8.  ld, ld_dst multiples of 8, ld at least Cc
+ * rounded up to 8, src and dst start on 16 bytes. */
+MVIT_API int mvit_transpose_padded(const void* src, long long ld, void* dst, long long ld_dst, int R, int Cc, mvit_stream_t stream);
 
 /* ---------------------------------------------------------------- decoder data movement (NHWC bf16) */
 /* dst[b,oy,ox,c] = sum_{ty,tx} ty_w[oy,ty]*tx_w[ox,tx] * f(src[b, ty_idx[oy,ty], tx_idx[ox,tx], c]),

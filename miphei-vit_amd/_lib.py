@@ -137,7 +137,8 @@ SIGNATURES = {
     "mvit_rotary": [C.POINTER(RotaryArgs), vp],
     "mvit_linear_act": [C.POINTER(LinearArgs), vp],
     "mvit_linear_fp8": [C.POINTER(LinearArgs), vp],
-    "mvit_act_bwd": [vp, ci, vp, ci, vp, vp, ci, vp, ci, ci, vp],
+    "mvit_act_bwd": [vp, ci, vp, ci, vp, ll, vp, ll, vp, ci, vp, ci, ci, vp],
+    "mvit_transpose_padded": [vp, ll, vp, ll, ci, ci, vp],
     "mvit_act_bwd_scratch_bytes": [ci, ci],
     "mvit_occupy_cus": [ci, ci, vp],
 }

@@ -1,5 +1,6 @@
 // The linear layer with activation and residual in its epilogue (kernels in linear_kernel.hpp), 16-bit and 8-bit operands.
 #include <cmath>
+#include "column_sums.hpp"
 #include "linear_kernel.hpp"
 
 using namespace mvit_linear;
@@ -103,132 +104,192 @@ extern "C" MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_strea
 }
 
 // ---------------------------------------------------------------- backward of the epilogue
-// dz = dy act'(pre) and its column sums, in one pass over dy and pre (HBM-bound).  A block owns 512 columns (64 lanes x 8; by elements
-// where N or an address is odd) and a run of rows, its 4 waves every fourth one; the sums of a run go through LDS in wave order to a
-// [runs][N] f32 workspace, which a second launch adds up in order.
+// dz = dy act'(pre), as rows and transposed, and its column sums, in one pass over dy and pre: bound by HBM.  The transposed copy is an
+// operand of dW = dz^T x, whose K axis is the rows; made from the values at hand it costs its write alone, a third of a transposition
+// by itself.  A block owns 64 columns and a run of rows, and goes down it by 64 x 64 tiles: a thread takes 8 columns of rows 2 r and
+// 2 r + 1 (16-byte loads), packs pairs of rows into LDS [column][row], and reads 8 rows of a column back.  Column stride 136 bytes: the 64
+// writes of a wave fall on 64 banks.  Sums over a run stay in registers, the runs meet in a f32 workspace (column_sums.hpp).
+// The same kernel with the identity and no sums transposes x and W.
 namespace {
 
-__device__ __forceinline__ float act_grad(float z, int act) {
+enum Slope { S_ONE, S_CLIP, S_SIGMOID, S_ERF, S_ANY };
+
+template <int SL>
+__device__ __forceinline__ float slope(float z, int act, float a, float b) {
+  if constexpr (SL == S_ONE) return 1.f;
+  if constexpr (SL == S_CLIP) return z > 0.f ? 1.f : z != z ? z : 0.f;
+  if constexpr (SL == S_SIGMOID) {   // z s(u), u = z (a + b z^2): s + z s (1 - s) (a + 3 b z^2)
+    const float z2 = z * z, p = sigmoid(z * __builtin_fmaf(z2, b, a));
+    return p + z * p * (1.f - p) * __builtin_fmaf(z2, 3.f * b, a);
+  }
+  if constexpr (SL == S_ERF) return normal_cdf(z) + z * 0.39894228040f * __builtin_amdgcn_exp2f(-0.72134752044f * z * z);
   switch (act) {
-    case MVIT_ACT_RELU:
-      return z > 0.f ? 1.f : z != z ? z : 0.f;
-    case MVIT_ACT_SILU: {
-      const float p = sigmoid(z);
-      return p + z * p * (1.f - p);
-    }
-    case MVIT_ACT_GELU:
-      return normal_cdf(z) + z * 0.39894228040f * __builtin_amdgcn_exp2f(-0.72134752044f * z * z);
-    case MVIT_ACT_GELU_TANH: {
-      const float p = sigmoid(TANH_K * (z + 0.044715f * z * z * z));
-      return p + z * p * (1.f - p) * TANH_K * (1.f + 0.134145f * z * z);
-    }
-    default:
+    case MVIT_ACT_NONE:
       return 1.f;
+    case MVIT_ACT_RELU:
+      return slope<S_CLIP>(z, act, a, b);
+    case MVIT_ACT_GELU:
+      return slope<S_ERF>(z, act, a, b);
+    default:
+      return slope<S_SIGMOID>(z, act, a, b);
   }
 }
 
-template <bool F32, bool VEC>
-__global__ __launch_bounds__(256) void act_bwd(const void* dy, const bf16_t* pre, int act, bf16_t* dz, float* part, int M, int N, int rows) {
-  __shared__ float lds[4][512];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
-  // VEC: lane owns columns c0 .. c0 + 7; else column c0 + 64 e
-  const int c0 = blockIdx.x * 512 + (VEC ? lane * 8 : lane);
+struct SlopeArgs {
+  const void* dy;
+  const bf16_t* pre;
+  bf16_t *dz, *dzt;
+  float* part;
+  long long ld, ld_dz, ld_dzt;   // ld: of dy (and of the source of a transposition); pre is dense
+  int M, N, rows, act;           // rows: of a run, a multiple of 64
+  float a, b;
+};
+
+template <int SL, bool F32>
+__global__ __launch_bounds__(256) void act_bwd_tiles(const SlopeArgs p) {
+  constexpr int LDT = 68;   // 16-bit values of a column in LDS
+  __shared__ __attribute__((aligned(16))) bf16_t tile[2][64 * LDT];
+  __shared__ float sums[32][65];
+  const int cg = threadIdx.x & 7, rp = threadIdx.x >> 3;
+  const int c0 = blockIdx.x * 64 + cg * 8;
+  const int r0 = blockIdx.y * p.rows, r1 = min(r0 + p.rows, (p.M + 63) / 64 * 64);
   float sum[8] = {};
-  for (int r = r0 + wave; r < r1; r += 4) {
-    const size_t o = (size_t)r * N + c0;
-    float g[8], z[8];
-    if constexpr (VEC) {
-      if (c0 >= N) break;
-      if constexpr (F32) {
-        const float4 a = *(const float4*)((const float*)dy + o), b = *(const float4*)((const float*)dy + o + 4);
-        g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, g[4] = b.x, g[5] = b.y, g[6] = b.z, g[7] = b.w;
-      } else {
-        const uint4 a = *(const uint4*)((const bf16_t*)dy + o);
-        g[0] = lo16f(a.x), g[1] = hi16f(a.x), g[2] = lo16f(a.y), g[3] = hi16f(a.y);
-        g[4] = lo16f(a.z), g[5] = hi16f(a.z), g[6] = lo16f(a.w), g[7] = hi16f(a.w);
-      }
-      if (pre) {
-        const uint4 a = *(const uint4*)(pre + o);
-        z[0] = lo16f(a.x), z[1] = hi16f(a.x), z[2] = lo16f(a.y), z[3] = hi16f(a.y);
-        z[4] = lo16f(a.z), z[5] = hi16f(a.z), z[6] = lo16f(a.w), z[7] = hi16f(a.w);
-      }
-    } else {
+  int buf = 0;
+  for (int t = r0; t < r1; t += 64, buf ^= 1) {
+    float g[2][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool ok = c0 + 64 * e < N;
-        g[e] = ok ? value_of(dy, o + 64 * e, F32) : 0.f;
-        if (pre) z[e] = ok ? bf2f(pre[o + 64 * e]) : 0.f;
+    for (int h = 0; h < 2; ++h) {
+      const int r = t + rp * 2 + h;
+      const bool in = r < p.M && c0 < p.N;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[h][e] = 0.f;
+      if (in) {
+        const size_t o = (size_t)r * p.ld + c0;
+        if constexpr (F32) {
+          const float4 u = *(const float4*)((const float*)p.dy + o), v = *(const float4*)((const float*)p.dy + o + 4);
+          g[h][0] = u.x, g[h][1] = u.y, g[h][2] = u.z, g[h][3] = u.w, g[h][4] = v.x, g[h][5] = v.y, g[h][6] = v.z, g[h][7] = v.w;
+        } else {
+          const uint4 u = *(const uint4*)((const bf16_t*)p.dy + o);
+          g[h][0] = lo16f(u.x), g[h][1] = hi16f(u.x), g[h][2] = lo16f(u.y), g[h][3] = hi16f(u.y);
+          g[h][4] = lo16f(u.z), g[h][5] = hi16f(u.z), g[h][6] = lo16f(u.w), g[h][7] = hi16f(u.w);
+        }
+        if constexpr (SL != S_ONE) {
+          const uint4 u = *(const uint4*)(p.pre + (size_t)r * p.N + c0);
+          const float z[8] = {lo16f(u.x), hi16f(u.x), lo16f(u.y), hi16f(u.y), lo16f(u.z), hi16f(u.z), lo16f(u.w), hi16f(u.w)};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[h][e] *= slope<SL>(z[e], 0, p.a, p.b);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += g[h][e];
+        if (p.dz) *(uint4*)(p.dz + (size_t)r * p.ld_dz + c0) = pack8(g[h]);
       }
     }
+    if (p.dzt) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (pre) g[e] *= act_grad(z[e], act);
-      sum[e] += g[e];
-    }
-    if (dz) {
-      if constexpr (VEC) {
-        *(uint4*)(dz + o) = make_uint4(pack2bf(g[0], g[1]), pack2bf(g[2], g[3]), pack2bf(g[4], g[5]), pack2bf(g[6], g[7]));
-      } else {
+      for (int e = 0; e < 8; ++e) *(uint32_t*)&tile[buf][(cg * 8 + e) * LDT + rp * 2] = pack2bf(g[0][e], g[1][e]);
+      __syncthreads();   // (the other buffer's reads are two barriers away from its next writes)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + 64 * e < N) dz[o + 64 * e] = f2bf(g[e]);
+      for (int h = 0; h < 2; ++h) {
+        const int c = rp + h * 32, r = t + cg * 8;   // 8 lanes a column: 128 bytes in a line; rows from M to the end of the last piece: zeros
+        if (blockIdx.x * 64 + c < p.N && r < p.ld_dzt) {
+          const uint2 *s = (const uint2*)&tile[buf][c * LDT + cg * 8], u = s[0], v = s[1];
+          *(uint4*)(p.dzt + (size_t)(blockIdx.x * 64 + c) * p.ld_dzt + r) = make_uint4(u.x, u.y, v.x, v.y);
+        }
       }
     }
   }
-  if (!part) return;
+  if (!p.part) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) lds[wave][VEC ? lane * 8 + e : lane + 64 * e] = sum[e];
+  for (int e = 0; e < 8; ++e) sums[rp][cg * 8 + e] = sum[e];
   __syncthreads();
-  for (int c = threadIdx.x; c < 512; c += 256)
-    if (blockIdx.x * 512 + c < N) part[(size_t)blockIdx.y * N + blockIdx.x * 512 + c] = lds[0][c] + lds[1][c] + lds[2][c] + lds[3][c];
+  if (threadIdx.x < 64 && blockIdx.x * 64 + (int)threadIdx.x < p.N) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) s += sums[k][threadIdx.x];
+    p.part[(size_t)blockIdx.y * p.N + blockIdx.x * 64 + threadIdx.x] = s;
+  }
 }
 
-// out[c] = sum over the runs in order
-__global__ __launch_bounds__(256) void add_runs(const float* part, void* out, int runs, int N, int out_f32) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= N) return;
-  float s = 0.f;
-#pragma unroll 8
-  for (int k = 0; k < runs; ++k) s += part[(size_t)k * N + c];
-  if (out_f32)
-    ((float*)out)[c] = s;
+// by elements, where N or an address is not a multiple of 8 values: a thread a column, dz with its rows padded by zeros to ld_dz
+template <bool F32>
+__global__ __launch_bounds__(256) void act_bwd_elements(const SlopeArgs p) {
+  const int c = blockIdx.x * 256 + threadIdx.x, r0 = blockIdx.y * p.rows, r1 = min(r0 + p.rows, p.M);
+  float sum = 0.f;
+  for (int r = r0; r < r1; ++r) {
+    float g = 0.f;
+    if (c < p.N) {
+      const size_t o = (size_t)r * p.N + c;
+      g = value_of(p.dy, o, F32);
+      if (p.act != MVIT_ACT_NONE) g *= slope<S_ANY>(bf2f(p.pre[o]), p.act, p.a, p.b);
+      sum += g;
+    }
+    if (p.dz && c < p.ld_dz) p.dz[(size_t)r * p.ld_dz + c] = f2bf(g);
+  }
+  if (p.part && c < p.N) p.part[(size_t)blockIdx.y * p.N + c] = sum;
+}
+
+// rows of a run: blocks enough for eight a CU, no more than 128 runs to add up
+int run_rows(int M, int N) {
+  const int tiles = (M + 63) / 64, cols = (N + 63) / 64;
+  int runs = (mvit_num_cus() * 8 + cols - 1) / cols;
+  runs = runs > 128 ? 128 : runs;
+  runs = runs > tiles ? tiles : runs;
+  return (tiles + runs - 1) / runs * 64;
+}
+int run_count(int M, int N) { return M <= 0 ? 0 : (M + run_rows(M, N) - 1) / run_rows(M, N); }
+
+template <bool F32>
+void launch_tiles(const SlopeArgs& a, dim3 grid, hipStream_t s) {
+  if (a.act == MVIT_ACT_NONE)
+    hipLaunchKernelGGL((act_bwd_tiles<S_ONE, F32>), grid, dim3(256), 0, s, a);
+  else if (a.act == MVIT_ACT_RELU)
+    hipLaunchKernelGGL((act_bwd_tiles<S_CLIP, F32>), grid, dim3(256), 0, s, a);
+  else if (a.act == MVIT_ACT_GELU)
+    hipLaunchKernelGGL((act_bwd_tiles<S_ERF, F32>), grid, dim3(256), 0, s, a);
   else
-    ((bf16_t*)out)[c] = f2bf(s);
+    hipLaunchKernelGGL((act_bwd_tiles<S_SIGMOID, F32>), grid, dim3(256), 0, s, a);
 }
-
-// rows of a run: runs enough to fill the chip, but no more than 64 of them to add up
-int run_rows(int M) {
-  const int r = (M + 63) / 64;
-  return r < 16 ? 16 : r;
-}
-int run_count(int M) { return M <= 0 ? 0 : (M + run_rows(M) - 1) / run_rows(M); }
 
 }  // namespace
 
-extern "C" MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N) { return M <= 0 || N <= 0 ? 0 : (long long)run_count(M) * N * 4; }
+extern "C" MVIT_API int mvit_transpose_padded(const void* src, long long ld, void* dst, long long ld_dst, int R, int Cc, mvit_stream_t stream) {
+  MVIT_CLEAR_ERROR();
+  if (!src || !dst || R <= 0 || Cc <= 0 || ld % 8 || ld_dst % 8 || ld < (Cc + 7) / 8 * 8 || ld_dst < R || ld_dst >= R + 8 || !aligned16(src) || !aligned16(dst))
+    return MVIT_EINVAL;
+  SlopeArgs a = {};
+  a.dy = src, a.dzt = (bf16_t*)dst, a.ld = ld, a.ld_dzt = ld_dst, a.M = R, a.N = Cc, a.rows = run_rows(R, Cc), a.act = MVIT_ACT_NONE;
+  launch_tiles<false>(a, dim3((Cc + 63) / 64, run_count(R, Cc)), (hipStream_t)stream);
+  return MVIT_LAUNCH_CHECK();
+}
 
-extern "C" MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, void* dbias, int dbias_f32, void* scratch,
-                                     int M, int N, mvit_stream_t stream) {
+extern "C" MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N) { return M <= 0 || N <= 0 ? 0 : (long long)run_count(M, N) * N * 4; }
+
+extern "C" MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dzt, long long ld_dzt,
+                                     void* dbias, int dbias_f32, void* scratch, int M, int N, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
   if (M < 0 || N <= 0 || (M > 0 && !dy) || act < MVIT_ACT_NONE || act > MVIT_ACT_GELU_TANH || (act != MVIT_ACT_NONE && M > 0 && !pre)) return MVIT_EINVAL;
   if (dbias && M > 0 && !scratch) return MVIT_EINVAL;
+  if ((dz && (ld_dz < N || ld_dz % 8 || !aligned16(dz))) || (dzt && (!dz || ld_dzt < M || ld_dzt >= M + 8 || ld_dzt % 8 || !aligned16(dzt))))
+    return MVIT_EINVAL;
   hipStream_t s = (hipStream_t)stream;
-  const int runs = run_count(M), rows = M > 0 ? run_rows(M) : 0;
+  const int runs = run_count(M, N);
   if (M > 0) {
-    const bool vec = N % 8 == 0 && aligned16(dy) && aligned16(pre) && aligned16(dz);
-    const dim3 grid((N + 511) / 512, runs);
-    float* part = dbias ? (float*)scratch : nullptr;
-    const bf16_t* z = act == MVIT_ACT_NONE ? nullptr : (const bf16_t*)pre;
-    if (dy_f32)
-      hipLaunchKernelGGL((vec ? act_bwd<true, true> : act_bwd<true, false>), grid, dim3(256), 0, s, dy, z, act, (bf16_t*)dz, part, M, N, rows);
-    else
-      hipLaunchKernelGGL((vec ? act_bwd<false, true> : act_bwd<false, false>), grid, dim3(256), 0, s, dy, z, act, (bf16_t*)dz, part, M, N, rows);
+    const SlopeArgs a = {dy, (const bf16_t*)pre, (bf16_t*)dz, (bf16_t*)dzt, dbias ? (float*)scratch : nullptr, N, ld_dz, ld_dzt, M, N, run_rows(M, N), act,
+                         act == MVIT_ACT_SILU ? 1.f : TANH_K, act == MVIT_ACT_SILU ? 0.f : TANH_K * 0.044715f};
+    if (N % 8 == 0 && aligned16(dy) && aligned16(pre)) {
+      const dim3 grid((N + 63) / 64, runs);
+      dy_f32 ? launch_tiles<true>(a, grid, s) : launch_tiles<false>(a, grid, s);
+    } else {
+      const dim3 grid((unsigned)(((dz ? ld_dz : N) + 255) / 256), runs);
+      if (dy_f32)
+        hipLaunchKernelGGL((act_bwd_elements<true>), grid, dim3(256), 0, s, a);
+      else
+        hipLaunchKernelGGL((act_bwd_elements<false>), grid, dim3(256), 0, s, a);
+      if (const int rc = MVIT_LAUNCH_CHECK()) return rc;
+      if (dzt)
+        if (const int rc = mvit_transpose_padded(dz, ld_dz, dzt, ld_dzt, M, N, stream)) return rc;
+    }
     if (const int rc = MVIT_LAUNCH_CHECK()) return rc;
   }
-  if (dbias) {
-    hipLaunchKernelGGL(add_runs, dim3((N + 255) / 256), dim3(256), 0, s, (const float*)scratch, dbias, runs, N, dbias_f32);
-    return MVIT_LAUNCH_CHECK();
-  }
-  return MVIT_OK;
+  return dbias ? launch_sum_parts((const float*)scratch, dbias, runs, N, dbias_f32, s) : MVIT_OK;
 }

@@ -13,6 +13,7 @@
 //  * Rows are walked with a grid stride, so that w is loaded once per thread and not once per row.
 // Sums and statistics are f32; sums over the rows (d w) go row by row in registers, over the waves of a block in LDS, over the blocks
 // through a [blocks][D] f32 workspace that a second launch adds up: a fixed order, no atomics, bit-identical from run to run.
+#include "column_sums.hpp"
 #include "common.hpp"
 #include "../../include/miphei_hip.h"
 
@@ -305,27 +306,6 @@ __global__ __launch_bounds__(512) void rms_bwd(const BwdArgs p) {
   }
 }
 
-// out[c] = sum over the parts, in order within 8 interleaved groups, then over the groups: 32 columns x 8 groups a block
-__global__ __launch_bounds__(256) void sum_parts(const float* part, void* out, int parts, int D, int out_f32) {
-  __shared__ float lds[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
-  float s = 0.f;
-  if (c < D) {
-#pragma unroll 8
-    for (int k = g; k < parts; k += 8) s += part[(size_t)k * D + c];
-  }
-  lds[g][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (g == 0 && c < D) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += lds[k][threadIdx.x];
-    if (out_f32)
-      ((float*)out)[c] = s;
-    else
-      ((bf16_t*)out)[c] = f2bf(s);
-  }
-}
-
 constexpr int MAX_D = 16384;
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -471,8 +451,7 @@ extern "C" MVIT_API int mvit_rmsnorm_bwd(const void* dy, int x_f32, const void* 
     if (rc) return rc;
   }
   if (dw) {
-    hipLaunchKernelGGL(sum_parts, dim3((D + 31) / 32), dim3(256), 0, s, (const float*)scratch, dw, grid, D, w_f32);
-    return MVIT_LAUNCH_CHECK();
+    return launch_sum_parts((const float*)scratch, dw, grid, D, w_f32, s);
   }
   return MVIT_OK;
 }

@@ -42,7 +42,7 @@ struct Lib {
   MVIT_FN(mvit_linear_fp8);
   MVIT_FN(mvit_act_bwd_scratch_bytes);
   MVIT_FN(mvit_act_bwd);
-  MVIT_FN(mvit_transpose_bf16);
+  MVIT_FN(mvit_transpose_padded);
 #undef MVIT_FN
 };
 std::array<Lib, 2> libs;   // [0] bf16, [1] fp16: filled by mvit_torch_bind before the first call
@@ -389,11 +389,12 @@ std::tuple<Tensor, Tensor> linear_act_forward_meta(const Tensor& x, const Tensor
   return {y, save_pre ? at::empty(y.sizes(), x.options()) : none(x, x.scalar_type())};
 }
 
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 // t^T with its rows padded by zeros to whole 16-byte pieces: an operand whose K axis is t's rows
 Tensor transposed(const Lib& l, const Tensor& t, void* st) {
-  const int64_t r = t.size(0), c = t.size(1), pad = (r + 7) / 8 * 8;
-  Tensor out = pad == r ? at::empty({c, r}, t.options()) : at::zeros({c, pad}, t.options());
-  ok(l.mvit_transpose_bf16(t.const_data_ptr(), out.mutable_data_ptr(), (int)r, (int)c, (int)ld(t), pad, st), "mvit_transpose_bf16");
+  Tensor out = at::empty({t.size(1), up8(t.size(0))}, t.options());
+  ok(l.mvit_transpose_padded(t.const_data_ptr(), ld(t), out.mutable_data_ptr(), out.size(1), (int)t.size(0), (int)t.size(1), st),
+     "mvit_transpose_padded");
   return out;
 }
 
@@ -409,28 +410,26 @@ std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const T
   if (M == 0) return {dx, dw.zero_(), db.zero_()};
   const Lib& l = lib(t == at::kHalf);
   void* st = stream(x);
-  const Tensor dy2 = dy.reshape({M, N}).contiguous();
-  Tensor dz = dy2;
-  const bool products = need_x || need_w, rounded = code != MVIT_ACT_NONE || dy2.scalar_type() != t;
-  if ((products && rounded) || need_b) {
-    if (products && rounded) dz = at::empty({M, N}, x.options());
+  Tensor dz = dy.reshape({M, N}).contiguous(), dzt;
+  const Tensor dy2 = dz;
+  // dz is dy itself where there is nothing to multiply, to round or to pad
+  const bool make = (need_x || need_w) && (code != MVIT_ACT_NONE || dy2.scalar_type() != t || N % 8);
+  if (make) dz = at::empty({M, up8(N)}, x.options());
+  if (need_w && (make || need_b)) dzt = at::empty({N, up8(M)}, x.options());
+  if (make || need_b) {
     const Tensor s = scratch(x, need_b ? l.mvit_act_bwd_scratch_bytes((int)M, (int)N) : 0);
+    if (dzt.defined() && !make) dz = at::empty({M, N}, x.options());   // (the transposed copy comes with the rows)
+    const bool rows = make || dzt.defined();
     ok(l.mvit_act_bwd(dy2.const_data_ptr(), f32(dy2), code == MVIT_ACT_NONE ? nullptr : pre.const_data_ptr(), code,
-                      products && rounded ? dz.mutable_data_ptr() : nullptr, need_b ? db.mutable_data_ptr() : nullptr, f32(db),
-                      need_b ? s.mutable_data_ptr() : nullptr, (int)M, (int)N, st),
+                      rows ? dz.mutable_data_ptr() : nullptr, rows ? dz.size(1) : 0, dzt.defined() ? dzt.mutable_data_ptr() : nullptr, up8(M),
+                      need_b ? db.mutable_data_ptr() : nullptr, f32(db), need_b ? s.mutable_data_ptr() : nullptr, (int)M, (int)N, st),
        "mvit_act_bwd");
   }
-  if (need_x) {   // dx = dz W: its K axis is N
-    const Tensor wt = transposed(l, rows(weight), st);
-    Tensor a = dz;
-    if (wt.size(1) != N) {
-      a = at::zeros({M, wt.size(1)}, dz.options());
-      a.narrow(1, 0, N).copy_(dz);
-    }
-    product(l, operand(a), wt, std::nullopt, std::nullopt, dx, nullptr, MVIT_ACT_NONE, nullptr, nullptr, M, K, st);
-  }
+  if (need_x)     // dx = dz W: its K axis is N
+    product(l, operand(dz), transposed(l, operand(weight), st), std::nullopt, std::nullopt, dx, nullptr, MVIT_ACT_NONE, nullptr, nullptr, M, K, st);
   if (need_w)     // dW = dz^T x: its K axis is M
-    product(l, transposed(l, dz, st), transposed(l, rows(x), st), std::nullopt, std::nullopt, dw, nullptr, MVIT_ACT_NONE, nullptr, nullptr, N, K, st);
+    product(l, dzt.defined() ? dzt : transposed(l, operand(dz), st), transposed(l, operand(x), st), std::nullopt, std::nullopt, dw, nullptr,
+            MVIT_ACT_NONE, nullptr, nullptr, N, K, st);
   return {dx, dw, db};
 }
 std::tuple<Tensor, Tensor, Tensor> linear_act_backward_meta(const Tensor&, const Tensor& x, const Tensor& weight, const Tensor&, c10::string_view,
@@ -665,7 +664,7 @@ extern "C" __attribute__((visibility("default"))) const char* mvit_torch_bind(co
     MVIT_FN(mvit_linear_fp8);
     MVIT_FN(mvit_act_bwd_scratch_bytes);
     MVIT_FN(mvit_act_bwd);
-    MVIT_FN(mvit_transpose_bf16);
+    MVIT_FN(mvit_transpose_padded);
 #undef MVIT_FN
   }
   libs = got;

@@ -204,8 +204,10 @@ def test_c_entries_refuse_what_they_cannot_do():
                                                   dict(act=-1), dict(x=p + 8), dict(w=p + 2), dict(y=None), dict(res=p, ldr=3), dict(ldx=1 << 24)))
         assert lin(fn, M=0) == 0
     assert lin(lib.mvit_linear_fp8, pre=p) == lin(lib.mvit_linear_fp8, x_scale=None) == -1
-    assert lib.mvit_act_bwd(p, 0, None, 3, p, None, 0, None, 4, 4, None) == -1                              # an activation without pre
-    assert lib.mvit_act_bwd(p, 0, p, 3, p, p, 0, None, 4, 4, None) == -1                                    # dbias without scratch
+    act = lambda pre=p, dz=p, ldz=8, dzt=None, ldzt=8, db=None, s=None: lib.mvit_act_bwd(p, 0, pre, 3, dz, ldz, dzt, ldzt, db, 0, s, 4, 8, None)  # noqa: E731
+    assert act(pre=None) == act(db=p) == act(ldz=4) == act(ldz=12) == act(dz=p + 2) == act(dz=None, dzt=p) == act(dzt=p, ldzt=16) == -1
+    assert lib.mvit_transpose_padded(p, 8, p, 16, 4, 8, None) == lib.mvit_transpose_padded(p, 8, p, 8, 4, 9, None) == -1
+    assert lib.mvit_transpose_padded(p + 2, 8, p, 8, 4, 8, None) == lib.mvit_transpose_padded(p, 12, p, 8, 4, 8, None) == -1
 
 
 def test_frequencies_and_grid():
