@@ -58,8 +58,10 @@ int dispatch(Args& a, bool vec, hipStream_t s) {
       return by_size<MODE, End<OUT32, A_CLIP, true>>(a, s);
     case MVIT_ACT_GELU:
       return by_size<MODE, End<OUT32, A_ERF, true>>(a, s);
+    case MVIT_ACT_SILU:
+      return by_size<MODE, End<OUT32, A_SILU, true>>(a, s);
     default:
-      return by_size<MODE, End<OUT32, A_SIGMOID, true>>(a, s);
+      return by_size<MODE, End<OUT32, A_TANH, true>>(a, s);
   }
 }
 
@@ -78,8 +80,7 @@ int check(const mvit_linear_args* g, int es, Args& a, bool& vec) {
   if (g->res && g->ldr < g->N) return MVIT_EINVAL;
   const int ye = g->y_f32 ? 4 : 2;
   a = {(const char*)g->x, (const char*)g->w, g->bias, g->res, g->y, g->pre, g->x_scale, g->w_scale, g->res ? g->ldr : 0, (unsigned)lx, (unsigned)lw,
-       g->M, g->N, (int)kb, g->act, g->bias_f32, g->act == MVIT_ACT_RELU ? 0.f : -INFINITY, g->act == MVIT_ACT_SILU ? 1.f : TANH_K,
-       g->act == MVIT_ACT_SILU ? 0.f : TANH_K * 0.044715f};
+       g->M, g->N, (int)kb, g->act, g->bias_f32, g->act == MVIT_ACT_RELU ? 0.f : -INFINITY};
   vec = g->N % 8 == 0 && aligned16(g->y) && aligned16(g->pre) && aligned16(g->res) && (!g->res || g->ldr * ye % 16 == 0);
   return 0;
 }
@@ -112,27 +113,28 @@ extern "C" MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_strea
 // The same kernel with the identity and no sums transposes x and W.
 namespace {
 
-enum Slope { S_ONE, S_CLIP, S_SIGMOID, S_ERF, S_ANY };
+enum Slope { S_ONE, S_CLIP, S_SILU, S_TANH, S_ERF, S_ANY };
 
 template <int SL>
-__device__ __forceinline__ float slope(float z, int act, float a, float b) {
+__device__ __forceinline__ float slope(float z, int act) {
   if constexpr (SL == S_ONE) return 1.f;
+  // (an infinity, as a z beyond fp16 is kept, has the slope of the far values: bounded, no infinity meets a zero.  A NaN stays one.)
+  z = __builtin_elementwise_minimum(__builtin_elementwise_maximum(z, -1e15f), 1e15f);
   if constexpr (SL == S_CLIP) return z > 0.f ? 1.f : z != z ? z : 0.f;
-  if constexpr (SL == S_SIGMOID) {   // z s(u), u = z (a + b z^2): s + z s (1 - s) (a + 3 b z^2)
-    const float z2 = z * z, p = sigmoid(z * __builtin_fmaf(z2, b, a));
-    return p + z * p * (1.f - p) * __builtin_fmaf(z2, 3.f * b, a);
+  if constexpr (SL == S_SILU) {   // z s(z): s + z s (1 - s)
+    const float p = sigmoid2(LOG2E * z);
+    return p + z * p * (1.f - p);
+  }
+  if constexpr (SL == S_TANH) {   // z s(u), u = z (a + b z^2): s + z s (1 - s) (a + 3 b z^2)
+    const float z2 = z * z, p = sigmoid2(z * __builtin_fmaf(z2, TANH_B, TANH_A));
+    return p + z * p * (1.f - p) * __builtin_fmaf(z2, 3.f * TANH_B / LOG2E, TANH_A / LOG2E);
   }
   if constexpr (SL == S_ERF) return normal_cdf(z) + z * 0.39894228040f * __builtin_amdgcn_exp2f(-0.72134752044f * z * z);
-  switch (act) {
-    case MVIT_ACT_NONE:
-      return 1.f;
-    case MVIT_ACT_RELU:
-      return slope<S_CLIP>(z, act, a, b);
-    case MVIT_ACT_GELU:
-      return slope<S_ERF>(z, act, a, b);
-    default:
-      return slope<S_SIGMOID>(z, act, a, b);
-  }
+  return act == MVIT_ACT_NONE        ? 1.f
+         : act == MVIT_ACT_RELU      ? slope<S_CLIP>(z, act)
+         : act == MVIT_ACT_SILU      ? slope<S_SILU>(z, act)
+         : act == MVIT_ACT_GELU_TANH ? slope<S_TANH>(z, act)
+                                     : slope<S_ERF>(z, act);
 }
 
 struct SlopeArgs {
@@ -142,7 +144,6 @@ struct SlopeArgs {
   float* part;
   long long ld, ld_dz, ld_dzt;   // ld: of dy (and of the source of a transposition); pre is dense
   int M, N, rows, act;           // rows: of a run, a multiple of 64
-  float a, b;
 };
 
 template <int SL, bool F32>
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(256) void act_bwd_tiles(const SlopeArgs p) {
           const uint4 u = *(const uint4*)(p.pre + (size_t)r * p.N + c0);
           const float z[8] = {lo16f(u.x), hi16f(u.x), lo16f(u.y), hi16f(u.y), lo16f(u.z), hi16f(u.z), lo16f(u.w), hi16f(u.w)};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) g[h][e] *= slope<SL>(z[e], 0, p.a, p.b);
+          for (int e = 0; e < 8; ++e) g[h][e] *= slope<SL>(z[e], 0);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += g[h][e];
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(256) void act_bwd_elements(const SlopeArgs p) {
     if (c < p.N) {
       const size_t o = (size_t)r * p.N + c;
       g = value_of(p.dy, o, F32);
-      if (p.act != MVIT_ACT_NONE) g *= slope<S_ANY>(bf2f(p.pre[o]), p.act, p.a, p.b);
+      if (p.act != MVIT_ACT_NONE) g *= slope<S_ANY>(bf2f(p.pre[o]), p.act);
       sum += g;
     }
     if (p.dz && c < p.ld_dz) p.dz[(size_t)r * p.ld_dz + c] = f2bf(g);
@@ -246,8 +247,10 @@ void launch_tiles(const SlopeArgs& a, dim3 grid, hipStream_t s) {
     hipLaunchKernelGGL((act_bwd_tiles<S_CLIP, F32>), grid, dim3(256), 0, s, a);
   else if (a.act == MVIT_ACT_GELU)
     hipLaunchKernelGGL((act_bwd_tiles<S_ERF, F32>), grid, dim3(256), 0, s, a);
+  else if (a.act == MVIT_ACT_SILU)
+    hipLaunchKernelGGL((act_bwd_tiles<S_SILU, F32>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((act_bwd_tiles<S_SIGMOID, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_tiles<S_TANH, F32>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -274,8 +277,7 @@ extern "C" MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre
   hipStream_t s = (hipStream_t)stream;
   const int runs = run_count(M, N);
   if (M > 0) {
-    const SlopeArgs a = {dy, (const bf16_t*)pre, (bf16_t*)dz, (bf16_t*)dzt, dbias ? (float*)scratch : nullptr, N, ld_dz, ld_dzt, M, N, run_rows(M, N), act,
-                         act == MVIT_ACT_SILU ? 1.f : TANH_K, act == MVIT_ACT_SILU ? 0.f : TANH_K * 0.044715f};
+    const SlopeArgs a = {dy, (const bf16_t*)pre, (bf16_t*)dz, (bf16_t*)dzt, dbias ? (float*)scratch : nullptr, N, ld_dz, ld_dzt, M, N, run_rows(M, N), act};
     if (N % 8 == 0 && aligned16(dy) && aligned16(pre)) {
       const dim3 grid((N + 63) / 64, runs);
       dy_f32 ? launch_tiles<true>(a, grid, s) : launch_tiles<false>(a, grid, s);

@@ -32,12 +32,12 @@ struct Args {
   unsigned ldx, ldw; // row strides in bytes
   int M, N, kb;      // kb: bytes of a row of x and W
   int act, bias_f32;
-  float act_lo, act_a, act_b;   // constants of the activation's class, see activate()
+  float act_lo;   // -inf, or 0 for relu
 };
 
 // What a tile kernel is compiled for besides its operands.  The epilogue is unrolled over the accumulators: with every activation and
 // output in one kernel it was 9800 instructions, more than the instruction cache holds, and cost 3 us a tile instead of 1.
-enum Act { A_CLIP, A_SIGMOID, A_ERF, A_ANY };
+enum Act { A_CLIP, A_SILU, A_TANH, A_ERF, A_ANY };
 template <bool OUT32, int ACT, bool VEC>   // VEC: rows of y, pre and res start on 16 bytes and N % 8 == 0; else by elements
 struct End {
   static constexpr bool out32 = OUT32, vec = VEC;
@@ -65,19 +65,23 @@ __device__ __forceinline__ float normal_cdf(float z) {
   const float q = half_erfc(fabsf(z));
   return z >= 0.f ? 1.f - q : q;
 }
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504089f * z)); }
-constexpr float TANH_K = 1.5957691216f;   // 2 sqrt(2 / pi)
+constexpr float LOG2E = 1.44269504089f;
+__device__ __forceinline__ float sigmoid2(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-u)); }   // of u / log2 e
 
-// Three classes: none and relu clip at act_lo (-inf, 0; a NaN stays one); silu and gelu_tanh are z sigmoid(z (a + b z^2)) with
-// (1, 0) and 2 sqrt(2 / pi) (1, 0.044715) -- (1 + tanh u) / 2 = sigmoid(2 u); gelu is z Phi(z).
+constexpr float TANH_A = LOG2E * 1.5957691216f, TANH_B = TANH_A * 0.044715f;   // 2 sqrt(2 / pi), log2 e
+
+// none and relu clip at act_lo (a NaN stays one); silu is z s(z), gelu_tanh z s(2 sqrt(2 / pi) (z + 0.044715 z^3)), as
+// (1 + tanh u) / 2 = s(2 u) for the logistic function s; gelu is z Phi(z)
 template <int ACT>
 __device__ __forceinline__ float activated(const Args& p, float z) {
-  if constexpr (ACT == A_CLIP) return z < p.act_lo ? p.act_lo : z;
-  if constexpr (ACT == A_SIGMOID) return z * sigmoid(z * __builtin_fmaf(z * z, p.act_b, p.act_a));
+  if constexpr (ACT == A_CLIP) return __builtin_elementwise_maximum(z, p.act_lo);
+  if constexpr (ACT == A_SILU) return z * sigmoid2(LOG2E * z);
+  if constexpr (ACT == A_TANH) return z * sigmoid2(z * __builtin_fmaf(z * z, TANH_B, TANH_A));
   if constexpr (ACT == A_ERF) return z * normal_cdf(z);
-  return p.act == MVIT_ACT_GELU ? z * normal_cdf(z)
-         : p.act == MVIT_ACT_SILU || p.act == MVIT_ACT_GELU_TANH ? z * sigmoid(z * __builtin_fmaf(z * z, p.act_b, p.act_a))
-                                                                  : z < p.act_lo ? p.act_lo : z;
+  return p.act == MVIT_ACT_GELU        ? activated<A_ERF>(p, z)
+         : p.act == MVIT_ACT_SILU      ? activated<A_SILU>(p, z)
+         : p.act == MVIT_ACT_GELU_TANH ? activated<A_TANH>(p, z)
+                                       : activated<A_CLIP>(p, z);
 }
 
 __device__ __forceinline__ float value_of(const void* p, size_t i, bool f32) { return f32 ? ((const float*)p)[i] : bf2f(((const bf16_t*)p)[i]); }

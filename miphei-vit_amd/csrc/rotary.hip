@@ -5,7 +5,10 @@
 // with (a, b) = values (i, i + P), or (2i, 2i + 1) where interleaved.  The gradient is the same turn by the negative angle.
 //
 // Bound by HBM (each value in once, out once); the sines cost as much as the rest if every head computed them again, so
-//  * a block takes TOKENS tokens and writes their P (cos, sin) pairs into LDS once; all heads of q and k read them from there;
+//  * a block takes one token (as many as give its 256 threads work, where heads are few) and writes its P (cos, sin) pairs into LDS
+//    once; all heads of q and k read them from there.  One token a block keeps the most loads on their way: packed bf16 [64, 329, 72, 64]
+//    forward and backward 135 us, 144 with two tokens a block, 152 with four; f32 [1, 10376, 16, 128] head-major 32 / 36 / 40 us
+//    (5.7 and 5.4 TB/s);
 //  * an angle is formed and reduced to one revolution in f64 (position * inv_freq / 2 pi: a far position's angle in f32 is off by more
 //    than a bf16 step from position 2^14 on), the sine of the remainder in f32;
 //  * a thread moves VEC values of both halves of a pair block (16-byte loads at VEC = 8 and 16-bit values).
@@ -28,7 +31,9 @@ struct RotArgs {
   int pos_type, freq_f64;             // 0 int32, 1 int64, 2 f32
   float sign;
   int copy;                           // 0: in place, nothing passes through
-  unsigned rot_units, pass_units;     // units of a token behind the prefix
+  unsigned rot_units, pass_units;     // units of a token: a thread's work at once
+  int tokens;                         // of a block
+  unsigned per_magic;
   unsigned rpu, rpu_magic;            // rotated units of a head
   unsigned tail, tail_magic;          // passing units of a rotated head
   unsigned full, full_magic;          // units of a whole head
@@ -110,14 +115,12 @@ __device__ __forceinline__ void copy_piece(const void* x, size_t i, void* y, siz
   }
 }
 
-constexpr int ROT_TOKENS = 4;   // tokens of a block
-
 template <bool F, int VEC, bool IL>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
-  extern __shared__ float2 turn[];   // [ROT_TOKENS][P]
+  extern __shared__ float2 turn[];   // [tokens of the block][P]
   const int tid = threadIdx.x;
-  const int n0 = blockIdx.x * ROT_TOKENS, b = blockIdx.y;
-  const int nt = min(ROT_TOKENS, p.N - n0);
+  const int n0 = blockIdx.x * p.tokens, b = blockIdx.y;
+  const int nt = min(p.tokens, p.N - n0);
   for (int i = tid; i < nt * p.P; i += 256) {
     const int k = i / p.P, pair = i - k * p.P, n = n0 + k - p.prefix;
     if (n < 0) continue;
@@ -133,59 +136,56 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
   }
   __syncthreads();
   const unsigned per = p.rot_units + p.pass_units;
-  for (int k = 0; k < nt; ++k) {
-    const size_t xt = (size_t)b * p.xb + (size_t)(n0 + k) * p.xn, yt = (size_t)b * p.yb + (size_t)(n0 + k) * p.yn;
-    if (n0 + k < p.prefix) {   // the whole token passes
-      if (!p.copy) continue;
-      for (unsigned u = tid; u < (unsigned)p.H * p.full; u += 256) {
-        const unsigned h = mvit_fast_div(u, p.full, p.full_magic), j = u - h * p.full;
-        copy_piece<F, VEC>(p.x, xt + (size_t)h * p.xh + j * VEC, p.y, yt + (size_t)h * p.yh + j * VEC);
+  for (unsigned i = tid; i < (unsigned)nt * per; i += 256) {
+    const unsigned k = p.tokens == 1 ? 0u : mvit_fast_div(i, per, p.per_magic), u = i - k * per;
+    const int n = n0 + (int)k;
+    const size_t xt = (size_t)b * p.xb + (size_t)n * p.xn, yt = (size_t)b * p.yb + (size_t)n * p.yn;
+    if (u < p.rot_units) {
+      const unsigned h = mvit_fast_div(u, p.rpu, p.rpu_magic), j = (u - h * p.rpu) * VEC;
+      const size_t xi = xt + (size_t)h * p.xh + j, yi = yt + (size_t)h * p.yh + j;
+      if (n < p.prefix) {   // the whole token passes
+        if (p.copy) {
+          copy_piece<F, VEC>(p.x, xi, p.y, yi);
+          if constexpr (!IL) copy_piece<F, VEC>(p.x, xi + p.P, p.y, yi + p.P);
+        }
+        continue;
       }
-      continue;
-    }
-    const float2* cs = turn + k * p.P;
-    for (unsigned u = tid; u < per; u += 256) {
-      if (u < p.rot_units) {
-        const unsigned h = mvit_fast_div(u, p.rpu, p.rpu_magic), j = (u - h * p.rpu) * VEC;
-        const size_t xi = xt + (size_t)h * p.xh + j, yi = yt + (size_t)h * p.yh + j;
-        if constexpr (IL) {
-          Piece<F, VEC> a;
-          a.load(p.x, xi);
+      const float2* cs = turn + k * p.P + (IL ? j / 2 : j);
+      Piece<F, VEC> a;
+      a.load(p.x, xi);
+      if constexpr (IL) {
 #pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            const float2 t = cs[(j + e) >> 1];
-            const float u0 = a.v[e], u1 = a.v[e + 1];
-            a.v[e] = u0 * t.x - u1 * t.y;
-            a.v[e + 1] = u1 * t.x + u0 * t.y;
-          }
-          a.store(p.y, yi);
-        } else {
-          Piece<F, VEC> a, c;
-          a.load(p.x, xi);
-          c.load(p.x, xi + p.P);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float2 t = cs[j + e];
-            const float u0 = a.v[e], u1 = c.v[e];
-            a.v[e] = u0 * t.x - u1 * t.y;
-            c.v[e] = u1 * t.x + u0 * t.y;
-          }
-          a.store(p.y, yi);
-          c.store(p.y, yi + p.P);
+        for (int e = 0; e < VEC; e += 2) {
+          const float2 t = cs[e / 2];
+          const float u0 = a.v[e], u1 = a.v[e + 1];
+          a.v[e] = u0 * t.x - u1 * t.y;
+          a.v[e + 1] = u1 * t.x + u0 * t.y;
         }
       } else {
-        unsigned v = u - p.rot_units, h, j;
-        if (v < (unsigned)p.rot * p.tail) {   // tails of the rotated heads
-          h = mvit_fast_div(v, p.tail, p.tail_magic);
-          j = 2 * p.P + (v - h * p.tail) * VEC;
-        } else {                              // heads that pass
-          v -= (unsigned)p.rot * p.tail;
-          h = mvit_fast_div(v, p.full, p.full_magic);
-          j = (v - h * p.full) * VEC;
-          h += p.rot;
+        Piece<F, VEC> c;
+        c.load(p.x, xi + p.P);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float2 t = cs[e];
+          const float u0 = a.v[e], u1 = c.v[e];
+          a.v[e] = u0 * t.x - u1 * t.y;
+          c.v[e] = u1 * t.x + u0 * t.y;
         }
-        copy_piece<F, VEC>(p.x, xt + (size_t)h * p.xh + j, p.y, yt + (size_t)h * p.yh + j);
+        c.store(p.y, yi + p.P);
       }
+      a.store(p.y, yi);
+    } else {
+      unsigned v = u - p.rot_units, h, j;
+      if (v < (unsigned)p.rot * p.tail) {   // tails of the rotated heads
+        h = mvit_fast_div(v, p.tail, p.tail_magic);
+        j = 2 * p.P + (v - h * p.tail) * VEC;
+      } else {                              // heads that pass
+        v -= (unsigned)p.rot * p.tail;
+        h = mvit_fast_div(v, p.full, p.full_magic);
+        j = (v - h * p.full) * VEC;
+        h += p.rot;
+      }
+      copy_piece<F, VEC>(p.x, xt + (size_t)h * p.xh + j, p.y, yt + (size_t)h * p.yh + j);
     }
   }
 }
@@ -198,8 +198,12 @@ int launch(RotArgs a, hipStream_t s) {
   a.full = full, a.full_magic = mvit_div_magic(full);
   a.rot_units = (unsigned)a.rot * rpu;
   a.pass_units = a.copy ? (unsigned)a.rot * tail + (unsigned)(a.H - a.rot) * full : 0u;
-  const dim3 grid((a.N + ROT_TOKENS - 1) / ROT_TOKENS, a.B);
-  hipLaunchKernelGGL((rotary_kernel<F, VEC, IL>), grid, dim3(256), (size_t)ROT_TOKENS * a.P * sizeof(float2), s, a);
+  const unsigned per = a.rot_units + a.pass_units;
+  if (per == 0) return MVIT_OK;   // (in place with no head to turn)
+  a.tokens = per >= 256 ? 1 : 256 / per < 32 ? 256 / per : 32;
+  a.per_magic = mvit_div_magic(per);
+  const dim3 grid((a.N + a.tokens - 1) / a.tokens, a.B);
+  hipLaunchKernelGGL((rotary_kernel<F, VEC, IL>), grid, dim3(256), (size_t)a.tokens * a.P * sizeof(float2), s, a);
   return MVIT_LAUNCH_CHECK();
 }
 

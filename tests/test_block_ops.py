@@ -641,6 +641,31 @@ def test_linear_act_gradient_against_differences(act):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_linear_act_far_values(act, M):
+    """z of infinities, a NaN and the largest values: what the definition gives, forward and slope (z is the bias)"""
+    ops = T()
+    z = torch.tensor([float("inf"), float("-inf"), float("nan"), 3e38, -3e38, 1e25, -1e25, 100.0, -100.0, 0.0, -0.0, 1e-30, -1e-38, 30.0, -30.0, 8.0],
+                     device="cuda").repeat(4)
+    x = torch.zeros(M, 8, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(64, 8, device="cuda", dtype=torch.bfloat16)
+    b = z.clone().requires_grad_()
+    y = ops.linear_act(x, w, b, torch.zeros(M, 64, device="cuda"), act)
+    want, slope = act_oracle(z.double(), act)
+    kept, got = y.detach()[M // 2].double(), want
+    assert torch.equal(kept.isnan(), got.isnan())
+    fine = got.isfinite()
+    assert torch.equal(kept[~fine & ~got.isnan()], got[~fine & ~got.isnan()])
+    assert ((kept - got)[fine].abs() <= 1e-5 * got[fine].abs() + 1e-5).all()      # (1.5e-7 of erf times |z| = 30, and f32)
+    (db,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    far = {"none": (1.0, 1.0)}.get(act, (1.0, 0.0))      # at the infinities: the limits
+    slope = torch.where(z == math.inf, far[0], torch.where(z == -math.inf, far[1], slope))
+    assert torch.equal(db.isnan(), z.isnan() & (act != "none"))
+    assert ((db.double() / M - slope)[~z.isnan()].abs() < 1e-4).all()
+
+
+@pytest.mark.gpu
 def test_linear_act_options():
     ops, g = T(), gen(21)
     x, w, b, r = linear_case(g, 37, 64, 48, torch.bfloat16, torch.float32, True)
