@@ -170,7 +170,7 @@ MVIT_API int mvit_attention_bwd(const void* qkv, const void* out, const void* ou
 /* Root-mean-square norm of a residual stream.  h = x + res (kept in res's type; what is normed is h as it is stored),
  * y = h / sqrt(mean(h^2) + eps) * w, rstd(f32)[M] (optional) = 1 / sqrt(...) for the backward pass.  *_f32 != 0: that operand is f32,
  * else 16-bit; row strides ldx, ldr in elements, h and y are dense [M, D].  res = NULL: h is x and is not written.
- * x 16-bit: res 16-bit or f32, y 16-bit.  x f32: res f32, y 16-bit or f32.  1 <= D <= 16384, any D and any alignment (16-byte loads
+ * x 16-bit: res 16-bit or f32, y 16-bit.  x f32: res f32, y 16-bit or f32.  1 <= D <= 16384, M <= 2^30, any D and any alignment (16-byte loads
  * where D % 8 == 0 and all rows start on 16 bytes). */
 MVIT_API int mvit_rmsnorm_fwd(const void* x, int x_f32, long long ldx, const void* res, int res_f32, long long ldr, const void* w,
                               int w_f32, void* h, void* y, int y_f32, float* rstd, int M, int D, float eps, mvit_stream_t stream);
@@ -193,7 +193,7 @@ MVIT_API int mvit_rmsnorm_bwd(const void* dy, int x_f32, const void* dh, const v
  * where interleaved, and turns by positions[n - prefix][axis of i] * inv_freq[i]; sections[a] consecutive pairs belong to axis a.
  * Tokens before prefix, heads from rotate_heads on and values from 2P on pass through.  inverse != 0: by the negative angle (the
  * gradient).  positions [N - prefix, axes], pos_b elements apart per batch entry (0: shared), pos_type 0 int32, 1 int64, 2 f32;
- * inv_freq [P] f64 (freq_f64) or f32.  Dh even, <= 1024; H <= 1024; B <= 65535. */
+ * inv_freq [P] f64 (freq_f64) or f32.  Dh even, <= 1024; H <= 1024; B <= 65535; N <= 2^30. */
 typedef struct mvit_rotary_args {
   const void* x; void* y; const void* positions; const void* inv_freq;
   long long xb, xn, xh, yb, yn, yh, pos_b;
@@ -207,7 +207,7 @@ MVIT_API int mvit_rotary(const mvit_rotary_args* args, mvit_stream_t stream);
  * receives the value in front of the activation for the backward pass.  mvit_linear_fp8: e4m3 x, W, the product times
  * x_scale(f32)[m] * w_scale(f32)[n]; no pre.  bias [N] f32 or 16-bit, may be NULL.  y dense, f32 or 16-bit; res (may be NULL) has y's type
  * and its own row stride ldr.  ldx, ldw, ldr in elements.  x, W rows start on 16 bytes and K is a multiple of 16 bytes (8 or 16 values);
- * K and the row strides of x and W are at most 2^23 bytes.  M, N of any size. */
+ * K and the row strides of x and W are at most 2^23 bytes.  M up to 2^30, N up to 2^24, of any size. */
 enum mvit_activation { MVIT_ACT_NONE = 0, MVIT_ACT_RELU = 1, MVIT_ACT_SILU = 2, MVIT_ACT_GELU = 3, MVIT_ACT_GELU_TANH = 4 };
 typedef struct mvit_linear_args {
   const void* x; const void* w; const void* bias; const void* res; void* y; void* pre; const float* x_scale; const float* w_scale;

@@ -65,11 +65,13 @@ int dispatch(Args& a, bool vec, hipStream_t s) {
   }
 }
 
+constexpr int MAX_M = 1 << 30, MAX_N = 1 << 24;   // tile numbers and grids stay in 31 bits
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // 0: go on, 1: nothing to do, < 0: refused.  es: bytes of an operand's value.
 int check(const mvit_linear_args* g, int es, Args& a, bool& vec) {
-  if (!g || g->M < 0 || g->N <= 0 || g->K <= 0) return MVIT_EINVAL;
+  if (!g || g->M < 0 || g->M > MAX_M || g->N <= 0 || g->N > MAX_N || g->K <= 0) return MVIT_EINVAL;
   if (g->M == 0) return 1;   // (an empty tensor has no address)
   if (!g->x || !g->w || !g->y) return MVIT_EINVAL;
   if (g->act < MVIT_ACT_NONE || g->act > MVIT_ACT_GELU_TANH) return MVIT_EINVAL;
@@ -257,7 +259,7 @@ void launch_tiles(const SlopeArgs& a, dim3 grid, hipStream_t s) {
 
 extern "C" MVIT_API int mvit_transpose_padded(const void* src, long long ld, void* dst, long long ld_dst, int R, int Cc, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
-  if (!src || !dst || R <= 0 || Cc <= 0 || ld % 8 || ld_dst % 8 || ld < (Cc + 7) / 8 * 8 || ld_dst < R || ld_dst >= R + 8 || !aligned16(src) || !aligned16(dst))
+  if (!src || !dst || R <= 0 || R > MAX_M || Cc <= 0 || Cc > MAX_N || ld % 8 || ld_dst % 8 || ld < (Cc + 7) / 8 * 8 || ld_dst < R || ld_dst >= R + 8 || !aligned16(src) || !aligned16(dst))
     return MVIT_EINVAL;
   SlopeArgs a = {};
   a.dy = src, a.dzt = (bf16_t*)dst, a.ld = ld, a.ld_dzt = ld_dst, a.M = R, a.N = Cc, a.rows = run_rows(R, Cc), a.act = MVIT_ACT_NONE;
@@ -270,7 +272,7 @@ extern "C" MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N) { return 
 extern "C" MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dzt, long long ld_dzt,
                                      void* dbias, int dbias_f32, void* scratch, int M, int N, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
-  if (M < 0 || N <= 0 || (M > 0 && !dy) || act < MVIT_ACT_NONE || act > MVIT_ACT_GELU_TANH || (act != MVIT_ACT_NONE && M > 0 && !pre)) return MVIT_EINVAL;
+  if (M < 0 || M > MAX_M || N <= 0 || N > MAX_N || (M > 0 && !dy) || act < MVIT_ACT_NONE || act > MVIT_ACT_GELU_TANH || (act != MVIT_ACT_NONE && M > 0 && !pre)) return MVIT_EINVAL;
   if (dbias && M > 0 && !scratch) return MVIT_EINVAL;
   if ((dz && (ld_dz < N || ld_dz % 8 || !aligned16(dz))) || (dzt && (!dz || ld_dzt < M || ld_dzt >= M + 8 || ld_dzt % 8 || !aligned16(dzt))))
     return MVIT_EINVAL;

@@ -7,12 +7,12 @@
 //
 // All of it is bound by HBM: a row is read once, lives in registers (f32) while its sum of squares, its largest value and its outputs
 // are formed, and is written once.
-//  * A row belongs to TPR = 64 threads (one wave: no barrier) or, from D > 4096 on or where there are fewer rows than the chip has
-//    waves, to 256 (the row's latency then counts, and a quarter of the loads per thread is what shortens it).
+//  * A row belongs to TPR = 64 threads (one wave: no barrier) or to a block (fewer registers and loads a thread: for wide rows, and for
+//    few, whose latency counts).
 //  * Each thread holds NV pieces of VEC values; VEC = 8 (16-byte loads) where D, the row strides and the addresses allow it, else 1.
 //  * Rows are walked with a grid stride, so that w is loaded once per thread and not once per row.
-// Measured against a 1 GiB copy's 5.05 TB/s (one MI355X): f32 stream of [21056, 1536] forward 76 us (388 MB, 5.1 TB/s), backward 109 us
-// (517 MB, 4.8 TB/s) and 5 us for d w; 16-bit stream to 8 bits [20816, 1536] 37 us (6.0 TB/s); quantisation [21056, 4096] 47 us (5.5 TB/s).
+// Measured against a 1 GiB copy's 5.05 TB/s (one MI355X): f32 stream of [21056, 1536] forward 75 us (388 MB, 5.2 TB/s), backward with
+// d w 96 us (517 MB, 5.4 TB/s); 16-bit stream to 8 bits [20816, 1536] 37 us (6.0 TB/s); quantisation [21056, 4096] 43 us (6.0 TB/s).
 // Sums and statistics are f32; sums over the rows (d w) go row by row in registers, over the waves of a block in LDS, over the blocks
 // through a [blocks][D] f32 workspace that a second launch adds up: a fixed order, no atomics, bit-identical from run to run.
 #include "column_sums.hpp"
@@ -220,11 +220,12 @@ struct BwdArgs {
   int M, D, w_f32;
 };
 
-// XT: the type of dy and dx; HT: the type of h, dh and dres.  One wave (TPR = 64) or 512 threads a row, 512 threads a block.
-template <int TPR, int NV, int VEC, int XT, int HT>
-__global__ __launch_bounds__(512) void rms_bwd(const BwdArgs p) {
-  constexpr int RPB = 512 / TPR;
-  extern __shared__ float lds[];   // TPR = 64: D floats (the block's sum of d w); 512: 2 * 8 words of the row sums
+// XT: the type of dy and dx; HT: the type of h, dh and dres.  Blocks of NT threads, a row to a wave (TPR = 64) or to the block (TPR = NT).
+template <int NT, int TPR, int NV, int VEC, int XT, int HT>
+__global__ __launch_bounds__(NT) void rms_bwd(const BwdArgs p) {
+  constexpr int RPB = NT / TPR;
+  static_assert(RPB == 1 || TPR == 64, "rows that share a barrier would have to end together");
+  extern __shared__ float lds[];   // TPR = 64: D floats (the block's sum of d w); else 2 * 8 words of the row sums
   int turn = 0;
   const int t = threadIdx.x % TPR;
   float w[NV][VEC], acc[NV][VEC];
@@ -284,9 +285,9 @@ __global__ __launch_bounds__(512) void rms_bwd(const BwdArgs p) {
   if (!p.part) return;
   float* out = p.part + (size_t)blockIdx.x * p.D;
   if constexpr (TPR == 64) {
-    for (int c = threadIdx.x; c < p.D; c += 512) lds[c] = 0.f;
+    for (int c = threadIdx.x; c < p.D; c += NT) lds[c] = 0.f;
     __syncthreads();
-    for (int k = 0; k < 8; ++k) {   // wave after wave: a fixed order
+    for (int k = 0; k < NT / 64; ++k) {   // wave after wave: a fixed order
       if ((int)(threadIdx.x >> 6) == k) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(512) void rms_bwd(const BwdArgs p) {
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < p.D; c += 512) out[c] = lds[c];
+    for (int c = threadIdx.x; c < p.D; c += NT) out[c] = lds[c];
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(512) void rms_bwd(const BwdArgs p) {
   }
 }
 
-constexpr int MAX_D = 16384;
+constexpr int MAX_D = 16384, MAX_M = 1 << 30;   // (row numbers run past M by a grid's stride)
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -316,7 +317,7 @@ template <int TPR, int NV, int VEC, int XT, int RT, int YT, bool NORM>
 int launch_fwd(const RowArgs& a, hipStream_t s) {
   const int rpb = 256 / TPR;
   // rounds of the grid stride: [20816, 1536] bf16 to 8 bits 40 us with 8 blocks a CU, 37 with 16, 39 with as many as rows; wider rows hold
-  // more registers and loads a thread: [21056, 4096] quantised 47, 49, 51 us
+  // more registers and loads a thread
   const long long need = ((long long)a.M + rpb - 1) / rpb, most = (long long)mvit_num_cus() * (a.D <= 2048 ? 16 : 8);
   hipLaunchKernelGGL((rms_fwd<TPR, NV, VEC, XT, RT, YT, NORM>), dim3((unsigned)(need < most ? need : most)), dim3(256), 0, s, a);
   return MVIT_LAUNCH_CHECK();
@@ -326,12 +327,14 @@ template <int XT, int RT, int YT, bool NORM>
 int fwd_layout(const RowArgs& a, bool vec, hipStream_t s) {
   const int D = a.D;
   if (vec) {
-    if (D <= 4096 && a.M >= 4 * mvit_num_cus()) {
-      if (D <= 512) return launch_fwd<64, 1, 8, XT, RT, YT, NORM>(a, s);
+    // a wave a row, or 256 threads (f32 stream to 8 bits, us): rows of 512: 1024 of them 3.1 / 3.8, 8192 9.1 / 12.1; of 1024: 256 3.4 / 3.2,
+    // 1024 4.1 / 4.3, 8192 15.7 / 16.5; of 1536: 256 4.1 / 3.4, 2048 7.6 / 6.9, 3072 9.7 / 10.6, 4096 12.0 / 13.2; of 4096: 64 6.9 / 3.7,
+    // 8192 83 / 75
+    if (D <= 512) return launch_fwd<64, 1, 8, XT, RT, YT, NORM>(a, s);
+    if (D <= 2048 && a.M >= (D <= 1024 ? 4 : 12) * mvit_num_cus()) {
       if (D <= 1024) return launch_fwd<64, 2, 8, XT, RT, YT, NORM>(a, s);
       if (D <= 1536) return launch_fwd<64, 3, 8, XT, RT, YT, NORM>(a, s);
-      if (D <= 2048) return launch_fwd<64, 4, 8, XT, RT, YT, NORM>(a, s);
-      return launch_fwd<64, 8, 8, XT, RT, YT, NORM>(a, s);
+      return launch_fwd<64, 4, 8, XT, RT, YT, NORM>(a, s);
     }
     if (D <= 2048) return launch_fwd<256, 1, 8, XT, RT, YT, NORM>(a, s);
     if (D <= 4096) return launch_fwd<256, 2, 8, XT, RT, YT, NORM>(a, s);
@@ -352,40 +355,43 @@ bool vec_ok(const RowArgs& a) {
 
 // (an empty tensor has no address: pointers are asked for where there are rows)
 bool rows_bad(const RowArgs& a) {
-  if (a.M < 0 || a.D <= 0 || a.D > MAX_D) return true;
+  if (a.M < 0 || a.M > MAX_M || a.D <= 0 || a.D > MAX_D) return true;
   return a.M > 0 && (!a.x || !a.y || a.ldx < a.D || (a.res && (!a.h || a.ldr < a.D)));
 }
 
-template <int TPR, int NV, int VEC, int XT, int HT>
-int launch_bwd(const BwdArgs& a, int grid, hipStream_t s) {
+// blocks of the backward pass at most, and so partial sums of d w: a CU's 1024 threads
+int bwd_blocks(int M, int nt) {
+  const long long most = (long long)mvit_num_cus() * (1024 / nt);
+  return (int)(M < most ? M : most);
+}
+
+template <int NT, int TPR, int NV, int VEC, int XT, int HT>
+int launch_bwd(const BwdArgs& a, int& grid, hipStream_t s) {
   const size_t lds = TPR == 64 ? (size_t)a.D * 4 : 64;
-  hipLaunchKernelGGL((rms_bwd<TPR, NV, VEC, XT, HT>), dim3(grid), dim3(512), lds, s, a);
+  constexpr int RPB = NT / TPR;
+  grid = bwd_blocks((a.M + RPB - 1) / RPB, NT);
+  hipLaunchKernelGGL((rms_bwd<NT, TPR, NV, VEC, XT, HT>), dim3(grid), dim3(NT), lds, s, a);
   return MVIT_LAUNCH_CHECK();
 }
 
 template <int XT, int HT>
-int bwd_layout(const BwdArgs& a, bool vec, int grid, hipStream_t s) {
+int bwd_layout(const BwdArgs& a, bool vec, int& grid, hipStream_t s) {
   const int D = a.D;
   if (vec) {
-    if (D <= 512) return launch_bwd<64, 1, 8, XT, HT>(a, grid, s);
-    if (D <= 1024) return launch_bwd<64, 2, 8, XT, HT>(a, grid, s);
-    if (D <= 1536) return launch_bwd<64, 3, 8, XT, HT>(a, grid, s);
-    if (D <= 2048) return launch_bwd<64, 4, 8, XT, HT>(a, grid, s);
-    if (D <= 4096) return launch_bwd<512, 1, 8, XT, HT>(a, grid, s);
-    if (D <= 8192) return launch_bwd<512, 2, 8, XT, HT>(a, grid, s);
-    return launch_bwd<512, 4, 8, XT, HT>(a, grid, s);
+    // f32 stream, with d w, us.  A wave a row or a block: rows of 1024: 1024 of them 9.6 / 8.1, 4096 17.5 / 17.7, 8192 26 / 28, 21056 69 / 87;
+    // of 1536: 21056 107 / 105; of 2048: 140 / 127.  A row to 256 threads or to 512: of 1536: 1024 11.1 / 9.0 (twice the partial sums of
+    // d w), 8192 35 / 34, 21056 96 / 105; of 2048: 131 / 126
+    if (D <= 512) return launch_bwd<512, 64, 1, 8, XT, HT>(a, grid, s);
+    if (D <= 1024 && a.M >= 16 * mvit_num_cus()) return launch_bwd<512, 64, 2, 8, XT, HT>(a, grid, s);
+    if (D <= 1536 && a.M >= 32 * mvit_num_cus()) return launch_bwd<256, 256, 1, 8, XT, HT>(a, grid, s);
+    if (D <= 4096) return launch_bwd<512, 512, 1, 8, XT, HT>(a, grid, s);
+    if (D <= 8192) return launch_bwd<512, 512, 2, 8, XT, HT>(a, grid, s);
+    return launch_bwd<512, 512, 4, 8, XT, HT>(a, grid, s);
   }
-  if (D <= 512) return launch_bwd<64, 8, 1, XT, HT>(a, grid, s);
-  if (D <= 1024) return launch_bwd<64, 16, 1, XT, HT>(a, grid, s);
-  if (D <= 4096) return launch_bwd<512, 8, 1, XT, HT>(a, grid, s);
-  return launch_bwd<512, 32, 1, XT, HT>(a, grid, s);
-}
-
-// blocks of the backward pass, which is also the number of partial sums of d w: two blocks of 512 threads a CU, no more than there are
-// rows for (8 rows a block where a wave has a row: D <= 2048 by vectors, D <= 1024 by elements; the smaller bound counts for both)
-int bwd_blocks(int M, int D) {
-  const long long rows = D <= 2048 ? 8 : 1, need = ((long long)M + rows - 1) / rows, most = (long long)mvit_num_cus() * 2;
-  return (int)(need < most ? need : most);
+  if (D <= 512) return launch_bwd<512, 64, 8, 1, XT, HT>(a, grid, s);
+  if (D <= 1024) return launch_bwd<512, 64, 16, 1, XT, HT>(a, grid, s);
+  if (D <= 4096) return launch_bwd<512, 512, 8, 1, XT, HT>(a, grid, s);
+  return launch_bwd<512, 512, 32, 1, XT, HT>(a, grid, s);
 }
 
 }  // namespace
@@ -433,17 +439,17 @@ extern "C" MVIT_API int mvit_quantize_rows_fp8(const void* x, int x_f32, long lo
 }
 
 extern "C" MVIT_API long long mvit_rmsnorm_bwd_scratch_bytes(int M, int D) {
-  return M <= 0 || D <= 0 ? 0 : (long long)bwd_blocks(M, D) * D * 4;
+  return M <= 0 || D <= 0 ? 0 : (long long)bwd_blocks(M, 256) * D * 4;
 }
 
 extern "C" MVIT_API int mvit_rmsnorm_bwd(const void* dy, int x_f32, const void* dh, const void* h, int h_f32, const void* w, int w_f32,
                                          const float* rstd, void* dx, void* dres, void* dw, void* scratch, long long scratch_bytes, int M,
                                          int D, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
-  if (M < 0 || D <= 0 || D > MAX_D || !w || (M > 0 && (!dy || !h || !rstd)) || (x_f32 && !h_f32)) return MVIT_EINVAL;
+  if (M < 0 || M > MAX_M || D <= 0 || D > MAX_D || !w || (M > 0 && (!dy || !h || !rstd)) || (x_f32 && !h_f32)) return MVIT_EINVAL;
   if (dw && M > 0 && (!scratch || scratch_bytes < mvit_rmsnorm_bwd_scratch_bytes(M, D))) return MVIT_EINVAL;
   hipStream_t s = (hipStream_t)stream;
-  const int grid = M > 0 ? bwd_blocks(M, D) : 0;
+  int grid = 0;
   if (M > 0) {
     const BwdArgs a = {dy, dh, h, w, rstd, dx, dres, dw ? (float*)scratch : nullptr, M, D, w_f32};
     const bool v = D % 8 == 0 && aligned16(dy) && aligned16(dh) && aligned16(h) && aligned16(w) && aligned16(dx) && aligned16(dres) && aligned16(scratch);

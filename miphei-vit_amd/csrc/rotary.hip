@@ -118,75 +118,77 @@ __device__ __forceinline__ void copy_piece(const void* x, size_t i, void* y, siz
 template <bool F, int VEC, bool IL>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
   extern __shared__ float2 turn[];   // [tokens of the block][P]
-  const int tid = threadIdx.x;
-  const int n0 = blockIdx.x * p.tokens, b = blockIdx.y;
-  const int nt = min(p.tokens, p.N - n0);
-  for (int i = tid; i < nt * p.P; i += 256) {
-    const int k = i / p.P, pair = i - k * p.P, n = n0 + k - p.prefix;
-    if (n < 0) continue;
-    const int axis = (pair >= p.end[0]) + (pair >= p.end[1]) + (pair >= p.end[2]);
-    const size_t at = (size_t)b * p.pos_b + (size_t)n * p.axes + axis;
-    const double f = p.freq_f64 ? ((const double*)p.freq)[pair] : (double)((const float*)p.freq)[pair];
-    const double q = p.pos_type == 0 ? (double)((const int*)p.pos)[at] : p.pos_type == 1 ? (double)((const long long*)p.pos)[at] : (double)((const float*)p.pos)[at];
-    double rev = q * f * 0.15915494309189533577;   // 1 / 2 pi
-    rev -= rint(rev);
-    float s, c;
-    sincospif((float)(2.0 * rev), &s, &c);
-    turn[i] = make_float2(c, s * p.sign);
-  }
-  __syncthreads();
-  const unsigned per = p.rot_units + p.pass_units;
-  for (unsigned i = tid; i < (unsigned)nt * per; i += 256) {
-    const unsigned k = p.tokens == 1 ? 0u : mvit_fast_div(i, per, p.per_magic), u = i - k * per;
-    const int n = n0 + (int)k;
-    const size_t xt = (size_t)b * p.xb + (size_t)n * p.xn, yt = (size_t)b * p.yb + (size_t)n * p.yn;
-    if (u < p.rot_units) {
-      const unsigned h = mvit_fast_div(u, p.rpu, p.rpu_magic), j = (u - h * p.rpu) * VEC;
-      const size_t xi = xt + (size_t)h * p.xh + j, yi = yt + (size_t)h * p.yh + j;
-      if (n < p.prefix) {   // the whole token passes
-        if (p.copy) {
-          copy_piece<F, VEC>(p.x, xi, p.y, yi);
-          if constexpr (!IL) copy_piece<F, VEC>(p.x, xi + p.P, p.y, yi + p.P);
-        }
-        continue;
-      }
-      const float2* cs = turn + k * p.P + (IL ? j / 2 : j);
-      Piece<F, VEC> a;
-      a.load(p.x, xi);
-      if constexpr (IL) {
-#pragma unroll
-        for (int e = 0; e < VEC; e += 2) {
-          const float2 t = cs[e / 2];
-          const float u0 = a.v[e], u1 = a.v[e + 1];
-          a.v[e] = u0 * t.x - u1 * t.y;
-          a.v[e + 1] = u1 * t.x + u0 * t.y;
-        }
-      } else {
-        Piece<F, VEC> c;
-        c.load(p.x, xi + p.P);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float2 t = cs[e];
-          const float u0 = a.v[e], u1 = c.v[e];
-          a.v[e] = u0 * t.x - u1 * t.y;
-          c.v[e] = u1 * t.x + u0 * t.y;
-        }
-        c.store(p.y, yi + p.P);
-      }
-      a.store(p.y, yi);
-    } else {
-      unsigned v = u - p.rot_units, h, j;
-      if (v < (unsigned)p.rot * p.tail) {   // tails of the rotated heads
-        h = mvit_fast_div(v, p.tail, p.tail_magic);
-        j = 2 * p.P + (v - h * p.tail) * VEC;
-      } else {                              // heads that pass
-        v -= (unsigned)p.rot * p.tail;
-        h = mvit_fast_div(v, p.full, p.full_magic);
-        j = (v - h * p.full) * VEC;
-        h += p.rot;
-      }
-      copy_piece<F, VEC>(p.x, xt + (size_t)h * p.xh + j, p.y, yt + (size_t)h * p.yh + j);
+  const int tid = threadIdx.x, b = blockIdx.y;
+  for (int n0 = blockIdx.x * p.tokens; n0 < p.N; n0 += gridDim.x * p.tokens) {   // (once, but for millions of tokens)
+    const int nt = min(p.tokens, p.N - n0);
+    for (int i = tid; i < nt * p.P; i += 256) {
+      const int k = i / p.P, pair = i - k * p.P, n = n0 + k - p.prefix;
+      if (n < 0) continue;
+      const int axis = (pair >= p.end[0]) + (pair >= p.end[1]) + (pair >= p.end[2]);
+      const size_t at = (size_t)b * p.pos_b + (size_t)n * p.axes + axis;
+      const double f = p.freq_f64 ? ((const double*)p.freq)[pair] : (double)((const float*)p.freq)[pair];
+      const double q = p.pos_type == 0 ? (double)((const int*)p.pos)[at] : p.pos_type == 1 ? (double)((const long long*)p.pos)[at] : (double)((const float*)p.pos)[at];
+      double rev = q * f * 0.15915494309189533577;   // 1 / 2 pi
+      rev -= rint(rev);
+      float s, c;
+      sincospif((float)(2.0 * rev), &s, &c);
+      turn[i] = make_float2(c, s * p.sign);
     }
+    __syncthreads();
+    const unsigned per = p.rot_units + p.pass_units;
+    for (unsigned i = tid; i < (unsigned)nt * per; i += 256) {
+      const unsigned k = p.tokens == 1 ? 0u : mvit_fast_div(i, per, p.per_magic), u = i - k * per;
+      const int n = n0 + (int)k;
+      const size_t xt = (size_t)b * p.xb + (size_t)n * p.xn, yt = (size_t)b * p.yb + (size_t)n * p.yn;
+      if (u < p.rot_units) {
+        const unsigned h = mvit_fast_div(u, p.rpu, p.rpu_magic), j = (u - h * p.rpu) * VEC;
+        const size_t xi = xt + (size_t)h * p.xh + j, yi = yt + (size_t)h * p.yh + j;
+        if (n < p.prefix) {   // the whole token passes
+          if (p.copy) {
+            copy_piece<F, VEC>(p.x, xi, p.y, yi);
+            if constexpr (!IL) copy_piece<F, VEC>(p.x, xi + p.P, p.y, yi + p.P);
+          }
+          continue;
+        }
+        const float2* cs = turn + k * p.P + (IL ? j / 2 : j);
+        Piece<F, VEC> a;
+        a.load(p.x, xi);
+        if constexpr (IL) {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float2 t = cs[e / 2];
+            const float u0 = a.v[e], u1 = a.v[e + 1];
+            a.v[e] = u0 * t.x - u1 * t.y;
+            a.v[e + 1] = u1 * t.x + u0 * t.y;
+          }
+        } else {
+          Piece<F, VEC> c;
+          c.load(p.x, xi + p.P);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float2 t = cs[e];
+            const float u0 = a.v[e], u1 = c.v[e];
+            a.v[e] = u0 * t.x - u1 * t.y;
+            c.v[e] = u1 * t.x + u0 * t.y;
+          }
+          c.store(p.y, yi + p.P);
+        }
+        a.store(p.y, yi);
+      } else {
+        unsigned v = u - p.rot_units, h, j;
+        if (v < (unsigned)p.rot * p.tail) {   // tails of the rotated heads
+          h = mvit_fast_div(v, p.tail, p.tail_magic);
+          j = 2 * p.P + (v - h * p.tail) * VEC;
+        } else {                              // heads that pass
+          v -= (unsigned)p.rot * p.tail;
+          h = mvit_fast_div(v, p.full, p.full_magic);
+          j = (v - h * p.full) * VEC;
+          h += p.rot;
+        }
+        copy_piece<F, VEC>(p.x, xt + (size_t)h * p.xh + j, p.y, yt + (size_t)h * p.yh + j);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -202,7 +204,8 @@ int launch(RotArgs a, hipStream_t s) {
   if (per == 0) return MVIT_OK;   // (in place with no head to turn)
   a.tokens = per >= 256 ? 1 : 256 / per < 32 ? 256 / per : 32;
   a.per_magic = mvit_div_magic(per);
-  const dim3 grid((a.N + a.tokens - 1) / a.tokens, a.B);
+  const int groups = (a.N + a.tokens - 1) / a.tokens;
+  const dim3 grid(groups < (1 << 22) ? groups : 1 << 22, a.B);   // (a grid has fewer than 2^32 threads in a dimension)
   hipLaunchKernelGGL((rotary_kernel<F, VEC, IL>), grid, dim3(256), (size_t)a.tokens * a.P * sizeof(float2), s, a);
   return MVIT_LAUNCH_CHECK();
 }
@@ -224,7 +227,7 @@ extern "C" MVIT_API int mvit_rotary(const mvit_rotary_args* args, mvit_stream_t 
   MVIT_CLEAR_ERROR();
   if (!args) return MVIT_EINVAL;
   const mvit_rotary_args& g = *args;
-  if (!g.x || !g.y || !g.inv_freq || g.B < 0 || g.N < 0 || g.H <= 0 || g.Dh <= 0 || (g.Dh & 1) || g.Dh > 1024 || g.H > 1024 || g.B > 65535)
+  if (!g.x || !g.y || !g.inv_freq || g.B < 0 || g.N < 0 || g.H <= 0 || g.Dh <= 0 || (g.Dh & 1) || g.Dh > 1024 || g.H > 1024 || g.B > 65535 || g.N > (1 << 30))
     return MVIT_EINVAL;   // H, Dh: the divisions by multiplication are exact below H * Dh^2 = 2^32
   if (g.rotate_heads < 0 || g.rotate_heads > g.H || g.prefix < 0 || g.prefix > g.N || g.axes < 1 || g.axes > 4) return MVIT_EINVAL;
   if (g.pos_type < 0 || g.pos_type > 2 || (g.prefix < g.N && !g.positions)) return MVIT_EINVAL;

@@ -86,7 +86,7 @@ void no_grad(const char* op, std::initializer_list<OptTensor> ts) {
     TORCH_CHECK(!t || !t->requires_grad(), "mvit::", op, " has no gradient: call it under torch.no_grad() or on detached tensors");
 }
 
-constexpr int64_t ROWS_MAX = 0x7fffffff;
+constexpr int64_t ROWS_MAX = 1 << 30;
 
 // ---------------------------------------------------------------- tensors as the kernels take them
 // [rows, last] view whose rows are dense, any row stride of at least their length; a copy only where there is none
@@ -122,7 +122,7 @@ std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
 HalfType norm_check(const char* op, const Tensor& x, const OptTensor& residual, const Tensor& weight, std::optional<ScalarType> out) {
   REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, op, "the last dimension must be 1 .. 16384");
   const int64_t d = x.size(-1);
-  REQUIRE(x.numel() / d <= ROWS_MAX, op, "more than 2^31 - 1 rows");
+  REQUIRE(x.numel() / d <= ROWS_MAX, op, "more than 2^30 rows");
   REQUIRE(weight.dim() == 1 && weight.size(0) == d, op, "weight ", weight.sizes(), " does not match input ", x.sizes());
   REQUIRE(!residual || residual->sizes() == x.sizes(), op, "residual ", residual->sizes(), " and input ", x.sizes(), " differ (it is not broadcast)");
   same_place(op, x, residual);
@@ -220,7 +220,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8_meta(const Tensor& x, const OptT
 
 HalfType quantize_check(const Tensor& x) {
   REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "quantize_fp8", "the last dimension must be 1 .. 16384");
-  REQUIRE(x.numel() / x.size(-1) <= ROWS_MAX, "quantize_fp8", "more than 2^31 - 1 rows");
+  REQUIRE(x.numel() / x.size(-1) <= ROWS_MAX, "quantize_fp8", "more than 2^30 rows");
   HalfType h{"quantize_fp8"};
   h.add(x);
   return h;
@@ -248,7 +248,7 @@ HalfType rotary_check(const char* op, const Tensor& x, const Tensor& positions, 
   REQUIRE(x.dim() == 4, op, "x must be [B, N, heads, head_dim], got ", x.sizes());
   const int64_t B = x.size(0), N = x.size(1), H = x.size(2), Dh = x.size(3), axes = (int64_t)sections.size();
   REQUIRE(Dh % 2 == 0 && Dh >= 2 && Dh <= 1024 && H >= 1 && H <= 1024 && B <= 65535 && N <= ROWS_MAX, op,
-          "head_dim must be even and at most 1024, heads 1 .. 1024, batch at most 65535");
+          "head_dim must be even and at most 1024, heads 1 .. 1024, batch at most 65535, tokens at most 2^30");
   int64_t pairs = 0;
   bool good = axes >= 1 && axes <= 4;
   for (const int64_t s : sections) good = good && s >= 0 && s <= Dh, pairs += good ? s : 0;
@@ -332,8 +332,8 @@ int linear_check(const char* op, const Tensor& x, const Tensor& weight, const Op
   REQUIRE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(1) % multiple == 0 && weight.numel() > 0, op, "weight ",
           weight.sizes(), " does not match input ", x.sizes(), " (K must be a multiple of ", multiple, ")");
   const int64_t K = weight.size(1), N = weight.size(0);
-  REQUIRE(K * (int64_t)weight.element_size() <= (1 << 23) && N <= ROWS_MAX && x.numel() / K <= ROWS_MAX, op,
-          "K is at most 2^23 bytes, N and the rows of x at most 2^31 - 1");
+  REQUIRE(K * (int64_t)weight.element_size() <= (1 << 23) && N <= (1 << 22) && x.numel() / K <= ROWS_MAX, op,
+          "K is at most 2^23 bytes, N at most 2^22, the rows of x at most 2^30");
   const int code = activation(op, act);
   REQUIRE(!bias || (bias->dim() == 1 && bias->size(0) == N), op, "bias ", bias->sizes(), ", expected [", N, "]");
   REQUIRE(!residual || residual->sizes() == at::IntArrayRef(with_last(x, N)), op, "residual ", residual->sizes(), ", expected ", with_last(x, N),
@@ -587,6 +587,8 @@ Tensor rotary_forward_autograd(const Tensor& x, const Tensor& positions, const T
 struct LinearAct : torch::autograd::Function<LinearAct> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                                std::string act) {
+    // (the K axis of dW = dz^T x)
+    REQUIRE(!weight.requires_grad() || x.numel() / weight.size(1) <= (1 << 22), "linear_act", "more than 2^22 rows of x with a gradient of weight");
     at::AutoDispatchBelowAutograd below;
     const bool keep = act != "none" && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
     auto [y, pre] = linear_forward_op().call(x, weight, bias, residual, act, keep);
