@@ -5,65 +5,16 @@
 
 using namespace mvit_linear;
 
-namespace {
-
-template <int MODE, class E, int BM, int BN, int WM, int WN, int BKB, int NST>
-int launch_tile(const Args& a, hipStream_t s) {
-  using T = Tile<MODE, BM, BN, WM, WN, BKB, NST>;
-  const long long nt = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  if (nt > 0x7fffffff) return MVIT_EINVAL;
-  static mvit_per_device_size raised;
-  const auto fn = linear_tile<MODE, E, BM, BN, WM, WN, BKB, NST>;
-  if (const int rc = mvit_ensure_dynamic_lds((const void*)fn, T::LDS, raised)) return rc;
-  const long long slots = (long long)mvit_num_cus() * T::BLOCKS_PER_CU;
-  hipLaunchKernelGGL(fn, dim3((unsigned)(nt < slots ? nt : slots)), dim3(T::NT), T::LDS, s, a);
-  return MVIT_LAUNCH_CHECK();
-}
-
-template <bool OP8, class E, int MT>
-int launch_rows(const Args& a, hipStream_t s) {
-  hipLaunchKernelGGL((linear_rows<OP8, E, MT>), dim3((a.N + 15) / 16), dim3(512), 0, s, a);
-  return MVIT_LAUNCH_CHECK();
-}
-
-// Rows or tiles, and which: by what a round of blocks costs.  A round is every CU's share at once (one 256 x 256 tile, two of the others);
-// measured at K = 1536, bf16, it takes 40 us with tiles of 256 x 256, 27 of 128 x 128 (20 with one a CU) and 12 of 64 x 64, and the
-// ratios hold for e4m3 and other K within some per cent.  Large tiles read less of x and W; small ones leave less of the chip idle in the
-// last round: [5264, 1536] x [4608, 1536]: 75 / 79 / 130 us, [5264, 4096] x [1536, 4096]: 80 / 62 / 104, [1301, 1536] x [4608, 1536]:
-// 36 / 26 / 35, [329, 1536] x [4608, 1536]: 34 / 20 / 13.
-template <int MODE, class E>
-int by_size(const Args& a, hipStream_t s) {
-  using Any = End<E::out32, A_ANY, E::vec>;   // (the row kernels' epilogue is not unrolled)
-  const long long cus = mvit_num_cus();
-  // few rows: [1, 1536] x [1536, 1536] bf16 5.8 us against 9.0 with tiles, [17, ..] 6.7 / 9.1, [32, 4096] x [1536, 4096] 14 / 18; from 33
-  // rows on (9.0 / 9.2) and, from 17 on, with more than one block a CU (N > 4096) the tiles are as fast or faster
-  if (a.M <= 16) return launch_rows<MODE != H16, Any, 1>(a, s);
-  if (a.M <= 32 && a.N <= 16 * cus) return launch_rows<MODE != H16, Any, 2>(a, s);
-  auto rounds = [&](long long edge, long long at_once) {
-    const long long t = ((a.M + edge - 1) / edge) * ((a.N + edge - 1) / edge);
-    return (t + at_once - 1) / at_once;
-  };
-  const long long c256 = 40 * rounds(256, cus), c128 = rounds(128, cus) == 1 ? 20 : 27 * rounds(128, 2 * cus), c64 = 12 * rounds(64, 2 * cus);
-  if (c256 < c128 && c256 < c64) return launch_tile<MODE, E, 256, 256, 2, 4, 128, 2>(a, s);
-  if (c128 < c64) return launch_tile<MODE, E, 128, 128, 2, 2, 128, 2>(a, s);
-  return launch_tile<MODE, E, 64, 64, 2, 2, 128, 4>(a, s);
-}
-
+namespace mvit_linear {
 template <int MODE, bool OUT32>
-int dispatch(Args& a, bool vec, hipStream_t s) {
-  if (!vec) return by_size<MODE, End<OUT32, A_ANY, false>>(a, s);
-  switch (a.act) {
-    case MVIT_ACT_NONE:
-    case MVIT_ACT_RELU:
-      return by_size<MODE, End<OUT32, A_CLIP, true>>(a, s);
-    case MVIT_ACT_GELU:
-      return by_size<MODE, End<OUT32, A_ERF, true>>(a, s);
-    case MVIT_ACT_SILU:
-      return by_size<MODE, End<OUT32, A_SILU, true>>(a, s);
-    default:
-      return by_size<MODE, End<OUT32, A_TANH, true>>(a, s);
-  }
-}
+int dispatch(const Args& a, bool vec, hipStream_t s);   // linear_launch.hpp
+extern template int dispatch<H16, false>(const Args&, bool, hipStream_t);
+extern template int dispatch<H16, true>(const Args&, bool, hipStream_t);
+extern template int dispatch<F8, false>(const Args&, bool, hipStream_t);
+extern template int dispatch<F8X, true>(const Args&, bool, hipStream_t);
+}  // namespace mvit_linear
+
+namespace {
 
 constexpr int MAX_M = 1 << 30, MAX_N = 1 << 24;   // tile numbers and grids stay in 31 bits
 
@@ -131,7 +82,10 @@ __device__ __forceinline__ float slope(float z, int act) {
     const float z2 = z * z, p = sigmoid2(z * __builtin_fmaf(z2, TANH_B, TANH_A));
     return p + z * p * (1.f - p) * __builtin_fmaf(z2, 3.f * TANH_B / LOG2E, TANH_A / LOG2E);
   }
-  if constexpr (SL == S_ERF) return normal_cdf(z) + z * 0.39894228040f * __builtin_amdgcn_exp2f(-0.72134752044f * z * z);
+  if constexpr (SL == S_ERF) {   // z Phi(z): Phi + z phi
+    const float e = gauss(z);
+    return normal_cdf(z, e) + z * e * 0.39894228040f;
+  }
   return act == MVIT_ACT_NONE        ? 1.f
          : act == MVIT_ACT_RELU      ? slope<S_CLIP>(z, act)
          : act == MVIT_ACT_SILU      ? slope<S_SILU>(z, act)
@@ -231,10 +185,10 @@ __global__ __launch_bounds__(256) void act_bwd_elements(const SlopeArgs p) {
   if (p.part && c < p.N) p.part[(size_t)blockIdx.y * p.N + c] = sum;
 }
 
-// rows of a run: blocks enough for eight a CU, no more than 128 runs to add up
+// rows of a run: blocks enough for sixteen a CU, no more than 128 runs to add up
 int run_rows(int M, int N) {
   const int tiles = (M + 63) / 64, cols = (N + 63) / 64;
-  int runs = (mvit_num_cus() * 8 + cols - 1) / cols;
+  int runs = (mvit_num_cus() * 16 + cols - 1) / cols;
   runs = runs > 128 ? 128 : runs;
   runs = runs > tiles ? tiles : runs;
   return (tiles + runs - 1) / runs * 64;

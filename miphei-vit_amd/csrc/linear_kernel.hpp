@@ -56,13 +56,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const char* p) {
 // ---------------------------------------------------------------- epilogue arithmetic
 // erf by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7, below f32 rounding of 1 + erf): one exp, one reciprocal and seven
 // multiply-adds where the library's erff takes about forty instructions -- at 64 lanes a cycle and CU that is what the epilogue costs.
-__device__ __forceinline__ float half_erfc(float a) {   // erfc(a / sqrt 2) / 2 for a >= 0
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.23164188684f * a);   // p / sqrt 2, p = 0.3275911
-  const float e = __builtin_amdgcn_exp2f(-0.72134752044f * a * a);   // exp(-a^2 / 2)
-  return 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-}
-__device__ __forceinline__ float normal_cdf(float z) {
-  const float q = half_erfc(fabsf(z));
+__device__ __forceinline__ float gauss(float z) { return __builtin_amdgcn_exp2f(-0.72134752044f * z * z); }   // exp(-z^2 / 2)
+__device__ __forceinline__ float normal_cdf(float z, float e) {   // e = gauss(z)
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.23164188684f, fabsf(z), 1.f));   // p / sqrt 2, p = 0.3275911
+  // erfc(|z| / sqrt 2) / 2: half of 7.1.26's coefficients
+  const float q = e * t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
   return z >= 0.f ? 1.f - q : q;
 }
 constexpr float LOG2E = 1.44269504089f;
@@ -77,7 +75,7 @@ __device__ __forceinline__ float activated(const Args& p, float z) {
   if constexpr (ACT == A_CLIP) return __builtin_elementwise_maximum(z, p.act_lo);
   if constexpr (ACT == A_SILU) return z * sigmoid2(LOG2E * z);
   if constexpr (ACT == A_TANH) return z * sigmoid2(z * __builtin_fmaf(z * z, TANH_B, TANH_A));
-  if constexpr (ACT == A_ERF) return z * normal_cdf(z);
+  if constexpr (ACT == A_ERF) return z * normal_cdf(z, gauss(z));
   return p.act == MVIT_ACT_GELU        ? activated<A_ERF>(p, z)
          : p.act == MVIT_ACT_SILU      ? activated<A_SILU>(p, z)
          : p.act == MVIT_ACT_GELU_TANH ? activated<A_TANH>(p, z)
@@ -178,9 +176,9 @@ __device__ __forceinline__ void widen(const i32x4& v, bf16x8 (&out)[2]) {
 }
 
 // ---------------------------------------------------------------- tiles
-// WM x WN waves form BM x BN of y at a time.  K goes by in tiles of BKB bytes a row; NST of them live in LDS, filled by DMA
-// (buffer_load ... lds, 16 bytes a lane).  LDS rows are BKB bytes; the 16-byte piece c of row r lies at place
-// c ^ (r / (256 / BKB) mod pieces), which puts the 16 rows that a fragment read touches on all 64 banks once.
+// WM x WN waves form BM x BN of y at a time.  K goes by in tiles of 128 bytes a row (BKB); NST of them live in LDS, filled by DMA
+// (buffer_load ... lds, 16 bytes a lane).  The 16-byte piece c of LDS row r lies at place c ^ x_place(r) (w_place(r) for W), which
+// puts the 16 rows that a fragment read touches on all 64 banks once.
 //  * The fragments of the next sub-step (64 bytes of K) are read into registers behind the current one's matrix instructions; the
 //    hand-over of a K tile (this wave's reads are back, its DMA of the next tile has landed, barrier) stands in front of the last
 //    sub-step, and the refill of the tile just read is issued behind it.
@@ -190,7 +188,9 @@ __device__ __forceinline__ void widen(const i32x4& v, bf16x8 (&out)[2]) {
 //    a fragment is free, and is chosen so that a lane's groups make up whole pieces of 16 bytes and the lanes of a row 64 bytes in a
 //    line: y leaves from the registers.  (Through panels in LDS, whole lines a store, the epilogue took 6 to 8 us of a 256 x 256 tile:
 //    a chain of LDS writes, reads and waits with two waves a SIMD to hide it.)
-template <int MODE, int BM, int BN, int WM, int WN, int BKB, int NST>
+constexpr int BKB = 128;
+
+template <int MODE, int BM, int BN, int WM, int WN, int NST>
 struct Tile {
   static constexpr int NW = WM * WN, NT = NW * 64;
   static constexpr int WTM = BM / WM, WTN = BN / WN;
@@ -200,18 +200,17 @@ struct Tile {
   static constexpr int ROWS_PER_DMA = 1024 / BKB;       // rows of one wave's DMA instruction
   static constexpr int A_DMA = BM / ROWS_PER_DMA / NW, B_DMA = BN / ROWS_PER_DMA / NW, LPT = A_DMA + B_DMA;
   static constexpr int STAGE = (BM + BN) * BKB;
-  static constexpr int NSUB = BKB / 64;                 // sub-steps of a K tile: 64 bytes each
   static constexpr int TABLE = MODE == F8 ? 2 * WTN : 0;   // floats of a wave's table of column constants
   static constexpr size_t LDS = (size_t)NST * STAGE + (size_t)NW * TABLE * 4;
   static constexpr int BLOCKS_PER_CU = 160 * 1024 / LDS < 512 / NT ? 160 * 1024 / LDS : 512 / NT;   // two waves a SIMD
-  static_assert(A_DMA >= 1 && B_DMA >= 1 && TM >= 1 && TN >= 1, "tile too small");
-  static_assert((BKB == 64 || BKB == 128) && NW * ROWS_PER_DMA % 32 == 0, "LDS places repeat every 32 rows");
+  static_assert(A_DMA >= 1 && B_DMA >= 1 && TM >= 1 && TN >= 1 && WTN <= 64, "sizes of a wave");
+  static_assert(NW * ROWS_PER_DMA % 32 == 0, "LDS places repeat every 32 rows");
   static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
 
-template <int MODE, class E, int BM, int BN, int WM, int WN, int BKB, int NST>
+template <int MODE, class E, int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
-  using T = Tile<MODE, BM, BN, WM, WN, BKB, NST>;
+  using T = Tile<MODE, BM, BN, WM, WN, NST>;
   constexpr bool OP8 = MODE != H16, WIDE = MODE == F8;   // WIDE: 32 x 32 instructions
   using frag = std::conditional_t<WIDE, i32x8, i32x4>;
   using acc_t = std::conditional_t<WIDE, f32x16, f32x4>;
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, nt = tm * tn;
-  const int nk = (p.kb + 127) / 128;            // turns of the main loop: 128 bytes of K each
+  const int nk = (p.kb + BKB - 1) / BKB;
 
   // tile number -> place: blocks go to the eight XCDs in turn, so the numbers of one XCD are put on one contiguous run of tiles, and runs
   // go down 8 rows of tiles before the next column: the blocks that share an L2 share rows of x and of W
@@ -235,8 +234,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   // the place of piece c of LDS row r is c ^ x_place(r), c ^ w_place(r): 16 lanes read 16 rows, for x 16 in a line, for W (H16 with 16-bit
   // y) those of bit 2 alike among 32
   constexpr bool PAIRED = MODE == H16 && !E::out32;
-  auto x_place = [](int r) __attribute__((always_inline)) { return BKB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; };
-  auto w_place = [](int r) __attribute__((always_inline)) { return BKB == 128 ? (PAIRED ? ((r >> 1) & 1) | ((r >> 2) & 6) : (r >> 1) & 7) : PAIRED ? (r >> 3) & 3 : (r >> 2) & 3; };
+  auto x_place = [](int r) __attribute__((always_inline)) { return (r >> 1) & 7; };
+  auto w_place = [](int r) __attribute__((always_inline)) { return PAIRED ? ((r >> 1) & 1) | ((r >> 2) & 6) : (r >> 1) & 7; };
 
   // ---- the DMA side: output tile `dv`, K tile `dk` of it come next
   const int dr = lane / T::PIECES;   // this lane's part of a wave's DMA instruction: one 16-byte piece of row `dr`
@@ -270,7 +269,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)to, 16, o, k, 0, 0);
   };
   auto advance = [&]() __attribute__((always_inline)) {
-    if (++dk == nk * (128 / BKB)) {
+    if (++dk == nk) {
       dk = 0;
       dv += gridDim.x;
       aim(0);
@@ -373,32 +372,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
       for (int j = 0; j < T::TN; ++j)
 #pragma unroll
         for (int r = 0; r < AR; ++r) acc[i][j][r] = 0.f;
-    auto wait_next = [&]() __attribute__((always_inline)) {   // this wave's reads are back, its DMA of the next K tile has landed
+    for (int t = 0; t < nk; ++t) {
+      const int next = stage + 1 == NST ? 0 : stage + 1;
+      sub_step(0, stage, 1, -1, std::false_type{});
       if (landed > 0)
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       else
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * T::LPT) : "memory");
       --landed;
       barrier();
-    };
-    for (int t = 0; t < nk; ++t) {
-      const int next = stage + 1 == NST ? 0 : stage + 1;
-      if constexpr (T::NSUB == 2) {
-        sub_step(0, stage, 1, -1, std::false_type{});
-        wait_next();
-        sub_step(1, next, 0, stage, std::true_type{});
-        advance();
-        stage = next;
-      } else {   // two K tiles a turn
-        const int after = next + 1 == NST ? 0 : next + 1;
-        wait_next();
-        sub_step(0, next, 0, stage, std::true_type{});
-        advance();
-        wait_next();
-        sub_step(1, after, 0, next, std::true_type{});
-        advance();
-        stage = after;
-      }
+      sub_step(1, next, 0, stage, std::true_type{});
+      advance();
+      stage = next;
     }
     // ---- epilogue, from the registers.  The DMA of the next tile's first K tiles is waited for in front of its stores: loads, DMA and
     // stores share one counter, and behind the stores it could not be told any more.

@@ -316,9 +316,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 template <int TPR, int NV, int VEC, int XT, int RT, int YT, bool NORM>
 int launch_fwd(const RowArgs& a, hipStream_t s) {
   const int rpb = 256 / TPR;
-  // rounds of the grid stride: [20816, 1536] bf16 to 8 bits 40 us with 8 blocks a CU, 37 with 16, 39 with as many as rows; wider rows hold
-  // more registers and loads a thread
-  const long long need = ((long long)a.M + rpb - 1) / rpb, most = (long long)mvit_num_cus() * (a.D <= 2048 ? 16 : 8);
+  // rounds of the grid stride: [20816, 1536] bf16 to 8 bits 40 us with 8 blocks a CU, 37 with 16, 39 with as many as there are rows for
+  const long long need = ((long long)a.M + rpb - 1) / rpb, most = (long long)mvit_num_cus() * 16;
   hipLaunchKernelGGL((rms_fwd<TPR, NV, VEC, XT, RT, YT, NORM>), dim3((unsigned)(need < most ? need : most)), dim3(256), 0, s, a);
   return MVIT_LAUNCH_CHECK();
 }

@@ -572,7 +572,9 @@ def act_oracle(z, act):
 LINEAR = [(1, 8, 1), (1, 1536, 1536), (5, 64, 33), (16, 136, 24), (17, 4096, 130), (32, 200, 72), (33, 96, 288), (64, 64, 64), (65, 72, 129),
           (329, 1536, 200), (1301, 96, 515), (2100, 264, 2056), (3000, 1544, 1100), (4111, 128, 1031),
           # the largest tiles: one a block, ragged and not, several a block (with a K of one and of an odd number of K tiles)
-          (5003, 72, 2397), (5000, 512, 2400), (8200, 328, 2600), (12000, 8, 2600)]
+          (5003, 72, 2397), (5000, 512, 2400), (8200, 328, 2600), (12000, 8, 2600),
+          # each of the tiles: 64 x 64, 128 x 128, 128 x 256, 192 x 256, 256 x 256, the last two several a block
+          (329, 264, 1000), (700, 136, 4096), (1301, 200, 4608), (5264, 136, 4096), (5260, 72, 4093), (5264, 88, 8192), (5300, 40, 8181)]
 
 
 def linear_case(g, M, K, N, dtype, res, bias_f32):
