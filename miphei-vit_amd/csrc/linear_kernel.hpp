@@ -346,7 +346,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
         }
     }
   };
-  auto barrier = [&]() __attribute__((always_inline)) {
+  auto barrier = [&]() __attribute__((always_inline)) {   // this wave's LDS reads are back: behind it others' DMA may overwrite what they read
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -375,10 +376,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
     for (int t = 0; t < nk; ++t) {
       const int next = stage + 1 == NST ? 0 : stage + 1;
       sub_step(0, stage, 1, -1, std::false_type{});
-      if (landed > 0)
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * T::LPT) : "memory");
+      if (landed <= 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * T::LPT) : "memory");
       --landed;
       barrier();
       sub_step(1, next, 0, stage, std::true_type{});
