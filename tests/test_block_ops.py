@@ -890,3 +890,49 @@ def test_inside_another_operand_mode():
                 got = (ops.linear_act(x, w), ops.rms_norm(x, torch.ones(64, device="cuda")), *ops.quantize_fp8(x))
                 assert _lib.operand_mode() == mode
             assert all(torch.equal(a.float(), b.float()) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_gradient_of_a_gradient_is_refused():
+    ops, g = T(), gen(41)
+    x, w = randn(g, 4, 64).requires_grad_(), randn(g, 64).requires_grad_()
+    (dx,) = torch.autograd.grad(ops.rms_norm(x, w).sum(), x, create_graph=False)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(ops.rms_norm(x, w).square().sum(), x, create_graph=True)
+    a, b = randn(g, 4, 64, dtype=torch.float16).requires_grad_(), randn(g, 32, 64, dtype=torch.float16).requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(ops.linear_act(a, b).square().sum(), a, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_traced_by_the_compiler_front_end():
+    """one graph without breaks through the shape implementations, with the eager results"""
+    ops, g = T(), gen(42)
+    x, r, w = randn(g, 6, 64, dtype=torch.bfloat16), randn(g, 6, 64), randn(g, 64)
+    wt, b = randn(g, 96, 64, dtype=torch.bfloat16), randn(g, 96, dtype=torch.bfloat16)
+    pos, freq = torch.arange(6, device="cuda", dtype=torch.int32)[:, None], ops.rotary_frequencies([16], device="cuda")
+
+    def f(x, r, w, wt, b):
+        y, h = ops.add_rms_norm(x, r, w)
+        z = ops.linear_act(y, wt, b, None, "silu").view(1, 6, 3, 32)
+        return ops.rotary(z, pos, freq, [16], 2), h, *ops.quantize_fp8(y.detach())
+    want = f(x, r, w, wt, b)
+    got = torch.compile(f, backend="aot_eager", fullgraph=True)(x, r, w, wt, b)
+    assert all(torch.equal(u.float(), v.float()) for u, v in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_saved_tensors_changed_in_place_are_noticed():
+    ops, g = T(), gen(43)
+    x, r, w = randn(g, 4, 64).requires_grad_(), randn(g, 4, 64), randn(g, 64).requires_grad_()
+    y, h = ops.add_rms_norm(x, r, w)
+    h.detach().add_(1)                                      # (the stream that the backward pass reads)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    q = randn(g, 1, 3, 2, 8, dtype=torch.float16)
+    p = (q.clone().requires_grad_() * 1)
+    z = p * p
+    with torch.no_grad():
+        ops.rotary_(p, torch.zeros(3, 1, device="cuda", dtype=torch.int32), torch.ones(4, device="cuda"), [4])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
