@@ -11,6 +11,9 @@ foundation_models.py:53-57``), ``WeightedMSELoss`` (``/root/reference/src/loss.p
                                                                                    -> mvit_attention_fwd / _bwd
     torch.ops.mvit.weighted_mse(pred, target, w, lam)  WeightedMSELoss.forward     -> mvit_wmse_fwd_bwd
 
+The further operators of a transformer block (RMS norm of a residual stream, rotary positions, linear with activation and residual, 8-bit
+forms) are defined in ``block_ops`` and re-exported here.
+
 Arithmetic is the reference's bf16-mixed mode: bf16 operands, f32 accumulation, f32 LayerNorm statistics.  Every op has a fake
 (meta) implementation, so FakeTensor tracing / torch.compile shape propagation work, and an autograd formula built on the
 backward kernels.  CUDA (ROCm) tensors only: there is no CPU implementation -- a CPU call raises from the dispatcher.
