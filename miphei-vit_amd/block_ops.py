@@ -7,6 +7,9 @@ functions below are their entry points, re-exported by ``torch_ops``.  CUDA (ROC
 the tensors are (fp16 runs in libmiphei_hip_f16.so), never a mixture; the work goes to the tensors' device, on its current stream.  Wrong
 arguments raise ValueError.
 
+All of them can be captured into a graph, forward and backward; as with any backward pass, let no eager graph over the same leaves live
+while one is captured (delete its outputs first): its accumulation nodes belong to the eager stream.
+
 Checks, allocations, autograd formulas and the calls of the C-ABI are in csrc/torch_ops.cpp (libmiphei_torch.so), not in Python: a call on
 one token costs its host time.
 """
@@ -114,8 +117,8 @@ def rotary(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequence[in
 def rotary_(x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequence[int], rotate_heads: Optional[int] = None, num_prefix: int = 0,
             interleaved: bool = False) -> Tensor:
     """``rotary`` in place, for serving (no gradient): what passes through is neither read nor written."""
-    return _ROTARY_(x, positions, inv_freq, sections, x.shape[2] if rotate_heads is None and x.dim() == 4 else rotate_heads or 0, num_prefix,
-                    interleaved)
+    _ROTARY_(x, positions, inv_freq, sections, x.shape[2] if rotate_heads is None and x.dim() == 4 else rotate_heads or 0, num_prefix, interleaved)
+    return x
 
 
 def rotary_frequencies(sections: Sequence[int], base: float = 10000.0, shared: bool = False, device=None) -> Tensor:

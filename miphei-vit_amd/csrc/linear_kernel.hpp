@@ -44,13 +44,13 @@ struct End {
   static constexpr int act = ACT;
 };
 
-constexpr unsigned OOB = 0x80000000u;   // beyond every descriptor's range: the load returns zeros
+constexpr unsigned OOB = 0x80000000u;   // a descriptor's size, and so beyond its range: the load returns zeros
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const char* p) {
   // uniform by construction; readfirstlane lets the compiler see it and keep the descriptor in scalar registers
   const unsigned long long v = (unsigned long long)p;
   const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
-  return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), 0, 0x7fffffff, 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), 0, (int)OOB, 0x00020000);
 }
 
 // ---------------------------------------------------------------- epilogue arithmetic

@@ -327,7 +327,7 @@ int fwd_layout(const RowArgs& a, bool vec, hipStream_t s) {
   const int D = a.D;
   if (vec) {
     // a wave a row, or 256 threads (f32 stream to 8 bits, us): rows of 512: 1024 of them 3.1 / 3.8, 8192 9.1 / 12.1; of 1024: 256 3.4 / 3.2,
-    // 1024 4.1 / 4.3, 8192 15.7 / 16.5; of 1536: 256 4.1 / 3.4, 2048 7.6 / 6.9, 3072 9.7 / 10.6, 4096 12.0 / 13.2; of 4096: 64 6.9 / 3.7,
+    // 1024 4.1 / 4.3, 8192 15.7 / 16.5; of 1536: 256 4.1 / 3.4, 2048 7.6 / 6.9, 4096 12.0 / 13.2; of 4096: 64 6.9 / 3.7,
     // 8192 83 / 75
     if (D <= 512) return launch_fwd<64, 1, 8, XT, RT, YT, NORM>(a, s);
     if (D <= 2048 && a.M >= (D <= 1024 ? 4 : 12) * mvit_num_cus()) {

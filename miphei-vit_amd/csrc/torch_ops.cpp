@@ -15,9 +15,12 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <optional>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "../../include/miphei_hip.h"
 
@@ -112,19 +115,26 @@ void* stream(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().
 Tensor scratch(const Tensor& x, int64_t bytes) { return at::empty({bytes}, x.options().dtype(at::kByte)); }
 Tensor none(const Tensor& x, ScalarType t) { return at::empty({0}, x.options().dtype(t)); }
 
-std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
-  auto s = x.sizes().vec();
+// Checks and output shapes take sizes as SymInt (plain integers but while a graph is traced with sizes that vary): a model compiled once runs
+// at other batch sizes
+using Sizes = std::vector<c10::SymInt>;
+Sizes with_last(const Tensor& x, const c10::SymInt& n) {
+  Sizes s = x.sym_sizes().vec();
   s.back() = n;
   return s;
 }
+Tensor empty(c10::SymIntArrayRef sizes, const Tensor& like, ScalarType t) { return at::empty_symint(sizes, like.options().dtype(t)); }
 
 // ================================================================ RMS norm
+void rows_check(const char* op, const Tensor& x) {
+  REQUIRE(x.dim() >= 1 && x.sym_size(-1) >= 1 && x.sym_size(-1) <= 16384, op, "the last dimension must be 1 .. 16384");
+  REQUIRE(x.sym_numel() <= x.sym_size(-1) * ROWS_MAX, op, "more than 2^30 rows");
+}
 HalfType norm_check(const char* op, const Tensor& x, const OptTensor& residual, const Tensor& weight, std::optional<ScalarType> out) {
-  REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, op, "the last dimension must be 1 .. 16384");
-  const int64_t d = x.size(-1);
-  REQUIRE(x.numel() / d <= ROWS_MAX, op, "more than 2^30 rows");
-  REQUIRE(weight.dim() == 1 && weight.size(0) == d, op, "weight ", weight.sizes(), " does not match input ", x.sizes());
-  REQUIRE(!residual || residual->sizes() == x.sizes(), op, "residual ", residual->sizes(), " and input ", x.sizes(), " differ (it is not broadcast)");
+  rows_check(op, x);
+  REQUIRE(weight.dim() == 1 && weight.sym_size(0) == x.sym_size(-1), op, "weight ", weight.sym_sizes(), " does not match input ", x.sym_sizes());
+  REQUIRE(!residual || residual->sym_sizes() == x.sym_sizes(), op, "residual ", residual->sym_sizes(), " and input ", x.sym_sizes(),
+          " differ (it is not broadcast)");
   same_place(op, x, residual);
   same_place(op, x, weight);
   HalfType h{op};
@@ -140,8 +150,8 @@ struct NormOut {
   Tensor y, h, row;   // row: one f32 a row (rstd, scale)
 };
 NormOut norm_out(const Tensor& x, const OptTensor& residual, ScalarType y) {
-  return {at::empty(x.sizes(), x.options().dtype(y)), residual ? at::empty(x.sizes(), x.options().dtype(residual->scalar_type())) : none(x, x.scalar_type()),
-          at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat))};
+  return {empty(x.sym_sizes(), x, y), residual ? empty(x.sym_sizes(), x, residual->scalar_type()) : none(x, x.scalar_type()),
+          empty(x.sym_sizes().slice(0, x.dim() - 1), x, at::kFloat)};
 }
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps,
@@ -171,11 +181,16 @@ struct NormBwd {
 };
 NormBwd norm_bwd_out(const Tensor& h, const Tensor& weight, ScalarType x_dtype, bool need_x, bool need_residual, bool need_weight) {
   const bool one = x_dtype == h.scalar_type(), x = need_x || (one && need_residual), res = need_residual && !one;
-  return {x ? at::empty(h.sizes(), h.options().dtype(x_dtype)) : none(h, x_dtype), res ? at::empty(h.sizes(), h.options()) : none(h, h.scalar_type()),
+  return {x ? empty(h.sym_sizes(), h, x_dtype) : none(h, x_dtype), res ? empty(h.sym_sizes(), h, h.scalar_type()) : none(h, h.scalar_type()),
           need_weight ? at::empty_like(weight, at::MemoryFormat::Contiguous) : none(weight, weight.scalar_type()), x, res};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_norm_backward(const Tensor& dy, const OptTensor& dh, const Tensor& h, const Tensor& weight, const Tensor& rstd,
                                                      ScalarType x_dtype, bool need_x, bool need_residual, bool need_weight) {
+  REQUIRE(h.dim() >= 1 && h.size(-1) >= 1 && dy.sizes() == h.sizes() && (!dh || dh->sizes() == h.sizes()) && weight.numel() == h.size(-1) &&
+              rstd.numel() == h.numel() / h.size(-1),
+          "rms_norm_backward", "sizes ", dy.sizes(), ", ", h.sizes(), ", ", weight.sizes(), ", ", rstd.sizes());
+  for (const Tensor* t : {&dy, &weight, &rstd}) same_place("rms_norm_backward", h, *t);
+  same_place("rms_norm_backward", h, dh);
   c10::DeviceGuard guard(h.device());
   NormBwd o = norm_bwd_out(h, weight, x_dtype, need_x, need_residual, need_weight);
   const int64_t d = h.size(-1), m = h.numel() / d;
@@ -219,8 +234,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8_meta(const Tensor& x, const OptT
 }
 
 HalfType quantize_check(const Tensor& x) {
-  REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "quantize_fp8", "the last dimension must be 1 .. 16384");
-  REQUIRE(x.numel() / x.size(-1) <= ROWS_MAX, "quantize_fp8", "more than 2^30 rows");
+  rows_check("quantize_fp8", x);
   HalfType h{"quantize_fp8"};
   h.add(x);
   return h;
@@ -245,28 +259,50 @@ std::tuple<Tensor, Tensor> quantize_fp8_meta(const Tensor& x) {
 // ================================================================ rotary positions
 HalfType rotary_check(const char* op, const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
                       int64_t num_prefix) {
-  REQUIRE(x.dim() == 4, op, "x must be [B, N, heads, head_dim], got ", x.sizes());
-  const int64_t B = x.size(0), N = x.size(1), H = x.size(2), Dh = x.size(3), axes = (int64_t)sections.size();
+  REQUIRE(x.dim() == 4, op, "x must be [B, N, heads, head_dim], got ", x.sym_sizes());
+  const c10::SymInt B = x.sym_size(0), N = x.sym_size(1), H = x.sym_size(2), Dh = x.sym_size(3);
+  const int64_t axes = (int64_t)sections.size();
   REQUIRE(Dh % 2 == 0 && Dh >= 2 && Dh <= 1024 && H >= 1 && H <= 1024 && B <= 65535 && N <= ROWS_MAX, op,
           "head_dim must be even and at most 1024, heads 1 .. 1024, batch at most 65535, tokens at most 2^30");
   int64_t pairs = 0;
   bool good = axes >= 1 && axes <= 4;
-  for (const int64_t s : sections) good = good && s >= 0 && s <= Dh, pairs += good ? s : 0;
-  REQUIRE(good && pairs >= 1 && pairs <= Dh / 2, op, "sections ", sections, ": 1 to 4 axes, together 1 .. head_dim / 2 pairs");
-  REQUIRE(rotate_heads >= 0 && rotate_heads <= H && num_prefix >= 0 && num_prefix <= N, op, "rotate_heads ", rotate_heads, " of ", H, ", num_prefix ",
+  for (const int64_t s : sections) good = good && s >= 0 && Dh >= s, pairs += good ? s : 0;
+  REQUIRE(good && pairs >= 1 && Dh >= 2 * pairs, op, "sections ", sections, ": 1 to 4 axes, together 1 .. head_dim / 2 pairs");
+  REQUIRE(rotate_heads >= 0 && H >= rotate_heads && num_prefix >= 0 && N >= num_prefix, op, "rotate_heads ", rotate_heads, " of ", H, ", num_prefix ",
           num_prefix, " of ", N);
-  const int64_t want[3] = {B, N - num_prefix, axes};
-  REQUIRE(positions.sizes() == at::IntArrayRef(want + 1, 2) || positions.sizes() == at::IntArrayRef(want, 3), op, "positions must be ",
-          at::IntArrayRef(want + 1, 2), " or ", at::IntArrayRef(want, 3), ", got ", positions.sizes());
+  const int pd = (int)positions.dim();
+  REQUIRE((pd == 2 || pd == 3) && positions.sym_size(-1) == axes && positions.sym_size(-2) == N - num_prefix && (pd == 2 || positions.sym_size(0) == B), op,
+          "positions must be [N - num_prefix, axes] or [B, N - num_prefix, axes] of ", x.sym_sizes(), " with ", num_prefix, " and ", axes, ", got ",
+          positions.sym_sizes());
   const ScalarType pt = positions.scalar_type(), ft = inv_freq.scalar_type();
   REQUIRE(pt == at::kInt || pt == at::kLong || pt == at::kFloat, op, "positions are int32, int64 or float32, got ", pt);
-  REQUIRE(inv_freq.dim() == 1 && inv_freq.size(0) == pairs && (ft == at::kFloat || ft == at::kDouble), op, "inv_freq must be float32 or float64 [", pairs,
-          "], got ", ft, " ", inv_freq.sizes());
+  REQUIRE(inv_freq.dim() == 1 && inv_freq.sym_size(0) == pairs && (ft == at::kFloat || ft == at::kDouble), op, "inv_freq must be float32 or float64 [", pairs,
+          "], got ", ft, " ", inv_freq.sym_sizes());
   same_place(op, x, positions);
   same_place(op, x, inv_freq);
   HalfType h{op};
   h.add(x);
   return h;
+}
+
+// y of rotary: x's own layout where that is a layout with dense heads (the order of overlapping windows is not), else contiguous
+Tensor rotary_out(const Tensor& x) {
+  Tensor y = at::empty_like(x);
+  return y.sym_stride(3) == 1 ? y : empty(x.sym_sizes(), x, x.scalar_type());
+}
+// no two elements share an address: every stride reaches beyond all that the smaller ones span
+bool apart(const Tensor& x) {
+  if (x.unsafeGetTensorImpl()->has_symbolic_sizes_strides()) return true;   // (told when it runs)
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t i = 0; i < x.dim(); ++i)
+    if (x.size(i) > 1) dims.emplace_back(x.stride(i), x.size(i));
+  std::sort(dims.begin(), dims.end());
+  int64_t span = 0;
+  for (const auto& [stride, size] : dims) {
+    if (stride <= span) return false;
+    span += stride * (size - 1);
+  }
+  return true;
 }
 
 void rotary_into(const HalfType& half, const Tensor& x, const Tensor& y, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections,
@@ -291,31 +327,31 @@ Tensor rotary_forward(const Tensor& x0, const Tensor& positions, const Tensor& i
   const HalfType h = rotary_check("rotary", x0, positions, inv_freq, sections, rotate_heads, num_prefix);
   c10::DeviceGuard guard(x0.device());
   const Tensor x = x0.stride(3) == 1 ? x0 : x0.contiguous();
-  Tensor y = at::empty_like(x);
+  Tensor y = rotary_out(x);
   rotary_into(h, x, y, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
   return y;
 }
 Tensor rotary_forward_meta(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
                            int64_t num_prefix, bool, bool) {
   rotary_check("rotary", x, positions, inv_freq, sections, rotate_heads, num_prefix);
-  return at::empty_like(x.stride(3) == 1 ? x : x.contiguous());
+  return rotary_out(x.sym_stride(3) == 1 ? x : x.contiguous());
 }
 
-Tensor& rotary_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix,
-                bool interleaved) {
-  no_grad("rotary_", {x});
+void rotary_check_(const Tensor& x) {
+  REQUIRE(x.sym_numel() == 0 || (x.sym_stride(3) == 1 && apart(x)), "rotary_", "x must have dense heads and no overlapping elements to be turned in place");
+}
+void rotary_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix,
+             bool interleaved) {
+  no_grad("rotary_", {x, positions, inv_freq});
   const HalfType h = rotary_check("rotary_", x, positions, inv_freq, sections, rotate_heads, num_prefix);
-  bool dense = x.stride(3) == 1;
-  for (int64_t i = 0; i < 4; ++i) dense = dense && (x.stride(i) != 0 || x.size(i) == 1);
-  REQUIRE(dense, "rotary_", "x must have dense heads and no expanded dimension to be turned in place");
+  rotary_check_(x);
   c10::DeviceGuard guard(x.device());
   rotary_into(h, x, x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, false);
   if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
-  return x;
 }
-Tensor& rotary_meta_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix, bool) {
+void rotary_meta_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix, bool) {
   rotary_check("rotary_", x, positions, inv_freq, sections, rotate_heads, num_prefix);
-  return x;
+  rotary_check_(x);
 }
 
 // ================================================================ linear
@@ -329,15 +365,18 @@ int activation(const char* op, c10::string_view a) {
 
 int linear_check(const char* op, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, c10::string_view act,
                  int64_t multiple) {
-  REQUIRE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(1) % multiple == 0 && weight.numel() > 0, op, "weight ",
-          weight.sizes(), " does not match input ", x.sizes(), " (K must be a multiple of ", multiple, ")");
-  const int64_t K = weight.size(1), N = weight.size(0);
-  REQUIRE(K * (int64_t)weight.element_size() <= (1 << 23) && N <= (1 << 22) && x.numel() / K <= ROWS_MAX, op,
+  REQUIRE(x.dim() >= 1 && weight.dim() == 2 && weight.sym_size(1) == x.sym_size(-1) && weight.sym_size(1) % multiple == 0 && weight.sym_numel() > 0, op,
+          "weight ", weight.sym_sizes(), " does not match input ", x.sym_sizes(), " (K must be a multiple of ", multiple, ")");
+  const c10::SymInt K = weight.sym_size(1), N = weight.sym_size(0);
+  REQUIRE(K * (int64_t)weight.element_size() <= (1 << 23) && N <= (1 << 22) && x.sym_numel() <= K * ROWS_MAX, op,
           "K is at most 2^23 bytes, N at most 2^22, the rows of x at most 2^30");
   const int code = activation(op, act);
-  REQUIRE(!bias || (bias->dim() == 1 && bias->size(0) == N), op, "bias ", bias->sizes(), ", expected [", N, "]");
-  REQUIRE(!residual || residual->sizes() == at::IntArrayRef(with_last(x, N)), op, "residual ", residual->sizes(), ", expected ", with_last(x, N),
-          " (it is not broadcast)");
+  REQUIRE(!bias || (bias->dim() == 1 && bias->sym_size(0) == N), op, "bias ", bias->sym_sizes(), ", expected [", N, "]");
+  if (residual) {
+    const Sizes want = with_last(x, N);
+    REQUIRE(residual->sym_sizes() == c10::SymIntArrayRef(want), op, "residual ", residual->sym_sizes(), ", expected ", c10::SymIntArrayRef(want),
+            " (it is not broadcast)");
+  }
   same_place(op, x, weight);
   same_place(op, x, bias);
   same_place(op, x, residual);
@@ -365,7 +404,7 @@ void product(const Lib& l, const Tensor& x, const Tensor& w, const OptTensor& bi
 }
 
 Tensor linear_out(const Tensor& x, const Tensor& weight, const OptTensor& residual, ScalarType t) {
-  return at::empty(with_last(x, weight.size(0)), x.options().dtype(residual ? residual->scalar_type() : t));
+  return empty(with_last(x, weight.sym_size(0)), x, residual ? residual->scalar_type() : t);
 }
 
 std::tuple<Tensor, Tensor> linear_act_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
@@ -386,7 +425,7 @@ std::tuple<Tensor, Tensor> linear_act_forward_meta(const Tensor& x, const Tensor
   linear_check("linear_act", x, weight, bias, residual, act, 8);
   linear_half("linear_act", x, weight, bias, residual);
   Tensor y = linear_out(x, weight, residual, x.scalar_type());
-  return {y, save_pre ? at::empty(y.sizes(), x.options()) : none(x, x.scalar_type())};
+  return {y, save_pre ? empty(y.sym_sizes(), x, x.scalar_type()) : none(x, x.scalar_type())};
 }
 
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -400,10 +439,15 @@ Tensor transposed(const Lib& l, const Tensor& t, void* st) {
 
 std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& pre, c10::string_view act,
                                                        bool need_x, bool need_w, bool need_b, ScalarType bias_dtype) {
-  const int code = activation("linear_act", act);
+  const int code = linear_check("linear_act_backward", x, weight, std::nullopt, dy, act, 8);
+  linear_half("linear_act_backward", x, weight, pre, dy);
+  REQUIRE(code == MVIT_ACT_NONE || (pre.sizes() == dy.sizes() && pre.scalar_type() == x.scalar_type() && pre.is_contiguous()), "linear_act_backward",
+          "pre ", pre.sizes(), " of ", dy.sizes());
+  same_place("linear_act_backward", x, pre);
   c10::DeviceGuard guard(x.device());
   const ScalarType t = x.scalar_type();
   const int64_t N = weight.size(0), K = weight.size(1), M = x.numel() / K;
+  REQUIRE(!need_w || M <= (1 << 22), "linear_act_backward", "more than 2^22 rows of x with a gradient of weight");
   Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : none(x, t);
   Tensor dw = need_w ? at::empty({N, K}, x.options()) : none(x, t);
   Tensor db = need_b ? at::empty({N}, x.options().dtype(bias_dtype)) : none(x, bias_dtype);
@@ -435,8 +479,8 @@ std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const T
 std::tuple<Tensor, Tensor, Tensor> linear_act_backward_meta(const Tensor&, const Tensor& x, const Tensor& weight, const Tensor&, c10::string_view,
                                                             bool need_x, bool need_w, bool need_b, ScalarType bias_dtype) {
   const ScalarType t = x.scalar_type();
-  return {need_x ? at::empty(x.sizes(), x.options()) : none(x, t), need_w ? at::empty(weight.sizes(), x.options()) : none(x, t),
-          need_b ? at::empty({weight.size(0)}, x.options().dtype(bias_dtype)) : none(x, bias_dtype)};
+  return {need_x ? empty(x.sym_sizes(), x, t) : none(x, t), need_w ? empty(weight.sym_sizes(), x, t) : none(x, t),
+          need_b ? empty(weight.sym_sizes().slice(0, 1), x, bias_dtype) : none(x, bias_dtype)};
 }
 
 int linear_fp8_check(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& w_scale, const OptTensor& bias,
@@ -445,10 +489,10 @@ int linear_fp8_check(const Tensor& x, const Tensor& x_scale, const Tensor& weigh
   REQUIRE(x.scalar_type() == at::kFloat8_e4m3fn && weight.scalar_type() == at::kFloat8_e4m3fn, op, "x and weight are float8_e4m3fn, got ",
           x.scalar_type(), " and ", weight.scalar_type());
   const int code = linear_check(op, x, weight, bias, residual, act, 16);
-  REQUIRE(x_scale.scalar_type() == at::kFloat && w_scale.scalar_type() == at::kFloat && x_scale.sizes() == x.sizes().slice(0, x.dim() - 1) &&
-              w_scale.sizes() == weight.sizes().slice(0, 1),
-          op, "float32 scales ", x.sizes().slice(0, x.dim() - 1), " and ", weight.sizes().slice(0, 1), ", got ", x_scale.scalar_type(), " ",
-          x_scale.sizes(), " and ", w_scale.scalar_type(), " ", w_scale.sizes());
+  const c10::SymIntArrayRef rows = x.sym_sizes().slice(0, x.dim() - 1), columns = weight.sym_sizes().slice(0, 1);
+  REQUIRE(x_scale.scalar_type() == at::kFloat && w_scale.scalar_type() == at::kFloat && x_scale.sym_sizes() == rows && w_scale.sym_sizes() == columns, op,
+          "float32 scales ", rows, " and ", columns, ", got ", x_scale.scalar_type(), " ", x_scale.sym_sizes(), " and ", w_scale.scalar_type(), " ",
+          w_scale.sym_sizes());
   same_place(op, x, x_scale);
   same_place(op, x, w_scale);
   REQUIRE(is_half(out_dtype) || out_dtype == at::kFloat, op, "out_dtype ", out_dtype);
@@ -579,6 +623,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 };
 Tensor rotary_forward_autograd(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
                                int64_t num_prefix, bool interleaved, bool inverse) {
+  TORCH_CHECK(!wants_grad({positions, inv_freq}), "mvit::rotary has no gradient of positions and inv_freq: detach them");
   if (wants_grad({x})) return Rotary::apply(x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
   at::AutoDispatchBelowAutograd below;
   return rotary_op().call(x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
@@ -588,7 +633,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                                std::string act) {
     // (the K axis of dW = dz^T x)
-    REQUIRE(!weight.requires_grad() || x.numel() / weight.size(1) <= (1 << 22), "linear_act", "more than 2^22 rows of x with a gradient of weight");
+    REQUIRE(!weight.requires_grad() || x.sym_numel() <= weight.sym_size(1) * (1 << 22), "linear_act", "more than 2^22 rows of x with a gradient of weight");
     at::AutoDispatchBelowAutograd below;
     const bool keep = act != "none" && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
     auto [y, pre] = linear_forward_op().call(x, weight, bias, residual, act, keep);
@@ -682,8 +727,7 @@ TORCH_LIBRARY_FRAGMENT(mvit, m) {
   m.def("quantize_fp8(Tensor x) -> (Tensor, Tensor)");
   m.def("rotary_forward(Tensor x, Tensor positions, Tensor inv_freq, int[] sections, int rotate_heads, int num_prefix, bool interleaved, "
         "bool inverse) -> Tensor");
-  m.def("rotary_(Tensor(a!) x, Tensor positions, Tensor inv_freq, int[] sections, int rotate_heads, int num_prefix, bool interleaved) -> "
-        "Tensor(a!)");
+  m.def("rotary_(Tensor(a!) x, Tensor positions, Tensor inv_freq, int[] sections, int rotate_heads, int num_prefix, bool interleaved) -> ()");
   m.def("linear_act_forward(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation, bool save_pre) -> (Tensor, Tensor)");
   m.def("linear_act_backward(Tensor dy, Tensor x, Tensor weight, Tensor pre, str activation, bool need_x, bool need_w, bool need_b, "
         "ScalarType bias_dtype) -> (Tensor, Tensor, Tensor)");
@@ -712,7 +756,7 @@ TORCH_LIBRARY_IMPL(mvit, Meta, m) {
   m.impl("linear_act_backward", linear_act_backward_meta);
   m.impl("linear_fp8", linear_fp8_meta);
 }
-TORCH_LIBRARY_IMPL(mvit, AutogradCUDA, m) {
+TORCH_LIBRARY_IMPL(mvit, Autograd, m) {
   m.impl("rms_norm_forward", rms_norm_forward_autograd);
   m.impl("rms_norm_backward", rms_norm_backward_autograd);
   m.impl("rotary_forward", rotary_forward_autograd);

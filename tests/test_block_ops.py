@@ -936,3 +936,204 @@ def test_saved_tensors_changed_in_place_are_noticed():
         ops.rotary_(p, torch.zeros(3, 1, device="cuda", dtype=torch.int32), torch.ones(4, device="cuda"), [4])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         z.sum().backward()
+
+
+# ------------------------------------------------------------------ calls that the documentation allows, at its edges
+def test_shapes_of_sizes_that_vary():
+    """the shape implementations with a symbolic number of rows, as a compiled model is traced for other batch sizes"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
+    ops, mode = T(), FakeTensorMode(shape_env=ShapeEnv())
+    x = mode.from_tensor(torch.empty(6, 64, dtype=torch.bfloat16, device="meta"),
+                         symbolic_context=StatelessSymbolicContext(dynamic_sizes=[DimDynamic.DYNAMIC, DimDynamic.STATIC]))
+    rows = x.shape[0]
+    assert not isinstance(rows, int)
+    with mode:
+        w, lw, b = (torch.empty(*s, device="meta") for s in ((64,), (48, 64), (48,)))
+        y, h = ops.add_rms_norm(x, x.float(), w)
+        assert y.shape == (rows, 64) and h.shape == (rows, 64) and y.shape[0] is not int
+        (q, s), (wq, ws) = ops.quantize_fp8(y), ops.quantize_fp8(lw)
+        assert q.shape == (rows, 64) and s.shape == (rows,)
+        assert ops.linear_act(x, lw.to(x.dtype), b, None, "gelu").shape == (rows, 48)
+        assert ops.linear_fp8(q, s, wq, ws, b, None, "silu").shape == (rows, 48)
+        pos, freq = torch.empty(x.shape[0], 1, dtype=torch.int32, device="meta"), torch.empty(8, device="meta")
+        assert ops.rotary(x.view(1, -1, 4, 16), pos, freq, [8]).shape == (1, rows, 4, 16)
+        with pytest.raises(ValueError, match="mvit::"):
+            ops.linear_act(x, lw[:, :56].to(x.dtype))
+
+
+def test_rotary_of_overlapping_windows():
+    """heads that are sliding windows of one row: an input may overlap, what is written may not"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = T()
+    with FakeTensorMode():
+        x = fake(2, 7, 20).unfold(2, 16, 1)
+        p, fr = fake(7, 1, dtype=torch.int32), fake(8, dtype=torch.float32)
+        assert x.stride()[2:] == (1, 1)
+        y = ops.rotary(x, p, fr, [8])
+        assert y.shape == x.shape and y.stride(3) == 1 and y.is_contiguous()
+        for z in (x, fake(2, 7, 36).unfold(2, 16, 4), fake(2, 5, 3, 16).expand(2, 5, 3, 16)[:, :1].expand(2, 7, 3, 16)):
+            with pytest.raises(ValueError, match="in place"):
+                ops.rotary_(z, p, fr, [8])
+        ops.rotary_(fake(7, 2, 3, 16).transpose(0, 1), p, fr, [8])      # apart in any order
+        ops.rotary_(fake(2, 7, 5, 32)[:, :, ::2, 8:24], p, fr, [8])
+
+
+@pytest.mark.gpu
+def test_rotary_of_overlapping_windows_on_the_gpu():
+    ops, g = T(), gen(51)
+    x = randn(g, 2, 7, 20, dtype=torch.bfloat16).unfold(2, 16, 1)
+    p, fr = torch.arange(7, device="cuda", dtype=torch.int32)[:, None], ops.rotary_frequencies([8], device="cuda")
+    for il in (False, True):
+        assert torch.equal(ops.rotary(x, p, fr, [8], interleaved=il), ops.rotary(x.contiguous(), p, fr, [8], interleaved=il))
+
+
+@pytest.mark.gpu
+def test_positions_and_frequencies_have_no_gradient():
+    ops = T()
+    x = torch.randn(1, 3, 2, 8, device="cuda")
+    p, fr = torch.zeros(3, 1, device="cuda"), torch.ones(4, device="cuda")
+    for a, b in ((p.clone().requires_grad_(), fr), (p, fr.clone().requires_grad_())):
+        for f in (ops.rotary, ops.rotary_):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                f(x, a, b, [4])
+        with torch.no_grad():
+            ops.rotary(x, a, b, [4])
+
+
+@pytest.mark.gpu
+def test_backward_operators_refuse_what_does_not_belong_together():
+    m = torch.ops.mvit
+    x, w, dy = (torch.zeros(*s, device="cuda", dtype=torch.bfloat16) for s in ((4, 16), (8, 16), (4, 8)))
+    for args in ((dy[:3], x, w, dy, "gelu"), (dy, x, w, dy[:3], "gelu"), (dy, x, w, x.new_empty(0), "silu"), (dy, x, w, dy.float(), "silu"),
+                 (dy, x, w[:, :8], dy, "none"), (dy, x.half(), w, dy, "none")):
+        with pytest.raises(ValueError, match="mvit::"):
+            m.linear_act_backward(*args, True, True, True, torch.float32)
+    v, rstd = torch.ones(16, device="cuda"), torch.ones(4, device="cuda")
+    for args in ((x[:3], None, x, v, rstd), (x, x[:3], x, v, rstd), (x, None, x, v[:8], rstd), (x, None, x, v, rstd[:3]), (x, None, x, v, rstd.cpu())):
+        with pytest.raises(ValueError, match="mvit::"):
+            m.rms_norm_backward(*args, torch.bfloat16, True, False, True)
+
+
+@pytest.mark.gpu
+def test_compiled_at_several_batch_sizes():
+    """one compiled model, forward and backward, at batch sizes that it was not traced with; the in-place turn among its operators"""
+    ops, g = T(), gen(52)
+    w, wt, b = randn(g, 64), randn(g, 96, 64, dtype=torch.bfloat16), randn(g, 96)
+    freq = ops.rotary_frequencies([16], device="cuda")
+
+    def f(x, r, w, wt, b, pos):
+        y, h = ops.add_rms_norm(x, r, w)
+        z = ops.linear_act(y, wt, b, None, "gelu")
+        return ops.rotary(z.view(1, -1, 3, 32), pos, freq, [16], 2), h
+
+    def serve(x, wt, pos):
+        q, s = ops.quantize_fp8(x)
+        z = ops.linear_fp8(q, s, *ops.quantize_fp8(wt)).view(1, -1, 3, 32)
+        return ops.rotary_(z, pos, freq, [16], 2) * 2
+    cf = torch.compile(f, backend="aot_eager", fullgraph=True, dynamic=True)
+    cs = torch.compile(serve, backend="aot_eager", fullgraph=True, dynamic=True)
+    for M in (6, 9, 40):
+        x, r = randn(g, M, 64, dtype=torch.bfloat16), randn(g, M, 64)
+        pos = torch.arange(M, device="cuda", dtype=torch.int32)[:, None]
+        leaves = [t.clone().requires_grad_() for t in (x, r, w, wt, b)]
+        results = []
+        for fn in (f, cf):
+            y, h = fn(*leaves, pos)
+            results.append((y.detach(), h.detach(), *torch.autograd.grad((y.float().square().sum() + h.sum()), leaves)))
+        assert all(torch.equal(u, v) for u, v in zip(*results))
+        assert torch.equal(serve(x, wt, pos), cs(x, wt, pos))
+
+
+@pytest.mark.gpu
+def test_operators_keep_their_schemas():
+    """what torch itself checks of an operator: nothing written that is not declared, shapes as traced, autograd where it belongs"""
+    g, m = gen(53), torch.ops.mvit
+    x, r, w = randn(g, 6, 64, dtype=torch.bfloat16), randn(g, 6, 64), randn(g, 64)
+    wt, b = randn(g, 96, 64, dtype=torch.bfloat16), randn(g, 96)
+    z, pos, freq = randn(g, 1, 6, 3, 32), torch.arange(6, device="cuda")[:, None], torch.rand(16, device="cuda")
+    q, s = m.quantize_fp8(x)
+    wq, ws = m.quantize_fp8(wt)
+    grad = lambda *ts: [t.clone().requires_grad_() for t in ts]  # noqa: E731
+    for name, args in (("rms_norm_forward", (*grad(x, r, w), 1e-6, None)), ("rms_norm_forward", (x, None, w, 1e-6, None)),
+                       ("rms_norm_fp8", (x, r, w, 1e-6)), ("quantize_fp8", (x,)), ("rotary_forward", (*grad(z), pos, freq, [16], 2, 1 - 1, False, False)),
+                       ("rotary_", (z, pos, freq, [16], 2, 0, False)), ("linear_act_forward", (*grad(x, wt, b, r.repeat(1, 2)[:, :96]), "silu", False)),
+                       ("linear_fp8", (q, s, wq, ws, b, None, "gelu", torch.bfloat16))):
+        # (torch's schema check compares by arithmetic that it does not have for e4m3 tensors)
+        utils = ("test_autograd_registration", "test_faketensor") + (() if "fp8" in name else ("test_schema",))
+        torch.library.opcheck(getattr(m, name).default, args, test_utils=utils)
+
+
+@pytest.mark.gpu
+def test_linear_fp8_operands_in_place():
+    """8-bit operands as slices: on 16 bytes as they are, else copied; scales with strides"""
+    ops, g = T(), gen(54)
+    for M in (3, 45):
+        (q, s), (wq, ws) = ops.quantize_fp8(randn(g, M, 64)), ops.quantize_fp8(randn(g, 40, 64))
+        want = ops.linear_fp8(q, s, wq, ws)
+        for lo in (0, 16, 5):
+            wide, wwide = torch.zeros(M, 2, 96, device="cuda").to(q.dtype), torch.zeros(80, 96, device="cuda").to(q.dtype)
+            wide.view(torch.uint8)[:, 1, lo:lo + 64] = q.view(torch.uint8)
+            wwide.view(torch.uint8)[::2, lo:lo + 64] = wq.view(torch.uint8)
+            ss = torch.stack((s, s), 1)[:, 1]
+            assert torch.equal(ops.linear_fp8(wide[:, 1, lo:lo + 64], ss, wwide[::2, lo:lo + 64], ws.repeat_interleave(2)[::2]), want)
+
+
+@pytest.mark.gpu
+def test_rows_far_apart():
+    """row strides up to 2^23 bytes, the most that is used without a copy: offsets of a tile's 256 rows up to 31 bits"""
+    ops, g = T(), gen(55)
+    M, N = 1030, 4608
+    for es, stride in ((2, 2 ** 22), (1, 2 ** 23)):
+        big = torch.empty(M, stride, device="cuda", dtype=torch.bfloat16 if es == 2 else torch.float8_e4m3fn)
+        x, w = randn(g, M, 64, dtype=torch.bfloat16), randn(g, N, 64, dtype=torch.bfloat16)
+        if es == 2:
+            big[:, -64:] = x
+            assert torch.equal(ops.linear_act(big[:, -64:], w), ops.linear_act(x, w))
+        else:
+            (q, s), (wq, ws) = ops.quantize_fp8(x), ops.quantize_fp8(w)
+            big.view(torch.uint8)[:, -64:] = q.view(torch.uint8)
+            for out in (torch.bfloat16, torch.float32):
+                assert torch.equal(ops.linear_fp8(big[:, -64:], s, wq, ws, out_dtype=out), ops.linear_fp8(q, s, wq, ws, out_dtype=out))
+        del big
+
+
+@pytest.mark.gpu
+def test_long_offsets():
+    """more than 2^31 elements: the last rows as a small call gives them, forward and backward"""
+    ops, g = T(), gen(56)
+    M, D = 2 ** 17 + 5, 16384
+    tail = slice(M - 8, M)
+    x = torch.zeros(M, D, device="cuda", dtype=torch.bfloat16)
+    x[tail] = randn(g, 8, D, dtype=torch.bfloat16)
+    w = randn(g, D)
+    few = x[tail].clone().requires_grad_()
+    q, s = ops.quantize_fp8(x)
+    q8, s8 = ops.quantize_fp8(few.detach())
+    assert torch.equal(q[tail].view(torch.uint8), q8.view(torch.uint8)) and torch.equal(s[tail], s8) and not q[:8].view(torch.uint8).any()
+    del q, s
+    dy = torch.zeros_like(x)
+    dy[tail] = randn(g, 8, D, dtype=torch.bfloat16)
+    x.requires_grad_()
+    y = ops.rms_norm(x, w)
+    y8 = ops.rms_norm(few, w)
+    (dx,), (dx8,) = torch.autograd.grad(y, x, dy), torch.autograd.grad(y8, few, dy[tail])
+    assert torch.equal(y.detach()[tail], y8.detach()) and torch.equal(dx[tail], dx8) and not dx[:8].any()
+    del x, y, dx, dy
+    M, K, N = 2 ** 17 + 5, 16, 16400
+    tail = slice(M - 5, M)
+    x, w, b = randn(g, M, K, dtype=torch.bfloat16), randn(g, N, K, dtype=torch.bfloat16).requires_grad_(), randn(g, N).requires_grad_()
+    r = torch.ones(M, N, device="cuda", dtype=torch.bfloat16)
+    x.requires_grad_()
+    y = ops.linear_act(x, w, b, r, "silu")
+    dy = torch.zeros_like(r)
+    dy[tail] = randn(g, 5, N, dtype=torch.bfloat16)
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    few = x.detach()[tail].clone().requires_grad_()
+    y5 = ops.linear_act(few, w, b, r[tail], "silu")
+    want = torch.autograd.grad(y5, (few, w, b), dy[tail])
+    for u, v in zip((y.detach()[tail], got[0][tail], *got[1:]), (y5.detach(), *want)):
+        # other kernels, other orders of the same sums: the kept z may round to the neighbouring 16-bit value, which moves dz by at most a unit
+        # of z times silu'' <= 2^-7 * 0.31 times |dy| <= 5, times |x| or |w| <= 5: 0.06; and a unit of the result's own rounding
+        assert ((u.float() - v.float()).abs() <= 2.0 ** -7 * v.float().abs() + 0.06).all()
+    assert not got[0][:8].any()
