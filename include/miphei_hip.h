@@ -216,17 +216,20 @@ typedef struct mvit_linear_args {
 } mvit_linear_args;
 MVIT_API int mvit_linear_act(const mvit_linear_args* args, mvit_stream_t stream);
 MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_stream_t stream);
-/* Backward of the epilogue: dz(16-bit) = dy * act'(pre), rows [M, ld_dz] and transposed [N, ld_dzt], dbias[N] (f32 or 16-bit) = its sum
- * over the rows, taken before dz is rounded; each of them may be NULL (dzt only beside dz).  dy [M, N] f32 or 16-bit and pre (16-bit; may be
- * NULL where act is none) dense; ld_dz, ld_dzt are multiples of 8 with ld_dz >= N, M <= ld_dzt < M + 8, dz and dzt start on 16 bytes; what
- * pads a row of dzt, and a row of dz up to ld_dz where N is no multiple of 8, is zero.  scratch: mvit_act_bwd_scratch_bytes(M, N) bytes
- * (needed with dbias only); ordered sums, bit-identical from run to run.  dx and dW are the products dz W and dz^T x (mvit_linear_act). */
+/* The products of its backward pass, 16-bit, f32 accumulation, of operands as they lie in memory: x_rows = 0: y[M,N] = x[M,K] W[K,N] (dx = dz W,
+ * x's rows padded by zeros to a multiple of 8); x_rows = 1: y[M,N] = x[K,M]^T W[K,N] (dW = dz^T x, ldx at least M rounded up to 8).  N and the
+ * row strides ldx, ldw are multiples of 8, at most 2^23 bytes; x, W, y start on 16 bytes; y dense.  K up to 2^29 (x_rows = 0: 2^22).  The other
+ * members are 0.  scratch: mvit_linear_grad_scratch_bytes(M, N, K) bytes, on 16 bytes: products of parts of K, added in order (none where that
+ * is 0). */
+MVIT_API long long mvit_linear_grad_scratch_bytes(int M, int N, int K);
+MVIT_API int mvit_linear_grad(const mvit_linear_args* args, int x_rows, void* scratch, long long scratch_bytes, mvit_stream_t stream);
+/* Backward of the epilogue: dz(16-bit)[M, ld_dz] = dy * act'(pre) and dbias[N] (f32 or 16-bit) = its sum over the rows, taken before dz is
+ * rounded; either may be NULL.  dy [M, N] f32 or 16-bit and pre (16-bit; may be NULL where act is none) dense; ld_dz a multiple of 8, at least N,
+ * dz starts on 16 bytes; what pads a row of dz up to ld_dz where N is no multiple of 8 is zero.  scratch: mvit_act_bwd_scratch_bytes(M, N)
+ * bytes (needed with dbias only); ordered sums, bit-identical from run to run. */
 MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N);
-MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dzt, long long ld_dzt,
-                          void* dbias, int dbias_f32, void* scratch, int M, int N, mvit_stream_t stream);
-/* dst[c][r] = src[r][c] (16-bit), rows of dst padded by zeros to ld_dst, R <= ld_dst < R + 8.  ld, ld_dst multiples of 8, ld at least Cc
- * rounded up to 8, src and dst start on 16 bytes. */
-MVIT_API int mvit_transpose_padded(const void* src, long long ld, void* dst, long long ld_dst, int R, int Cc, mvit_stream_t stream);
+MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dbias, int dbias_f32, void* scratch,
+                          int M, int N, mvit_stream_t stream);
 
 /* ---------------------------------------------------------------- decoder data movement (NHWC bf16) */
 /* dst[b,oy,ox,c] = sum_{ty,tx} ty_w[oy,ty]*tx_w[ox,tx] * f(src[b, ty_idx[oy,ty], tx_idx[ox,tx], c]),

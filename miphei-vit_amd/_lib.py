@@ -137,8 +137,9 @@ SIGNATURES = {
     "mvit_rotary": [C.POINTER(RotaryArgs), vp],
     "mvit_linear_act": [C.POINTER(LinearArgs), vp],
     "mvit_linear_fp8": [C.POINTER(LinearArgs), vp],
-    "mvit_act_bwd": [vp, ci, vp, ci, vp, ll, vp, ll, vp, ci, vp, ci, ci, vp],
-    "mvit_transpose_padded": [vp, ll, vp, ll, ci, ci, vp],
+    "mvit_act_bwd": [vp, ci, vp, ci, vp, ll, vp, ci, vp, ci, ci, vp],
+    "mvit_linear_grad": [vp, ci, vp, ll, vp],
+    "mvit_linear_grad_scratch_bytes": [ci, ci, ci],
     "mvit_act_bwd_scratch_bytes": [ci, ci],
     "mvit_occupy_cus": [ci, ci, vp],
 }

@@ -141,7 +141,7 @@ def grid_positions(*sizes: int, device=None) -> Tensor:
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None, activation: str = "none") -> Tensor:
     """residual + act(x @ weight^T + bias) in one launch; act: none, relu, silu, gelu (erf) or gelu_tanh.
 
-    x [..., K], weight [N, K]: both bf16 or both fp16, K a multiple of 8 (at most 2^22, and so N; at most 2^22 rows of x where weight's
+    x [..., K], weight [N, K]: both bf16 or both fp16, K a multiple of 8 (at most 2^22, and so N; at most 2^29 rows of x where weight's
     gradient is wanted); bias [N] and residual [..., N]: that type or f32.  The output has
     the residual's type (f32: a residual stream), else x's.  f32 accumulation, one rounding at the end.  Differentiable in x, weight, bias
     and residual; the value in front of the activation is kept in 16 bits for it."""

@@ -8,15 +8,19 @@ using namespace mvit_linear;
 namespace mvit_linear {
 template <int MODE, bool OUT32>
 int dispatch(const Args& a, bool vec, hipStream_t s);   // linear_launch.hpp
+template <int MODE>
+int dispatch_grad(const Args& a, int tile, hipStream_t s);
 extern template int dispatch<H16, false>(const Args&, bool, hipStream_t);
 extern template int dispatch<H16, true>(const Args&, bool, hipStream_t);
 extern template int dispatch<F8, false>(const Args&, bool, hipStream_t);
 extern template int dispatch<F8X, true>(const Args&, bool, hipStream_t);
+extern template int dispatch_grad<DX>(const Args&, int, hipStream_t);
+extern template int dispatch_grad<DW>(const Args&, int, hipStream_t);
 }  // namespace mvit_linear
 
 namespace {
 
-constexpr int MAX_M = 1 << 30, MAX_N = 1 << 24;   // tile numbers and grids stay in 31 bits
+constexpr int MAX_M = 1 << 30, MAX_N = 1 << 24, MAX_K = 1 << 29;   // tile numbers, grids and bytes of K stay in 31 bits
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -33,7 +37,7 @@ int check(const mvit_linear_args* g, int es, Args& a, bool& vec) {
   if (g->res && g->ldr < g->N) return MVIT_EINVAL;
   const int ye = g->y_f32 ? 4 : 2;
   a = {(const char*)g->x, (const char*)g->w, g->bias, g->res, g->y, g->pre, g->x_scale, g->w_scale, g->res ? g->ldr : 0, (unsigned)lx, (unsigned)lw,
-       g->M, g->N, (int)kb, g->act, g->bias_f32, g->act == MVIT_ACT_RELU ? 0.f : -INFINITY};
+       g->M, g->N, (int)kb, g->act, g->bias_f32, g->act == MVIT_ACT_RELU ? 0.f : -INFINITY, 0, 0, 1, nullptr};
   vec = g->N % 8 == 0 && aligned16(g->y) && aligned16(g->pre) && aligned16(g->res) && (!g->res || g->ldr * ye % 16 == 0);
   return 0;
 }
@@ -57,13 +61,79 @@ extern "C" MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_strea
   return args->y_f32 ? dispatch<F8X, true>(a, vec, (hipStream_t)stream) : dispatch<F8, false>(a, vec, (hipStream_t)stream);
 }
 
+// ---------------------------------------------------------------- the gradients' products
+namespace {
+
+// Which tile, and K in how many parts: dW has few tiles and a K axis of all rows, dx of few rows few tiles.  The parts' f32 products are added
+// by a second launch, in order.  By what it costs, in tenths of a microsecond: 40 for a round of blocks and, for each of its K tiles of 64, with
+// the tiles of 256 x 256, 128 x 256, 128 x 128 and 64 x 64, 16, 10, 10 and 4 (7 and 3 with one block a CU); 50 for the second launch and
+// 8 bytes an output and part at 5 TB/s.  us without and with splits: dW
+// [1536, 1536] of 21056 rows 252 / 96, of 5264 rows 52 / 39, [64, 512] of 20816 rows 86 / 13, [4096, 1536] of 21056 rows 289 / 251; dx [33, 1536] of
+// 4096 columns 18 / 10, [329, 1536] 19 / 15
+struct Plan {
+  int tile, splits, kper;
+};
+Plan plan_grad(int M, int N, int K) {
+  static constexpr int BM[4] = {256, 128, 128, 64}, BN[4] = {256, 256, 128, 64}, full[4] = {16, 10, 10, 4}, alone[4] = {16, 10, 7, 3};
+  const long long cus = mvit_num_cus(), nk = ((long long)K + 63) / 64;
+  Plan best = {0, 1, (int)nk};
+  double least = 1e300;
+  for (int t = 0; t < 4; ++t) {
+    const long long tiles = (((long long)M + BM[t] - 1) / BM[t]) * (((long long)N + BN[t] - 1) / BN[t]), slots = t < 2 ? cus : 2 * cus;
+    for (int want = 1; want <= 64; ++want) {
+      const long long kper = (nk + want - 1) / want, s = (nk + kper - 1) / kper, n = tiles * s;
+      if (s != want || (want > 1 && kper < 4)) continue;
+      double c = (double)((n + slots - 1) / slots) * (40. + (double)(n <= cus ? alone[t] : full[t]) * kper);
+      if (s > 1) c += 50. + (double)s * M * N * 8. / 5e5;
+      if (c < least) least = c, best = {t, (int)s, (int)kper};
+    }
+  }
+  return best;
+}
+
+// 4 outputs a thread
+__global__ __launch_bounds__(256) void sum_splits(const float* part, bf16_t* y, int splits, long long n4) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
+    f32x4 s = *(const f32x4*)(part + i * 4);
+#pragma unroll 4
+    for (int k = 1; k < splits; ++k) s += *(const f32x4*)(part + (k * n4 + i) * 4);
+    *(uint2*)(y + i * 4) = make_uint2(pack2bf(s[0], s[1]), pack2bf(s[2], s[3]));
+  }
+}
+
+}  // namespace
+
+extern "C" MVIT_API long long mvit_linear_grad_scratch_bytes(int M, int N, int K) {
+  if (M <= 0 || M > MAX_M || N <= 0 || N > MAX_N || K <= 0 || K > MAX_K) return 0;
+  const Plan p = plan_grad(M, N, K);
+  return p.splits > 1 ? (long long)p.splits * M * N * 4 : 0;
+}
+
+extern "C" MVIT_API int mvit_linear_grad(const mvit_linear_args* g, int x_rows, void* scratch, long long scratch_bytes, mvit_stream_t stream) {
+  MVIT_CLEAR_ERROR();
+  if (!g || g->M <= 0 || g->M > MAX_M || g->N <= 0 || g->N > MAX_N || g->K <= 0 || g->K > MAX_K || !g->x || !g->w || !g->y) return MVIT_EINVAL;
+  if (g->bias || g->res || g->pre || g->x_scale || g->w_scale || g->act != MVIT_ACT_NONE || g->y_f32) return MVIT_EINVAL;
+  // 16-byte pieces of the rows in memory; 31-bit offsets inside a block's rows
+  const long long lx = g->ldx * 2, lw = g->ldw * 2, up8 = (g->K + 7LL) / 8 * 8;
+  if (lx % 16 || lw % 16 || lx > (1 << 23) || lw > (1 << 23) || g->N % 8 || g->ldw < g->N || !aligned16(g->x) || !aligned16(g->w) || !aligned16(g->y))
+    return MVIT_EINVAL;
+  if (g->ldx < (x_rows ? (g->M + 7LL) / 8 * 8 : up8)) return MVIT_EINVAL;   // (x_rows = 0: and so K is at most 2^22)
+  const Plan plan = plan_grad(g->M, g->N, g->K);
+  if (plan.splits > 1 && (!scratch || !aligned16(scratch) || scratch_bytes < mvit_linear_grad_scratch_bytes(g->M, g->N, g->K))) return MVIT_EINVAL;
+  hipStream_t s = (hipStream_t)stream;
+  const Args a = {(const char*)g->x, (const char*)g->w, nullptr, nullptr, g->y, nullptr, nullptr, nullptr, 0, (unsigned)lx, (unsigned)lw,
+                  g->M, g->N, (int)(up8 * 2), MVIT_ACT_NONE, 0, -INFINITY, g->K, plan.kper, plan.splits, (float*)scratch};
+  if (const int rc = x_rows ? dispatch_grad<DW>(a, plan.tile, s) : dispatch_grad<DX>(a, plan.tile, s)) return rc;
+  if (plan.splits == 1) return MVIT_OK;
+  const long long n4 = (long long)g->M * g->N / 4, blocks = (n4 + 255) / 256, most = (long long)mvit_num_cus() * 16;
+  hipLaunchKernelGGL(sum_splits, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, (const float*)scratch, (bf16_t*)g->y, plan.splits, n4);
+  return MVIT_LAUNCH_CHECK();
+}
+
 // ---------------------------------------------------------------- backward of the epilogue
-// dz = dy act'(pre), as rows and transposed, and its column sums, in one pass over dy and pre: bound by HBM.  The transposed copy is an
-// operand of dW = dz^T x, whose K axis is the rows; made from the values at hand it costs its write alone, a third of a transposition
-// by itself.  A block owns 64 columns and a run of rows, and goes down it by 64 x 64 tiles: a thread takes 8 columns of rows 2 r and
-// 2 r + 1 (16-byte loads), packs pairs of rows into LDS [column][row], and reads 8 rows of a column back.  Column stride 136 bytes: the 64
-// writes of a wave fall on 64 banks.  Sums over a run stay in registers, the runs meet in a f32 workspace (column_sums.hpp).
-// The same kernel with the identity and no sums transposes x and W.
+// dz = dy act'(pre) and its column sums, in one pass over dy and pre: bound by HBM ([5264, 4096] bf16, gelu: 24 us, 129 MB, 5.3 TB/s).  A block owns 256
+// columns and a run of rows: 32 lanes of 8 columns (16-byte loads) by 8 rows at a time.  Sums over a run stay in registers, then LDS; the
+// runs meet in a f32 workspace (column_sums.hpp): a fixed order, no atomics.
 namespace {
 
 enum Slope { S_ONE, S_CLIP, S_SILU, S_TANH, S_ERF, S_ANY };
@@ -96,74 +166,52 @@ __device__ __forceinline__ float slope(float z, int act) {
 struct SlopeArgs {
   const void* dy;
   const bf16_t* pre;
-  bf16_t *dz, *dzt;
+  bf16_t* dz;
   float* part;
-  long long ld, ld_dz, ld_dzt;   // ld: of dy (and of the source of a transposition); pre is dense
-  int M, N, rows, act;           // rows: of a run, a multiple of 64
+  long long ld_dz;          // dy and pre are dense
+  int M, N, rows, act;      // rows: of a run
 };
 
 template <int SL, bool F32>
-__global__ __launch_bounds__(256) void act_bwd_tiles(const SlopeArgs p) {
-  constexpr int LDT = 68;   // 16-bit values of a column in LDS
-  __shared__ __attribute__((aligned(16))) bf16_t tile[2][64 * LDT];
-  __shared__ float sums[32][65];
-  const int cg = threadIdx.x & 7, rp = threadIdx.x >> 3;
-  const int c0 = blockIdx.x * 64 + cg * 8;
-  const int r0 = blockIdx.y * p.rows, r1 = min(r0 + p.rows, (p.M + 63) / 64 * 64);
+__global__ __launch_bounds__(256) void act_bwd_rows(const SlopeArgs p) {
+  __shared__ float sums[8][256];
+  const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5, c0 = blockIdx.x * 256 + cg * 8;
+  const int r0 = blockIdx.y * p.rows, r1 = min(r0 + p.rows, p.M);
   float sum[8] = {};
-  int buf = 0;
-  for (int t = r0; t < r1; t += 64, buf ^= 1) {
-    float g[2][8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = t + rp * 2 + h;
-      const bool in = r < p.M && c0 < p.N;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[h][e] = 0.f;
-      if (in) {
-        const size_t o = (size_t)r * p.ld + c0;
-        if constexpr (F32) {
-          const float4 u = *(const float4*)((const float*)p.dy + o), v = *(const float4*)((const float*)p.dy + o + 4);
-          g[h][0] = u.x, g[h][1] = u.y, g[h][2] = u.z, g[h][3] = u.w, g[h][4] = v.x, g[h][5] = v.y, g[h][6] = v.z, g[h][7] = v.w;
-        } else {
-          const uint4 u = *(const uint4*)((const bf16_t*)p.dy + o);
-          g[h][0] = lo16f(u.x), g[h][1] = hi16f(u.x), g[h][2] = lo16f(u.y), g[h][3] = hi16f(u.y);
-          g[h][4] = lo16f(u.z), g[h][5] = hi16f(u.z), g[h][6] = lo16f(u.w), g[h][7] = hi16f(u.w);
-        }
-        if constexpr (SL != S_ONE) {
-          const uint4 u = *(const uint4*)(p.pre + (size_t)r * p.N + c0);
-          const float z[8] = {lo16f(u.x), hi16f(u.x), lo16f(u.y), hi16f(u.y), lo16f(u.z), hi16f(u.z), lo16f(u.w), hi16f(u.w)};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[h][e] *= slope<SL>(z[e], 0);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += g[h][e];
-        if (p.dz) *(uint4*)(p.dz + (size_t)r * p.ld_dz + c0) = pack8(g[h]);
+  if (c0 < p.N) {
+#pragma unroll 2
+    for (int r = r0 + rg; r < r1; r += 8) {
+      const size_t o = (size_t)r * p.N + c0;
+      float g[8];
+      if constexpr (F32) {
+        const float4 u = *(const float4*)((const float*)p.dy + o), v = *(const float4*)((const float*)p.dy + o + 4);
+        g[0] = u.x, g[1] = u.y, g[2] = u.z, g[3] = u.w, g[4] = v.x, g[5] = v.y, g[6] = v.z, g[7] = v.w;
+      } else {
+        const uint4 u = *(const uint4*)((const bf16_t*)p.dy + o);
+        g[0] = lo16f(u.x), g[1] = hi16f(u.x), g[2] = lo16f(u.y), g[3] = hi16f(u.y);
+        g[4] = lo16f(u.z), g[5] = hi16f(u.z), g[6] = lo16f(u.w), g[7] = hi16f(u.w);
       }
-    }
-    if (p.dzt) {
+      if constexpr (SL != S_ONE) {
+        const uint4 u = *(const uint4*)(p.pre + o);
+        const float z[8] = {lo16f(u.x), hi16f(u.x), lo16f(u.y), hi16f(u.y), lo16f(u.z), hi16f(u.z), lo16f(u.w), hi16f(u.w)};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) *(uint32_t*)&tile[buf][(cg * 8 + e) * LDT + rp * 2] = pack2bf(g[0][e], g[1][e]);
-      __syncthreads();   // (the other buffer's reads are two barriers away from its next writes)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = rp + h * 32, r = t + cg * 8;   // 8 lanes a column: 128 bytes in a line; rows from M to the end of the last piece: zeros
-        if (blockIdx.x * 64 + c < p.N && r < p.ld_dzt) {
-          const uint2 *s = (const uint2*)&tile[buf][c * LDT + cg * 8], u = s[0], v = s[1];
-          *(uint4*)(p.dzt + (size_t)(blockIdx.x * 64 + c) * p.ld_dzt + r) = make_uint4(u.x, u.y, v.x, v.y);
-        }
+        for (int e = 0; e < 8; ++e) g[e] *= slope<SL>(z[e], 0);
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += g[e];
+      if (p.dz) *(uint4*)(p.dz + (size_t)r * p.ld_dz + c0) = pack8(g);
     }
   }
   if (!p.part) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sums[rp][cg * 8 + e] = sum[e];
+  for (int e = 0; e < 8; ++e) sums[rg][cg * 8 + e] = sum[e];
   __syncthreads();
-  if (threadIdx.x < 64 && blockIdx.x * 64 + (int)threadIdx.x < p.N) {
-    float s = 0.f;
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < p.N) {
+    float s = sums[0][threadIdx.x];
 #pragma unroll
-    for (int k = 0; k < 32; ++k) s += sums[k][threadIdx.x];
-    p.part[(size_t)blockIdx.y * p.N + blockIdx.x * 64 + threadIdx.x] = s;
+    for (int k = 1; k < 8; ++k) s += sums[k][threadIdx.x];
+    p.part[(size_t)blockIdx.y * p.N + c] = s;
   }
 }
 
@@ -185,67 +233,53 @@ __global__ __launch_bounds__(256) void act_bwd_elements(const SlopeArgs p) {
   if (p.part && c < p.N) p.part[(size_t)blockIdx.y * p.N + c] = sum;
 }
 
-// rows of a run: blocks enough for sixteen a CU, no more than 128 runs to add up
+// rows of a run: blocks enough for eight a CU, no more than 128 runs to add up, no fewer than 8 rows
 int run_rows(int M, int N) {
-  const int tiles = (M + 63) / 64, cols = (N + 63) / 64;
-  int runs = (mvit_num_cus() * 16 + cols - 1) / cols;
+  const int cols = (N + 255) / 256;
+  int runs = (mvit_num_cus() * 8 + cols - 1) / cols;
   runs = runs > 128 ? 128 : runs;
-  runs = runs > tiles ? tiles : runs;
-  return (tiles + runs - 1) / runs * 64;
+  const int rows = (M + runs - 1) / runs;
+  return rows < 8 ? 8 : rows;
 }
 int run_count(int M, int N) { return M <= 0 ? 0 : (M + run_rows(M, N) - 1) / run_rows(M, N); }
 
 template <bool F32>
-void launch_tiles(const SlopeArgs& a, dim3 grid, hipStream_t s) {
+void launch_rows_bwd(const SlopeArgs& a, dim3 grid, hipStream_t s) {
   if (a.act == MVIT_ACT_NONE)
-    hipLaunchKernelGGL((act_bwd_tiles<S_ONE, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_ONE, F32>), grid, dim3(256), 0, s, a);
   else if (a.act == MVIT_ACT_RELU)
-    hipLaunchKernelGGL((act_bwd_tiles<S_CLIP, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_CLIP, F32>), grid, dim3(256), 0, s, a);
   else if (a.act == MVIT_ACT_GELU)
-    hipLaunchKernelGGL((act_bwd_tiles<S_ERF, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_ERF, F32>), grid, dim3(256), 0, s, a);
   else if (a.act == MVIT_ACT_SILU)
-    hipLaunchKernelGGL((act_bwd_tiles<S_SILU, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_SILU, F32>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((act_bwd_tiles<S_TANH, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_TANH, F32>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace
 
-extern "C" MVIT_API int mvit_transpose_padded(const void* src, long long ld, void* dst, long long ld_dst, int R, int Cc, mvit_stream_t stream) {
-  MVIT_CLEAR_ERROR();
-  if (!src || !dst || R <= 0 || R > MAX_M || Cc <= 0 || Cc > MAX_N || ld % 8 || ld_dst % 8 || ld < (Cc + 7) / 8 * 8 || ld_dst < R || ld_dst >= R + 8 || !aligned16(src) || !aligned16(dst))
-    return MVIT_EINVAL;
-  SlopeArgs a = {};
-  a.dy = src, a.dzt = (bf16_t*)dst, a.ld = ld, a.ld_dzt = ld_dst, a.M = R, a.N = Cc, a.rows = run_rows(R, Cc), a.act = MVIT_ACT_NONE;
-  launch_tiles<false>(a, dim3((Cc + 63) / 64, run_count(R, Cc)), (hipStream_t)stream);
-  return MVIT_LAUNCH_CHECK();
-}
-
 extern "C" MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N) { return M <= 0 || N <= 0 ? 0 : (long long)run_count(M, N) * N * 4; }
 
-extern "C" MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dzt, long long ld_dzt,
-                                     void* dbias, int dbias_f32, void* scratch, int M, int N, mvit_stream_t stream) {
+extern "C" MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dbias, int dbias_f32,
+                                     void* scratch, int M, int N, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
   if (M < 0 || M > MAX_M || N <= 0 || N > MAX_N || (M > 0 && !dy) || act < MVIT_ACT_NONE || act > MVIT_ACT_GELU_TANH || (act != MVIT_ACT_NONE && M > 0 && !pre)) return MVIT_EINVAL;
   if (dbias && M > 0 && !scratch) return MVIT_EINVAL;
-  if ((dz && (ld_dz < N || ld_dz % 8 || !aligned16(dz))) || (dzt && (!dz || ld_dzt < M || ld_dzt >= M + 8 || ld_dzt % 8 || !aligned16(dzt))))
-    return MVIT_EINVAL;
+  if (dz && (ld_dz < N || ld_dz % 8 || !aligned16(dz))) return MVIT_EINVAL;
   hipStream_t s = (hipStream_t)stream;
   const int runs = run_count(M, N);
   if (M > 0) {
-    const SlopeArgs a = {dy, (const bf16_t*)pre, (bf16_t*)dz, (bf16_t*)dzt, dbias ? (float*)scratch : nullptr, N, ld_dz, ld_dzt, M, N, run_rows(M, N), act};
+    const SlopeArgs a = {dy, (const bf16_t*)pre, (bf16_t*)dz, dbias ? (float*)scratch : nullptr, ld_dz, M, N, run_rows(M, N), act};
     if (N % 8 == 0 && aligned16(dy) && aligned16(pre)) {
-      const dim3 grid((N + 63) / 64, runs);
-      dy_f32 ? launch_tiles<true>(a, grid, s) : launch_tiles<false>(a, grid, s);
+      const dim3 grid((N + 255) / 256, runs);
+      dy_f32 ? launch_rows_bwd<true>(a, grid, s) : launch_rows_bwd<false>(a, grid, s);
     } else {
       const dim3 grid((unsigned)(((dz ? ld_dz : N) + 255) / 256), runs);
       if (dy_f32)
         hipLaunchKernelGGL((act_bwd_elements<true>), grid, dim3(256), 0, s, a);
       else
         hipLaunchKernelGGL((act_bwd_elements<false>), grid, dim3(256), 0, s, a);
-      if (const int rc = MVIT_LAUNCH_CHECK()) return rc;
-      if (dzt)
-        if (const int rc = mvit_transpose_padded(dz, ld_dz, dzt, ld_dzt, M, N, stream)) return rc;
     }
     if (const int rc = MVIT_LAUNCH_CHECK()) return rc;
   }

@@ -19,9 +19,14 @@ namespace mvit_linear {
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef __attribute__((ext_vector_type(4))) short i16x4;
 typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef __attribute__((address_space(3))) i16x4* lds_4x16;
 
-enum Mode { H16, F8, F8X };   // 16-bit operands; e4m3 on the e4m3 instructions; e4m3 widened to 16 bits
+// 16-bit operands; e4m3 on the e4m3 instructions; e4m3 widened to 16 bits; and the gradients' products, whose K axis goes along the rows of
+// memory of an operand: dx = dz W (DX: W [K, N] as it lies) and dW = dz^T x (DW: dz [K, M] and x [K, N])
+enum Mode { H16, F8, F8X, DX, DW };
 
 struct Args {
   const char *x, *w;
@@ -33,6 +38,9 @@ struct Args {
   int M, N, kb;      // kb: bytes of a row of x and W
   int act, bias_f32;
   float act_lo;   // -inf, or 0 for relu
+  // DX, DW: rows of the operands whose rows are K; K tiles of a split and splits; their products f32 [splits][M][N] where there is more than one
+  int krows, kper, splits;
+  float* part;
 };
 
 // What a tile kernel is compiled for besides its operands.  The epilogue is unrolled over the accumulators: with every activation and
@@ -188,7 +196,31 @@ __device__ __forceinline__ void widen(const i32x4& v, bf16x8 (&out)[2]) {
 //    a fragment is free, and is chosen so that a lane's groups make up whole pieces of 16 bytes and the lanes of a row 64 bytes in a
 //    line: y leaves from the registers.  (Through panels in LDS, whole lines a store, the epilogue took 6 to 8 us of a 256 x 256 tile:
 //    a chain of LDS writes, reads and waits with two waves a SIMD to hide it.)
+//  * An operand whose rows are K (DX, DW) lies in LDS as it does in memory, 64 rows of the tile's columns, and is turned by the transposing
+//    LDS reads (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 columns, a lane gets the 4 values of its column), two for a fragment.
+//    (With transposed copies of x, W and dz in memory forward and
+//    backward of [5264, 1536] x [4096, 1536], gelu, took 266 us instead of 231.)
 constexpr int BKB = 128;
+
+// Layout of 64 rows of BN columns: the 16-byte piece c of row k at place c ^ fold(k).  What 32 lanes read at once -- 32 bytes each of rows
+// k .. k + 3 and k + 8 .. k + 11 -- falls on all 64 banks once (rows of 128 bytes: two rows span them, so two bits of k are enough).
+template <int COLS>
+struct KRows {
+  static constexpr int RL = COLS * 2, PER_DMA = 1024 / RL;   // bytes of a row, rows of a wave's DMA instruction
+  static constexpr bool ok(int waves) { return (RL & (RL - 1)) == 0 && RL >= 128 && RL <= 512 && waves * PER_DMA % 16 == 0; }
+  static __device__ __forceinline__ int fold(int k) { return RL == 128 ? (k & 2) | ((k >> 1) & 4) : (k & 3) << 1 | (k & 8); }
+  // (__restrict: nothing else writes here in this function's scope.  DMA into LDS is waited for by hand, a stage at a time; without the word
+  // the compiler waits for all that is in flight in front of every one of these reads, as it does not for ordinary ones.)
+  static __device__ __forceinline__ i32x2 turned(lds_4x16 __restrict p) { return __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p)); }
+  // 16 columns from `col` on (a multiple of 16), 32 rows from 32 s on: lane l gets column l % 16, rows 8 (l / 16) .. + 7
+  static __device__ __forceinline__ i32x4 read(char* base, int col, int s) {
+    const int lane = threadIdx.x & 63, i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
+    const int at = k * RL + ((((i & 3) >> 1) ^ fold(k)) << 4) + (i & 1) * 8;
+    char* p = base + s * 32 * RL + (at ^ (col * 2));
+    const i32x2 a = turned((lds_4x16)p), b = turned((lds_4x16)(p + 4 * RL));
+    return (i32x4){a.x, a.y, b.x, b.y};
+  }
+};
 
 template <int MODE, int BM, int BN, int WM, int WN, int NST>
 struct Tile {
@@ -199,6 +231,7 @@ struct Tile {
   static constexpr int PIECES = BKB / 16;
   static constexpr int ROWS_PER_DMA = 1024 / BKB;       // rows of one wave's DMA instruction
   static constexpr int A_DMA = BM / ROWS_PER_DMA / NW, B_DMA = BN / ROWS_PER_DMA / NW, LPT = A_DMA + B_DMA;
+  static constexpr bool XR = MODE == DW, WR = MODE == DX || MODE == DW;   // K along the rows of x, of W
   static constexpr int STAGE = (BM + BN) * BKB;
   static constexpr int TABLE = MODE == F8 ? 2 * WTN : 0;   // floats of a wave's table of column constants
   static constexpr size_t LDS = (size_t)NST * STAGE + (size_t)NW * TABLE * 4;
@@ -206,12 +239,13 @@ struct Tile {
   static_assert(A_DMA >= 1 && B_DMA >= 1 && TM >= 1 && TN >= 1 && WTN <= 64, "sizes of a wave");
   static_assert(NW * ROWS_PER_DMA % 32 == 0, "LDS places repeat every 32 rows");
   static_assert(LDS <= 160 * 1024, "LDS of a CU");
+  static_assert(!WR || (TN % 2 == 0 && KRows<BN>::ok(NW) && (!XR || KRows<BM>::ok(NW))), "K along the rows");
 };
 
 template <int MODE, class E, int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   using T = Tile<MODE, BM, BN, WM, WN, NST>;
-  constexpr bool OP8 = MODE != H16, WIDE = MODE == F8;   // WIDE: 32 x 32 instructions
+  constexpr bool OP8 = MODE == F8 || MODE == F8X, WIDE = MODE == F8;   // WIDE: 32 x 32 instructions
   using frag = std::conditional_t<WIDE, i32x8, i32x4>;
   using acc_t = std::conditional_t<WIDE, f32x16, f32x4>;
   constexpr int AR = WIDE ? 16 : 4, NR = T::TM + T::TN;
@@ -221,10 +255,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   const int wm = wave / WN, wn = wave % WN;
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, nt = tm * tn;
   const int nk = (p.kb + BKB - 1) / BKB;
+  // DX, DW: number v is split v / nt of tile v % nt; the K tiles [first, end) of a number
+  const int nv = T::WR ? nt * p.splits : nt;
+  auto first_k = [&](int v) __attribute__((always_inline)) { return T::WR ? v / nt * p.kper : 0; };
+  auto end_k = [&](int v) __attribute__((always_inline)) { return T::WR ? min(nk, (v / nt + 1) * p.kper) : nk; };
 
   // tile number -> place: blocks go to the eight XCDs in turn, so the numbers of one XCD are put on one contiguous run of tiles, and runs
   // go down 8 rows of tiles before the next column: the blocks that share an L2 share rows of x and of W
   auto place = [&](int v, int& m0, int& n0) __attribute__((always_inline)) {
+    if constexpr (T::WR) v %= nt;
     const int q = nt >> 3, r = nt & 7, xcd = v & 7;
     const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (v >> 3);
     const int per = 8 * tn, g0 = id / per * 8, gsz = min(tm - g0, 8), in = id % per;
@@ -240,28 +279,43 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   // ---- the DMA side: output tile `dv`, K tile `dk` of it come next
   const int dr = lane / T::PIECES;   // this lane's part of a wave's DMA instruction: one 16-byte piece of row `dr`
   const int drow = wave * T::ROWS_PER_DMA + dr;   // (further instructions of the wave are a multiple of 32 rows on: the same places)
-  const int x_piece = (lane % T::PIECES ^ x_place(drow)) * 16, w_piece = (lane % T::PIECES ^ w_place(drow)) * 16;
+  // (K along the rows: this lane's row kx, kw of the tile's 64 and its piece of it, for every instruction the next `step` rows)
+  constexpr int XL = KRows<BM>::RL, WL = KRows<BN>::RL, x_step = T::NW * 1024 / XL, w_step = T::NW * 1024 / WL;
+  const int kx = wave * (1024 / XL) + lane / (XL / 16), kw = wave * (1024 / WL) + lane / (WL / 16);
+  const int x_piece = (T::XR ? lane % (XL / 16) ^ KRows<BM>::fold(kx) : lane % T::PIECES ^ x_place(drow)) * 16;
+  const int w_piece = (T::WR ? lane % (WL / 16) ^ KRows<BN>::fold(kw) : lane % T::PIECES ^ w_place(drow)) * 16;
   __amdgpu_buffer_rsrc_t rx, rw;
   unsigned off[T::LPT];
-  int dv = blockIdx.x, dk = 0;
+  int dv = blockIdx.x, dk = 0, dk_end = 0;
+  const char *bx = p.x, *bw = p.w;   // where the K tile's rows begin (K along the rows)
   auto aim = [&](auto) __attribute__((always_inline)) {
     int m0 = 0, n0 = 0;
-    const bool any = dv < nt;
-    if (any) place(dv, m0, n0);
-    rx = make_rsrc(p.x + (size_t)m0 * p.ldx), rw = make_rsrc(p.w + (size_t)n0 * p.ldw);
+    const bool any = dv < nv;
+    dk = 0, dk_end = nk;
+    if (any) place(dv, m0, n0), dk = first_k(dv), dk_end = end_k(dv);
+    bx = p.x + (T::XR ? (size_t)m0 * 2 + (size_t)p.ldx * (BKB / 2) * dk : (size_t)m0 * p.ldx);
+    bw = p.w + (T::WR ? (size_t)n0 * 2 + (size_t)p.ldw * (BKB / 2) * dk : (size_t)n0 * p.ldw);
+    rx = make_rsrc(bx), rw = make_rsrc(bw);
 #pragma unroll
     for (int j = 0; j < T::LPT; ++j) {
       const bool a = j < T::A_DMA;
       const int row = ((a ? j : j - T::A_DMA) * T::NW + wave) * T::ROWS_PER_DMA + dr;
-      const bool in = any && (a ? m0 + row < p.M : n0 + row < p.N);
-      off[j] = in ? (unsigned)row * (a ? p.ldx : p.ldw) + (unsigned)(a ? x_piece : w_piece) : OOB;
+      if (a ? T::XR : T::WR) {
+        const bool in = any && (a ? m0 + x_piece / 2 < p.M : n0 + w_piece / 2 < p.N);
+        off[j] = in ? (unsigned)(a ? kx + j * x_step : kw + (j - T::A_DMA) * w_step) * (a ? p.ldx : p.ldw) + (unsigned)(a ? x_piece : w_piece) : OOB;
+      } else {
+        const bool in = any && (a ? m0 + row < p.M : n0 + row < p.N);
+        off[j] = in ? (unsigned)row * (a ? p.ldx : p.ldw) + (unsigned)(a ? x_piece : w_piece) : OOB;
+      }
     }
   };
   auto issue = [&](int stage, int j, auto) __attribute__((always_inline)) {   // piece j of the next K tile; beyond K or M, N: zeros
     const bool a = j < T::A_DMA;
     char* to = smem + stage * T::STAGE + (a ? 0 : BM * BKB) + ((a ? j : j - T::A_DMA) * T::NW + wave) * 1024;
-    const int k = dk * BKB;
-    unsigned o = k + (a ? x_piece : w_piece) < p.kb ? off[j] : OOB;
+    const bool rows = a ? T::XR : T::WR;
+    const int k = rows ? 0 : dk * BKB;
+    const bool in = rows ? (a ? kx + j * x_step : kw + (j - T::A_DMA) * w_step) < p.krows - dk * (BKB / 2) : k + (a ? x_piece : w_piece) < p.kb;
+    unsigned o = in ? off[j] : OOB;
     asm volatile("" : "+v"(o));   // one unconditional instruction a piece: the waits count them
     if (a)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_ptr)to, 16, o, k, 0, 0);
@@ -269,10 +323,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_ptr)to, 16, o, k, 0, 0);
   };
   auto advance = [&]() __attribute__((always_inline)) {
-    if (++dk == nk) {
-      dk = 0;
+    if (++dk == dk_end) {
       dv += gridDim.x;
       aim(0);
+    } else {
+      if constexpr (T::XR) rx = make_rsrc(bx += (size_t)p.ldx * (BKB / 2));
+      if constexpr (T::WR) rw = make_rsrc(bw += (size_t)p.ldw * (BKB / 2));
     }
   };
 
@@ -298,11 +354,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   auto w_row_of = [&](int j) __attribute__((always_inline)) { return w_row + (PAIRED ? (j >> 1) * 32 + (j & 1) * 4 : j * T::FR); };
   // fragment r of sub-step s of a stage into set f, in the order the products take them: x 0, all of W, x 1 ...
   auto load1 = [&](int stage, int s, int f, int r) __attribute__((always_inline)) {
-    const char* st = smem + stage * T::STAGE;
-    if (r >= 1 && r <= T::TN)   // (the places of rows 32 or 4 apart agree where w_row_of() steps by them)
-      fb[f][r - 1] = read(st + BM * BKB + wn * T::WTN * BKB, w_row_of(r - 1), w_place(w_row), s);
-    else
-      fa[f][r ? r - T::TN : 0] = read(st + wm * T::WTM * BKB, fr + (r ? r - T::TN : 0) * T::FR, x_place(fr), s);
+    char* st = smem + stage * T::STAGE;
+    const int i = r ? r - T::TN : 0;
+    if (r >= 1 && r <= T::TN) {   // (the places of rows 32 or 4 apart agree where w_row_of() steps by them)
+      if constexpr (T::WR)
+        fb[f][r - 1] = KRows<BN>::read(st + BM * BKB, wn * T::WTN + (r - 1) * 16, s);
+      else
+        fb[f][r - 1] = read(st + BM * BKB + wn * T::WTN * BKB, w_row_of(r - 1), w_place(w_row), s);
+    } else {
+      if constexpr (T::XR)
+        fa[f][i] = KRows<BM>::read(st, wm * T::WTM + i * 16, s);
+      else
+        fa[f][i] = read(st + wm * T::WTM * BKB, fr + i * T::FR, x_place(fr), s);
+    }
   };
   acc_t acc[T::TM][T::TN];
   // One sub-step: the products of fragment set f, and behind each of them its share of the reads of the next set (sub-step s of a stage)
@@ -366,14 +430,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   for (int r = 0; r < NR; ++r) load1(0, 0, 0, r);
 
   int stage = 0, landed = 0;   // landed: K tiles behind the current one whose DMA has been waited for already
-  for (int v = blockIdx.x; v < nt; v += gridDim.x) {
+  for (int v = blockIdx.x; v < nv; v += gridDim.x) {
 #pragma unroll
     for (int i = 0; i < T::TM; ++i)
 #pragma unroll
       for (int j = 0; j < T::TN; ++j)
 #pragma unroll
         for (int r = 0; r < AR; ++r) acc[i][j][r] = 0.f;
-    for (int t = 0; t < nk; ++t) {
+    for (int t = first_k(v), end = end_k(v); t < end; ++t) {
       const int next = stage + 1 == NST ? 0 : stage + 1;
       sub_step(0, stage, 1, -1, std::false_type{});
       if (landed <= 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * T::LPT) : "memory");
@@ -387,69 +451,98 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
     // stores share one counter, and behind the stores it could not be told any more.
     int m0, n0;
     place(v, m0, n0);
-    constexpr int W = E::out32 ? 4 : 8, NP = T::TN * AR / W;   // pieces of a lane in one row of fragments
-    const int row0 = m0 + wm * T::WTM + fr, col0 = n0 + wn * T::WTN;
-    auto col_of = [&](int q) __attribute__((always_inline)) {
-      return col0 + (PAIRED ? q * 32 + fh * 8 : WIDE ? (q >> 1) * 32 + (q & 1) * 16 + fh * 8 : q * 16 + fh * 4);
-    };
-    // column constants: in registers, or (F8: 64 of them, beside 128 accumulators) in a table of the wave's own
-    Columns<OP8, W> cols[NP];
-    float rs[T::TM];
-    float* table = (float*)(smem + NST * T::STAGE) + wave * T::TABLE;
-    if constexpr (WIDE) {
-      const int c = min(col0 + lane, p.N - 1);
-      if (lane < T::WTN) {
-        table[lane] = p.ws[c];
-        table[T::WTN + lane] = p.bias ? value_of(p.bias, c, p.bias_f32) : 0.f;
+    if constexpr (T::WR) {
+      // nothing to add: y's 16 bits as they are.  A lane has 4 columns of two neighbouring fragments; traded with the next 16 lanes they make 8
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      landed = NST - 1;
+      if (p.splits > 1) {
+        float* part = p.part + (size_t)(v / nt) * p.M * p.N;
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+          const int row = m0 + wm * T::WTM + i * 16 + fr;
+#pragma unroll
+          for (int j = 0; j < T::TN; ++j) {
+            const int col = n0 + wn * T::WTN + j * 16 + fh * 4;
+            if (row < p.M && col < p.N) *(f32x4*)(part + (size_t)row * p.N + col) = acc[i][j];
+          }
+        }
+      } else
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < T::TN; j += 2) {
+          const acc_t &c0 = acc[i][j], &c1 = acc[i][j + 1];
+          const auto lo = __builtin_amdgcn_permlane16_swap(pack2bf(c0[0], c0[1]), pack2bf(c1[0], c1[1]), false, false);
+          const auto hi = __builtin_amdgcn_permlane16_swap(pack2bf(c0[2], c0[3]), pack2bf(c1[2], c1[3]), false, false);
+          store_piece<E>(p, m0 + wm * T::WTM + i * 16 + fr, n0 + wn * T::WTN + (j + (fh & 1)) * 16 + (fh >> 1) * 8, make_uint4(lo[0], hi[0], lo[1], hi[1]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-#pragma unroll
-      for (int q = 0; q < NP; ++q) cols[q].load(p, col_of(q));
-    }
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) rs[i] = OP8 ? p.xs[min(row0 + i * T::FR, p.M - 1)] : 1.f;
-    uint4 res[2][NP];   // of this row of fragments and the next
-#pragma unroll
-    for (int q = 0; q < NP; ++q) res[0][q] = residual_piece<E>(p, row0, col_of(q));
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    landed = NST - 1;
-#pragma unroll
-    for (int i = 0; i < T::TM; ++i) {
-      const int row = row0 + i * T::FR;
-      if (i + 1 < T::TM)
-#pragma unroll
-        for (int q = 0; q < NP; ++q) res[(i + 1) & 1][q] = residual_piece<E>(p, row + T::FR, col_of(q));
-      uint4 out[NP];
-#pragma unroll
-      for (int q = 0; q < NP; ++q) {
-        if constexpr (WIDE) {
-          const float* t = table + (col_of(q) - col0);
-#pragma unroll
-          for (int e = 0; e < W; ++e) cols[q].s[e] = t[e], cols[q].b[e] = t[T::WTN + e];
+      constexpr int W = E::out32 ? 4 : 8, NP = T::TN * AR / W;   // pieces of a lane in one row of fragments
+      const int row0 = m0 + wm * T::WTM + fr, col0 = n0 + wn * T::WTN;
+      auto col_of = [&](int q) __attribute__((always_inline)) {
+        return col0 + (PAIRED ? q * 32 + fh * 8 : WIDE ? (q >> 1) * 32 + (q & 1) * 16 + fh * 8 : q * 16 + fh * 4);
+      };
+      // column constants: in registers, or (F8: 64 of them, beside 128 accumulators) in a table of the wave's own
+      Columns<OP8, W> cols[NP];
+      float rs[T::TM];
+      float* table = (float*)(smem + NST * T::STAGE) + wave * T::TABLE;
+      if constexpr (WIDE) {
+        const int c = min(col0 + lane, p.N - 1);
+        if (lane < T::WTN) {
+          table[lane] = p.ws[c];
+          table[T::WTN + lane] = p.bias ? value_of(p.bias, c, p.bias_f32) : 0.f;
         }
-        float o[W];
+      } else {
 #pragma unroll
-        for (int e = 0; e < W; ++e)
-          o[e] = (WIDE ? acc[i][q >> 1][(q & 1) * 8 + e] : PAIRED ? acc[i][q * 2 + (e >> 2)][e & 3] : acc[i][q][e & 3]) * (OP8 ? rs[i] : 1.f);
-        out[q] = finish<OP8, E, W>(p, o, row, col_of(q), cols[q], res[i & 1][q]);
-        if constexpr (!WIDE) store_piece<E>(p, row, col_of(q), out[q]);
+        for (int q = 0; q < NP; ++q) cols[q].load(p, col_of(q));
       }
-      if constexpr (WIDE && E::vec) {
-        // two lanes of a row, 32 bytes a store: trade pieces between rows r and r + 16, so that four lanes have 64 bytes of one row
 #pragma unroll
-        for (int q = 0; q < NP; q += 2) {
-          uint32_t *a = (uint32_t*)&out[q], *b = (uint32_t*)&out[q + 1];
+      for (int i = 0; i < T::TM; ++i) rs[i] = OP8 ? p.xs[min(row0 + i * T::FR, p.M - 1)] : 1.f;
+      uint4 res[2][NP];   // of this row of fragments and the next
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const auto s = __builtin_amdgcn_permlane16_swap(a[e], b[e], false, false);
-            a[e] = s[0], b[e] = s[1];
+      for (int q = 0; q < NP; ++q) res[0][q] = residual_piece<E>(p, row0, col_of(q));
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      landed = NST - 1;
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i) {
+        const int row = row0 + i * T::FR;
+        if (i + 1 < T::TM)
+#pragma unroll
+          for (int q = 0; q < NP; ++q) res[(i + 1) & 1][q] = residual_piece<E>(p, row + T::FR, col_of(q));
+        uint4 out[NP];
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          if constexpr (WIDE) {
+            const float* t = table + (col_of(q) - col0);
+#pragma unroll
+            for (int e = 0; e < W; ++e) cols[q].s[e] = t[e], cols[q].b[e] = t[T::WTN + e];
           }
-          const int r = row - fr + (lane & 15), c = col0 + (q >> 1) * 32 + ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;
-          store_piece<E>(p, r, c, out[q]);
-          store_piece<E>(p, r + 16, c, out[q + 1]);
+          float o[W];
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+            o[e] = (WIDE ? acc[i][q >> 1][(q & 1) * 8 + e] : PAIRED ? acc[i][q * 2 + (e >> 2)][e & 3] : acc[i][q][e & 3]) * (OP8 ? rs[i] : 1.f);
+          out[q] = finish<OP8, E, W>(p, o, row, col_of(q), cols[q], res[i & 1][q]);
+          if constexpr (!WIDE) store_piece<E>(p, row, col_of(q), out[q]);
         }
+        if constexpr (WIDE && E::vec) {
+          // two lanes of a row, 32 bytes a store: trade pieces between rows r and r + 16, so that four lanes have 64 bytes of one row
+#pragma unroll
+          for (int q = 0; q < NP; q += 2) {
+            uint32_t *a = (uint32_t*)&out[q], *b = (uint32_t*)&out[q + 1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const auto s = __builtin_amdgcn_permlane16_swap(a[e], b[e], false, false);
+              a[e] = s[0], b[e] = s[1];
+            }
+            const int r = row - fr + (lane & 15), c = col0 + (q >> 1) * 32 + ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;
+            store_piece<E>(p, r, c, out[q]);
+            store_piece<E>(p, r + 16, c, out[q + 1]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);   // (rows of fragments pulled together cost registers that are not there)
       }
-      __builtin_amdgcn_sched_barrier(0);   // (rows of fragments pulled together cost registers that are not there)
     }
     // the next tile's first fragments again: read once more, they need no registers during the epilogue
 #pragma unroll

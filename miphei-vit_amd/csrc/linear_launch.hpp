@@ -8,7 +8,7 @@ namespace mvit_linear {
 template <int MODE, class E, int BM, int BN, int WM, int WN, int NST>
 int launch_tile(const Args& a, hipStream_t s) {
   using T = Tile<MODE, BM, BN, WM, WN, NST>;
-  const long long nt = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  const long long nt = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN) * (T::WR ? a.splits : 1);
   if (nt > 0x7fffffff) return MVIT_EINVAL;
   static mvit_per_device_size raised;
   const auto fn = linear_tile<MODE, E, BM, BN, WM, WN, NST>;
@@ -31,7 +31,7 @@ int launch_rows(const Args& a, hipStream_t s) {
 //   [5264, 1536] x [4096, 1536]   72  63  72  76 113      [5264, 4096] x [1536, 4096]   78  68  58  60 104
 //   [5264, 1536] x [8192, 1536]  115 125 140              [21056, 1536] x [1536, 1536]  88 102  99 109 174
 //   [1301, 1536] x [4608, 1536]   36      24  25  34      [700, 1536] x [4096, 1536]            22  20  20
-//   [4096, 5264] x [1536, 5264]  117 109  74  80          [329, 1536] x [4608, 1536]    34      22  20  13
+//   [329, 1536] x [4608, 1536]    34      22  20  13
 template <int MODE, class E>
 int by_size(const Args& a, hipStream_t s) {
   using Any = End<E::out32, A_ANY, E::vec>;   // (the row kernels' epilogue is not unrolled)
@@ -56,6 +56,22 @@ int by_size(const Args& a, hipStream_t s) {
     case 2:
       return launch_tile<MODE, E, 128, 256, 2, 4, 3>(a, s);
     case 3:
+      return launch_tile<MODE, E, 128, 128, 2, 2, 2>(a, s);
+    default:
+      return launch_tile<MODE, E, 64, 64, 2, 2, 4>(a, s);
+  }
+}
+
+// The gradients' products: one of four tiles (plan_grad in linear.hip)
+template <int MODE>
+int dispatch_grad(const Args& a, int tile, hipStream_t s) {
+  using E = End<false, A_CLIP, true>;
+  switch (tile) {
+    case 0:
+      return launch_tile<MODE, E, 256, 256, 2, 4, 2>(a, s);
+    case 1:
+      return launch_tile<MODE, E, 128, 256, 2, 4, 3>(a, s);
+    case 2:
       return launch_tile<MODE, E, 128, 128, 2, 2, 2>(a, s);
     default:
       return launch_tile<MODE, E, 64, 64, 2, 2, 4>(a, s);

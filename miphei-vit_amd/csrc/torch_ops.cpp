@@ -45,7 +45,8 @@ struct Lib {
   MVIT_FN(mvit_linear_fp8);
   MVIT_FN(mvit_act_bwd_scratch_bytes);
   MVIT_FN(mvit_act_bwd);
-  MVIT_FN(mvit_transpose_padded);
+  MVIT_FN(mvit_linear_grad_scratch_bytes);
+  MVIT_FN(mvit_linear_grad);
 #undef MVIT_FN
 };
 std::array<Lib, 2> libs;   // [0] bf16, [1] fp16: filled by mvit_torch_bind before the first call
@@ -429,12 +430,13 @@ std::tuple<Tensor, Tensor> linear_act_forward_meta(const Tensor& x, const Tensor
 }
 
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
-// t^T with its rows padded by zeros to whole 16-byte pieces: an operand whose K axis is t's rows
-Tensor transposed(const Lib& l, const Tensor& t, void* st) {
-  Tensor out = at::empty({t.size(1), up8(t.size(0))}, t.options());
-  ok(l.mvit_transpose_padded(t.const_data_ptr(), ld(t), out.mutable_data_ptr(), out.size(1), (int)t.size(0), (int)t.size(1), st),
-     "mvit_transpose_padded");
-  return out;
+// y[M, N] = x W (x [M, K]) or x^T W (x [K, M]) with W [K, N]
+void grad_product(const Lib& l, const Tensor& x, bool x_rows, const Tensor& w, const Tensor& y, int64_t M, int64_t N, int64_t K, void* st) {
+  mvit_linear_args a = {};
+  a.x = x.const_data_ptr(), a.w = w.const_data_ptr(), a.y = y.mutable_data_ptr(), a.ldx = ld(x), a.ldw = ld(w), a.M = (int)M, a.N = (int)N, a.K = (int)K;
+  const long long bytes = l.mvit_linear_grad_scratch_bytes(a.M, a.N, a.K);
+  const Tensor s = bytes ? scratch(y, bytes) : Tensor();
+  ok(l.mvit_linear_grad(&a, x_rows, bytes ? s.mutable_data_ptr() : nullptr, bytes, st), "mvit_linear_grad");
 }
 
 std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& pre, c10::string_view act,
@@ -447,33 +449,27 @@ std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const T
   c10::DeviceGuard guard(x.device());
   const ScalarType t = x.scalar_type();
   const int64_t N = weight.size(0), K = weight.size(1), M = x.numel() / K;
-  REQUIRE(!need_w || M <= (1 << 22), "linear_act_backward", "more than 2^22 rows of x with a gradient of weight");
+  REQUIRE(!need_w || M <= (1 << 29), "linear_act_backward", "more than 2^29 rows of x with a gradient of weight");
   Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : none(x, t);
   Tensor dw = need_w ? at::empty({N, K}, x.options()) : none(x, t);
   Tensor db = need_b ? at::empty({N}, x.options().dtype(bias_dtype)) : none(x, bias_dtype);
   if (M == 0) return {dx, dw.zero_(), db.zero_()};
   const Lib& l = lib(t == at::kHalf);
   void* st = stream(x);
-  Tensor dz = dy.reshape({M, N}).contiguous(), dzt;
+  Tensor dz = dy.reshape({M, N}).contiguous();
   const Tensor dy2 = dz;
   // dz is dy itself where there is nothing to multiply, to round or to pad
   const bool make = (need_x || need_w) && (code != MVIT_ACT_NONE || dy2.scalar_type() != t || N % 8);
   if (make) dz = at::empty({M, up8(N)}, x.options());
-  if (need_w && (make || need_b)) dzt = at::empty({N, up8(M)}, x.options());
   if (make || need_b) {
     const Tensor s = scratch(x, need_b ? l.mvit_act_bwd_scratch_bytes((int)M, (int)N) : 0);
-    if (dzt.defined() && !make) dz = at::empty({M, N}, x.options());   // (the transposed copy comes with the rows)
-    const bool rows = make || dzt.defined();
-    ok(l.mvit_act_bwd(dy2.const_data_ptr(), f32(dy2), code == MVIT_ACT_NONE ? nullptr : pre.const_data_ptr(), code,
-                      rows ? dz.mutable_data_ptr() : nullptr, rows ? dz.size(1) : 0, dzt.defined() ? dzt.mutable_data_ptr() : nullptr, up8(M),
-                      need_b ? db.mutable_data_ptr() : nullptr, f32(db), need_b ? s.mutable_data_ptr() : nullptr, (int)M, (int)N, st),
+    ok(l.mvit_act_bwd(dy2.const_data_ptr(), f32(dy2), code == MVIT_ACT_NONE ? nullptr : pre.const_data_ptr(), code, make ? dz.mutable_data_ptr() : nullptr,
+                      make ? dz.size(1) : 0, need_b ? db.mutable_data_ptr() : nullptr, f32(db), need_b ? s.mutable_data_ptr() : nullptr, (int)M, (int)N, st),
        "mvit_act_bwd");
   }
-  if (need_x)     // dx = dz W: its K axis is N
-    product(l, operand(dz), transposed(l, operand(weight), st), std::nullopt, std::nullopt, dx, nullptr, MVIT_ACT_NONE, nullptr, nullptr, M, K, st);
-  if (need_w)     // dW = dz^T x: its K axis is M
-    product(l, dzt.defined() ? dzt : transposed(l, operand(dz), st), transposed(l, operand(x), st), std::nullopt, std::nullopt, dw, nullptr,
-            MVIT_ACT_NONE, nullptr, nullptr, N, K, st);
+  dz = operand(dz);
+  if (need_x) grad_product(l, dz, false, operand(weight), dx, M, K, N, st);
+  if (need_w) grad_product(l, dz, true, operand(x), dw, N, K, M, st);
   return {dx, dw, db};
 }
 std::tuple<Tensor, Tensor, Tensor> linear_act_backward_meta(const Tensor&, const Tensor& x, const Tensor& weight, const Tensor&, c10::string_view,
@@ -633,7 +629,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                                std::string act) {
     // (the K axis of dW = dz^T x)
-    REQUIRE(!weight.requires_grad() || x.sym_numel() <= weight.sym_size(1) * (1 << 22), "linear_act", "more than 2^22 rows of x with a gradient of weight");
+    REQUIRE(!weight.requires_grad() || x.sym_numel() <= weight.sym_size(1) * (1 << 29), "linear_act", "more than 2^29 rows of x with a gradient of weight");
     at::AutoDispatchBelowAutograd below;
     const bool keep = act != "none" && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
     auto [y, pre] = linear_forward_op().call(x, weight, bias, residual, act, keep);
@@ -711,7 +707,8 @@ extern "C" __attribute__((visibility("default"))) const char* mvit_torch_bind(co
     MVIT_FN(mvit_linear_fp8);
     MVIT_FN(mvit_act_bwd_scratch_bytes);
     MVIT_FN(mvit_act_bwd);
-    MVIT_FN(mvit_transpose_padded);
+    MVIT_FN(mvit_linear_grad_scratch_bytes);
+    MVIT_FN(mvit_linear_grad);
 #undef MVIT_FN
   }
   libs = got;

@@ -204,10 +204,17 @@ def test_c_entries_refuse_what_they_cannot_do():
                                                   dict(act=-1), dict(x=p + 8), dict(w=p + 2), dict(y=None), dict(res=p, ldr=3), dict(ldx=1 << 24)))
         assert lin(fn, M=0) == 0
     assert lin(lib.mvit_linear_fp8, pre=p) == lin(lib.mvit_linear_fp8, x_scale=None) == -1
-    act = lambda pre=p, dz=p, ldz=8, dzt=None, ldzt=8, db=None, s=None: lib.mvit_act_bwd(p, 0, pre, 3, dz, ldz, dzt, ldzt, db, 0, s, 4, 8, None)  # noqa: E731
-    assert act(pre=None) == act(db=p) == act(ldz=4) == act(ldz=12) == act(dz=p + 2) == act(dz=None, dzt=p) == act(dzt=p, ldzt=16) == -1
-    assert lib.mvit_transpose_padded(p, 8, p, 16, 4, 8, None) == lib.mvit_transpose_padded(p, 8, p, 8, 4, 9, None) == -1
-    assert lib.mvit_transpose_padded(p + 2, 8, p, 8, 4, 8, None) == lib.mvit_transpose_padded(p, 12, p, 8, 4, 8, None) == -1
+    act = lambda pre=p, dz=p, ldz=8, db=None, s=None: lib.mvit_act_bwd(p, 0, pre, 3, dz, ldz, db, 0, s, 4, 8, None)  # noqa: E731
+    assert act(pre=None) == act(db=p) == act(ldz=4) == act(ldz=12) == act(dz=p + 2) == -1
+    a = L.LinearArgs(x=p, w=p, y=p, ldx=16, ldw=16, M=4, N=16, K=16)
+    for rows in (0, 1):
+        grad = lambda **kw: lin(lambda b, s: lib.mvit_linear_grad(b, rows, p, 1 << 40, s), **kw)  # noqa: E731
+        assert all(grad(**kw) == -1 for kw in (dict(M=0), dict(N=0), dict(N=12), dict(K=0), dict(ldx=12), dict(ldw=8), dict(ldw=20), dict(x=p + 8), dict(w=p + 2),
+                                               dict(y=p + 4), dict(y=None), dict(bias=p), dict(res=p), dict(pre=p), dict(act=1), dict(y_f32=1), dict(ldw=1 << 23)))
+        assert grad(ldx=8) == -1 or rows
+    assert lib.mvit_linear_grad(C.byref(L.LinearArgs(x=p, w=p, y=p, ldx=8, ldw=16, M=9, N=16, K=4)), 1, None, 0, None) == -1      # 9 columns in rows of 8
+    assert lib.mvit_linear_grad_scratch_bytes(64, 512, 20816) > 0 == lib.mvit_linear_grad_scratch_bytes(4, 8, 64)
+    assert lib.mvit_linear_grad(C.byref(L.LinearArgs(x=p, w=p, y=p, ldx=64, ldw=512, M=64, N=512, K=20816)), 1, p, 64, None) == -1
 
 
 def test_frequencies_and_grid():
@@ -1090,6 +1097,9 @@ def test_rows_far_apart():
         if es == 2:
             big[:, -64:] = x
             assert torch.equal(ops.linear_act(big[:, -64:], w), ops.linear_act(x, w))
+            dy, w = randn(g, M, N, dtype=torch.bfloat16), w.requires_grad_()
+            assert torch.equal(torch.autograd.grad(ops.linear_act(big[:, -64:], w), w, dy)[0], torch.autograd.grad(ops.linear_act(x, w), w, dy)[0])
+            w = w.detach()
         else:
             (q, s), (wq, ws) = ops.quantize_fp8(x), ops.quantize_fp8(w)
             big.view(torch.uint8)[:, -64:] = q.view(torch.uint8)
@@ -1137,3 +1147,20 @@ def test_long_offsets():
         # of z times silu'' <= 2^-7 * 0.31 times |dy| <= 5, times |x| or |w| <= 5: 0.06; and a unit of the result's own rounding
         assert ((u.float() - v.float()).abs() <= 2.0 ** -7 * v.float().abs() + 0.06).all()
     assert not got[0][:8].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,K,N", [(20816, 512, 64), (20815, 64, 60), (33, 1536, 4096), (1, 1536, 4096), (5264, 1536, 1536), (700, 512, 4100), (200, 72, 2568)])
+def test_linear_act_gradients_of_few_tiles(M, K, N, dtype):
+    """products whose K axis is taken in parts: all rows of a small weight, all columns of few rows; the same every time"""
+    ops, g = T(), gen(M + K + N)
+    x, w = randn(g, M, K, dtype=dtype).requires_grad_(), randn(g, N, K, dtype=dtype, scale=K ** -0.5).requires_grad_()
+    dy = randn(g, M, N, dtype=dtype)
+    y = ops.linear_act(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    d, xd, wd = dy.double(), x.detach().double(), w.detach().double()
+    close(dx, d @ wd, d.abs() @ wd.abs(), "dx")
+    close(dw, d.t() @ xd, d.abs().t() @ xd.abs(), "dw")
+    again = torch.autograd.grad(y, (x, w), dy)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
