@@ -9,6 +9,7 @@
 // captured graph owns its own.  Wrong arguments raise ValueError in the GPU and in the meta (shape) implementation alike.
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
@@ -113,8 +114,6 @@ Tensor operand(const Tensor& t) {
 const void* ptr(const OptTensor& t) { return t ? t->const_data_ptr() : nullptr; }
 int f32(const OptTensor& t) { return t && t->scalar_type() == at::kFloat; }
 void* stream(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
-Tensor scratch(const Tensor& x, int64_t bytes) { return at::empty({bytes}, x.options().dtype(at::kByte)); }
-Tensor none(const Tensor& x, ScalarType t) { return at::empty({0}, x.options().dtype(t)); }
 
 // Checks and output shapes take sizes as SymInt (plain integers but while a graph is traced with sizes that vary): a model compiled once runs
 // at other batch sizes
@@ -124,7 +123,13 @@ Sizes with_last(const Tensor& x, const c10::SymInt& n) {
   s.back() = n;
   return s;
 }
-Tensor empty(c10::SymIntArrayRef sizes, const Tensor& like, ScalarType t) { return at::empty_symint(sizes, like.options().dtype(t)); }
+// (straight to the allocator on the GPU: through the dispatcher each output costs a call on one token 0.2 us more of 5 to 6)
+Tensor empty(c10::SymIntArrayRef sizes, const Tensor& like, ScalarType t) {
+  if (like.device().is_cuda()) return at::detail::empty_cuda(C10_AS_INTARRAYREF_SLOW(sizes), like.options().dtype(t));
+  return at::empty_symint(sizes, like.options().dtype(t));
+}
+Tensor scratch(const Tensor& x, int64_t bytes) { return empty({bytes}, x, at::kByte); }
+Tensor none(const Tensor& x, ScalarType t) { return empty({0}, x, t); }
 
 // ================================================================ RMS norm
 void rows_check(const char* op, const Tensor& x) {
@@ -183,7 +188,7 @@ struct NormBwd {
 NormBwd norm_bwd_out(const Tensor& h, const Tensor& weight, ScalarType x_dtype, bool need_x, bool need_residual, bool need_weight) {
   const bool one = x_dtype == h.scalar_type(), x = need_x || (one && need_residual), res = need_residual && !one;
   return {x ? empty(h.sym_sizes(), h, x_dtype) : none(h, x_dtype), res ? empty(h.sym_sizes(), h, h.scalar_type()) : none(h, h.scalar_type()),
-          need_weight ? at::empty_like(weight, at::MemoryFormat::Contiguous) : none(weight, weight.scalar_type()), x, res};
+          need_weight ? empty(weight.sym_sizes(), weight, weight.scalar_type()) : none(weight, weight.scalar_type()), x, res};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_norm_backward(const Tensor& dy, const OptTensor& dh, const Tensor& h, const Tensor& weight, const Tensor& rstd,
                                                      ScalarType x_dtype, bool need_x, bool need_residual, bool need_weight) {
@@ -288,6 +293,7 @@ HalfType rotary_check(const char* op, const Tensor& x, const Tensor& positions, 
 
 // y of rotary: x's own layout where that is a layout with dense heads (the order of overlapping windows is not), else contiguous
 Tensor rotary_out(const Tensor& x) {
+  if (x.is_contiguous()) return empty(x.sym_sizes(), x, x.scalar_type());
   Tensor y = at::empty_like(x);
   return y.sym_stride(3) == 1 ? y : empty(x.sym_sizes(), x, x.scalar_type());
 }
@@ -414,7 +420,7 @@ std::tuple<Tensor, Tensor> linear_act_forward(const Tensor& x, const Tensor& wei
   const HalfType h = linear_half("linear_act", x, weight, bias, residual);
   c10::DeviceGuard guard(x.device());
   Tensor y = linear_out(x, weight, residual, x.scalar_type());
-  Tensor pre = save_pre ? at::empty(y.sizes(), x.options()) : none(x, x.scalar_type());
+  Tensor pre = save_pre ? empty(y.sym_sizes(), x, x.scalar_type()) : none(x, x.scalar_type());
   if (y.numel())
     product(lib(h.f16()), operand(x), operand(weight), bias ? OptTensor(bias->contiguous()) : std::nullopt,
             residual ? OptTensor(rows(*residual)) : std::nullopt, y, save_pre ? pre.mutable_data_ptr() : nullptr, code, nullptr, nullptr,
@@ -450,9 +456,9 @@ std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const T
   const ScalarType t = x.scalar_type();
   const int64_t N = weight.size(0), K = weight.size(1), M = x.numel() / K;
   REQUIRE(!need_w || M <= (1 << 29), "linear_act_backward", "more than 2^29 rows of x with a gradient of weight");
-  Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : none(x, t);
-  Tensor dw = need_w ? at::empty({N, K}, x.options()) : none(x, t);
-  Tensor db = need_b ? at::empty({N}, x.options().dtype(bias_dtype)) : none(x, bias_dtype);
+  Tensor dx = need_x ? empty(x.sym_sizes(), x, t) : none(x, t);
+  Tensor dw = need_w ? empty({N, K}, x, t) : none(x, t);
+  Tensor db = need_b ? empty({N}, x, bias_dtype) : none(x, bias_dtype);
   if (M == 0) return {dx, dw.zero_(), db.zero_()};
   const Lib& l = lib(t == at::kHalf);
   void* st = stream(x);
@@ -460,7 +466,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_act_backward(const Tensor& dy, const T
   const Tensor dy2 = dz;
   // dz is dy itself where there is nothing to multiply, to round or to pad
   const bool make = (need_x || need_w) && (code != MVIT_ACT_NONE || dy2.scalar_type() != t || N % 8);
-  if (make) dz = at::empty({M, up8(N)}, x.options());
+  if (make) dz = empty({M, up8(N)}, x, t);
   if (make || need_b) {
     const Tensor s = scratch(x, need_b ? l.mvit_act_bwd_scratch_bytes((int)M, (int)N) : 0);
     ok(l.mvit_act_bwd(dy2.const_data_ptr(), f32(dy2), code == MVIT_ACT_NONE ? nullptr : pre.const_data_ptr(), code, make ? dz.mutable_data_ptr() : nullptr,
