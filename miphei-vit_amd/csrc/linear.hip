@@ -75,21 +75,26 @@ struct Plan {
 };
 Plan plan_grad(int M, int N, int K) {
   static constexpr int BM[4] = {256, 128, 128, 64}, BN[4] = {256, 256, 128, 64}, full[4] = {16, 10, 10, 4}, alone[4] = {16, 10, 7, 3};
-  const long long cus = mvit_num_cus(), nk = ((long long)K + 63) / 64;
-  Plan best = {0, 1, (int)nk};
+  const int cus = mvit_num_cus(), nk = (int)(((long long)K + 63) / 64);
+  Plan best = {0, 1, nk};
   double least = 1e300;
   for (int t = 0; t < 4; ++t) {
-    const long long tiles = (((long long)M + BM[t] - 1) / BM[t]) * (((long long)N + BN[t] - 1) / BN[t]), slots = t < 2 ? cus : 2 * cus;
-    for (int want = 1; want <= 64; ++want) {
-      const long long kper = (nk + want - 1) / want, s = (nk + kper - 1) / kper, n = tiles * s;
-      if (s != want || (want > 1 && kper < 4)) continue;
-      double c = (double)((n + slots - 1) / slots) * (40. + (double)(n <= cus ? alone[t] : full[t]) * kper);
-      if (s > 1) c += 50. + (double)s * M * N * 8. / 5e5;
-      if (c < least) least = c, best = {t, (int)s, (int)kper};
+    const long long tiles = (((long long)M + BM[t] - 1) / BM[t]) * ((N + BN[t] - 1) / BN[t]);
+    const int slots = t < 2 ? cus : 2 * cus;
+    // up to two rounds and a part; four K tiles a part at least
+    const int most = tiles > 2 * slots ? 1 : 1 + 2 * slots / (int)tiles;
+    for (int want = 1; want <= 64 && want <= most && (want == 1 || nk >= 4 * want); ++want) {
+      const int kper = (nk + want - 1) / want, s = want == 1 ? 1 : (nk + kper - 1) / kper;
+      const long long n = tiles * s, rounds = want == 1 ? (n + slots - 1) / slots : ((int)n + slots - 1) / slots;
+      double c = (double)rounds * (40. + (double)(n <= cus ? alone[t] : full[t]) * kper);
+      if (s > 1) c += 50. + (double)s * M * N * (8. / 5e5);
+      if (c < least) least = c, best = {t, s, kper};
     }
   }
   return best;
 }
+
+long long split_bytes(const Plan& p, int M, int N) { return p.splits > 1 ? (long long)p.splits * M * N * 4 : 0; }
 
 // 4 outputs a thread
 __global__ __launch_bounds__(256) void sum_splits(const float* part, bf16_t* y, int splits, long long n4) {
@@ -105,8 +110,7 @@ __global__ __launch_bounds__(256) void sum_splits(const float* part, bf16_t* y, 
 
 extern "C" MVIT_API long long mvit_linear_grad_scratch_bytes(int M, int N, int K) {
   if (M <= 0 || M > MAX_M || N <= 0 || N > MAX_N || K <= 0 || K > MAX_K) return 0;
-  const Plan p = plan_grad(M, N, K);
-  return p.splits > 1 ? (long long)p.splits * M * N * 4 : 0;
+  return split_bytes(plan_grad(M, N, K), M, N);
 }
 
 extern "C" MVIT_API int mvit_linear_grad(const mvit_linear_args* g, int x_rows, void* scratch, long long scratch_bytes, mvit_stream_t stream) {
@@ -119,7 +123,7 @@ extern "C" MVIT_API int mvit_linear_grad(const mvit_linear_args* g, int x_rows, 
     return MVIT_EINVAL;
   if (g->ldx < (x_rows ? (g->M + 7LL) / 8 * 8 : up8)) return MVIT_EINVAL;   // (x_rows = 0: and so K is at most 2^22)
   const Plan plan = plan_grad(g->M, g->N, g->K);
-  if (plan.splits > 1 && (!scratch || !aligned16(scratch) || scratch_bytes < mvit_linear_grad_scratch_bytes(g->M, g->N, g->K))) return MVIT_EINVAL;
+  if (plan.splits > 1 && (!scratch || !aligned16(scratch) || scratch_bytes < split_bytes(plan, g->M, g->N))) return MVIT_EINVAL;
   hipStream_t s = (hipStream_t)stream;
   const Args a = {(const char*)g->x, (const char*)g->w, nullptr, nullptr, g->y, nullptr, nullptr, nullptr, 0, (unsigned)lx, (unsigned)lw,
                   g->M, g->N, (int)(up8 * 2), MVIT_ACT_NONE, 0, -INFINITY, g->K, plan.kper, plan.splits, (float*)scratch};
