@@ -1164,3 +1164,24 @@ def test_linear_act_gradients_of_few_tiles(M, K, N, dtype):
     close(dw, d.t() @ xd, d.abs().t() @ xd.abs(), "dw")
     again = torch.autograd.grad(y, (x, w), dy)
     assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("N", [72, 75])
+def test_linear_act_gradients_of_odd_upstream_layouts(N, act):
+    """a gradient that is one value off 16 bytes, transposed, expanded or f32 gives what its dense copy gives"""
+    ops, g = T(), gen(57 + N)
+    M, K = 70, 40
+    x, w, b = randn(g, M, K, dtype=torch.bfloat16).requires_grad_(), randn(g, N, K, dtype=torch.bfloat16).requires_grad_(), randn(g, N).requires_grad_()
+    y = ops.linear_act(x, w, b, None, act)
+    dy = randn(g, M, N, dtype=torch.bfloat16)
+    want = torch.autograd.grad(y, (x, w, b), dy, retain_graph=True)
+    off = torch.zeros(M * N + 1, device="cuda", dtype=torch.bfloat16)[1:].view(M, N).copy_(dy)
+    for d in (off, dy.t().contiguous().t()):
+        for u, v in zip(torch.autograd.grad(y, (x, w, b), d, retain_graph=True), want):
+            # (db's sums go in another order where the gradient is taken by elements: 70 values of at most 5 each)
+            assert torch.equal(u, v) if u.dtype == torch.bfloat16 else ((u - v).abs() <= 70 * 5 * 70 * 2.0 ** -24).all()
+    row = dy[:1].expand(M, N)
+    for u, v in zip(torch.autograd.grad(y, (x, w, b), row, retain_graph=True), torch.autograd.grad(y, (x, w, b), row.contiguous())):
+        assert torch.equal(u, v)
