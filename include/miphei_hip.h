@@ -225,7 +225,7 @@ MVIT_API long long mvit_linear_grad_scratch_bytes(int M, int N, int K);
 MVIT_API int mvit_linear_grad(const mvit_linear_args* args, int x_rows, void* scratch, long long scratch_bytes, mvit_stream_t stream);
 /* Backward of the epilogue: dz(16-bit)[M, ld_dz] = dy * act'(pre) and dbias[N] (f32 or 16-bit) = its sum over the rows, taken before dz is
  * rounded; either may be NULL.  dy [M, N] f32 or 16-bit and pre (16-bit; may be NULL where act is none) dense; ld_dz a multiple of 8, at least N,
- * dz starts on 16 bytes; what pads a row of dz up to ld_dz where N is no multiple of 8 is zero.  scratch: mvit_act_bwd_scratch_bytes(M, N)
+ * dz starts on 16 bytes; what pads a row of dz up to the next multiple of 8 is zero.  scratch: mvit_act_bwd_scratch_bytes(M, N)
  * bytes (needed with dbias only); ordered sums, bit-identical from run to run. */
 MVIT_API long long mvit_act_bwd_scratch_bytes(int M, int N);
 MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre, int act, void* dz, long long ld_dz, void* dbias, int dbias_f32, void* scratch,

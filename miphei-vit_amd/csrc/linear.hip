@@ -140,10 +140,10 @@ extern "C" MVIT_API int mvit_linear_grad(const mvit_linear_args* g, int x_rows, 
 // runs meet in a f32 workspace (column_sums.hpp): a fixed order, no atomics.
 namespace {
 
-enum Slope { S_ONE, S_CLIP, S_SILU, S_TANH, S_ERF, S_ANY };
+enum Slope { S_ONE, S_CLIP, S_SILU, S_TANH, S_ERF };
 
 template <int SL>
-__device__ __forceinline__ float slope(float z, int act) {
+__device__ __forceinline__ float slope(float z) {
   if constexpr (SL == S_ONE) return 1.f;
   // (an infinity, as a z beyond fp16 is kept, has the slope of the far values: bounded, no infinity meets a zero.  A NaN stays one.)
   z = __builtin_elementwise_minimum(__builtin_elementwise_maximum(z, -1e15f), 1e15f);
@@ -160,11 +160,6 @@ __device__ __forceinline__ float slope(float z, int act) {
     const float e = gauss(z);
     return normal_cdf(z, e) + z * e * 0.39894228040f;
   }
-  return act == MVIT_ACT_NONE        ? 1.f
-         : act == MVIT_ACT_RELU      ? slope<S_CLIP>(z, act)
-         : act == MVIT_ACT_SILU      ? slope<S_SILU>(z, act)
-         : act == MVIT_ACT_GELU_TANH ? slope<S_TANH>(z, act)
-                                     : slope<S_ERF>(z, act);
 }
 
 struct SlopeArgs {
@@ -176,7 +171,25 @@ struct SlopeArgs {
   int M, N, rows, act;      // rows: of a run
 };
 
-template <int SL, bool F32>
+// 8 values of a row, `left` of them in it; ODD: at any address
+template <bool F32, bool ODD>
+__device__ __forceinline__ void values8(const void* p, size_t i, int left, float (&v)[8]) {
+  if (ODD && left < 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < left ? value_of(p, i + e, F32) : 0.f;
+  } else if constexpr (F32) {
+    float4 a, b;
+    __builtin_memcpy(&a, __builtin_assume_aligned((const float*)p + i, ODD ? 4 : 16), 16);
+    __builtin_memcpy(&b, __builtin_assume_aligned((const float*)p + i + 4, ODD ? 4 : 16), 16);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    uint4 u;
+    __builtin_memcpy(&u, __builtin_assume_aligned((const bf16_t*)p + i, ODD ? 2 : 16), 16);
+    v[0] = lo16f(u.x), v[1] = hi16f(u.x), v[2] = lo16f(u.y), v[3] = hi16f(u.y), v[4] = lo16f(u.z), v[5] = hi16f(u.z), v[6] = lo16f(u.w), v[7] = hi16f(u.w);
+  }
+}
+
+template <int SL, bool F32, bool ODD>
 __global__ __launch_bounds__(256) void act_bwd_rows(const SlopeArgs p) {
   __shared__ float sums[8][256];
   const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5, c0 = blockIdx.x * 256 + cg * 8;
@@ -187,19 +200,12 @@ __global__ __launch_bounds__(256) void act_bwd_rows(const SlopeArgs p) {
     for (int r = r0 + rg; r < r1; r += 8) {
       const size_t o = (size_t)r * p.N + c0;
       float g[8];
-      if constexpr (F32) {
-        const float4 u = *(const float4*)((const float*)p.dy + o), v = *(const float4*)((const float*)p.dy + o + 4);
-        g[0] = u.x, g[1] = u.y, g[2] = u.z, g[3] = u.w, g[4] = v.x, g[5] = v.y, g[6] = v.z, g[7] = v.w;
-      } else {
-        const uint4 u = *(const uint4*)((const bf16_t*)p.dy + o);
-        g[0] = lo16f(u.x), g[1] = hi16f(u.x), g[2] = lo16f(u.y), g[3] = hi16f(u.y);
-        g[4] = lo16f(u.z), g[5] = hi16f(u.z), g[6] = lo16f(u.w), g[7] = hi16f(u.w);
-      }
+      values8<F32, ODD>(p.dy, o, p.N - c0, g);
       if constexpr (SL != S_ONE) {
-        const uint4 u = *(const uint4*)(p.pre + o);
-        const float z[8] = {lo16f(u.x), hi16f(u.x), lo16f(u.y), hi16f(u.y), lo16f(u.z), hi16f(u.z), lo16f(u.w), hi16f(u.w)};
+        float z[8];
+        values8<false, ODD>(p.pre, o, p.N - c0, z);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] *= slope<SL>(z[e], 0);
+        for (int e = 0; e < 8; ++e) g[e] *= slope<SL>(z[e]);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] += g[e];
@@ -219,24 +225,6 @@ __global__ __launch_bounds__(256) void act_bwd_rows(const SlopeArgs p) {
   }
 }
 
-// by elements, where N or an address is not a multiple of 8 values: a thread a column, dz with its rows padded by zeros to ld_dz
-template <bool F32>
-__global__ __launch_bounds__(256) void act_bwd_elements(const SlopeArgs p) {
-  const int c = blockIdx.x * 256 + threadIdx.x, r0 = blockIdx.y * p.rows, r1 = min(r0 + p.rows, p.M);
-  float sum = 0.f;
-  for (int r = r0; r < r1; ++r) {
-    float g = 0.f;
-    if (c < p.N) {
-      const size_t o = (size_t)r * p.N + c;
-      g = value_of(p.dy, o, F32);
-      if (p.act != MVIT_ACT_NONE) g *= slope<S_ANY>(bf2f(p.pre[o]), p.act);
-      sum += g;
-    }
-    if (p.dz && c < p.ld_dz) p.dz[(size_t)r * p.ld_dz + c] = f2bf(g);
-  }
-  if (p.part && c < p.N) p.part[(size_t)blockIdx.y * p.N + c] = sum;
-}
-
 // rows of a run: blocks enough for eight a CU, no more than 128 runs to add up, no fewer than 8 rows
 int run_rows(int M, int N) {
   const int cols = (N + 255) / 256;
@@ -247,18 +235,18 @@ int run_rows(int M, int N) {
 }
 int run_count(int M, int N) { return M <= 0 ? 0 : (M + run_rows(M, N) - 1) / run_rows(M, N); }
 
-template <bool F32>
+template <bool F32, bool ODD>
 void launch_rows_bwd(const SlopeArgs& a, dim3 grid, hipStream_t s) {
   if (a.act == MVIT_ACT_NONE)
-    hipLaunchKernelGGL((act_bwd_rows<S_ONE, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_ONE, F32, ODD>), grid, dim3(256), 0, s, a);
   else if (a.act == MVIT_ACT_RELU)
-    hipLaunchKernelGGL((act_bwd_rows<S_CLIP, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_CLIP, F32, ODD>), grid, dim3(256), 0, s, a);
   else if (a.act == MVIT_ACT_GELU)
-    hipLaunchKernelGGL((act_bwd_rows<S_ERF, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_ERF, F32, ODD>), grid, dim3(256), 0, s, a);
   else if (a.act == MVIT_ACT_SILU)
-    hipLaunchKernelGGL((act_bwd_rows<S_SILU, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_SILU, F32, ODD>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((act_bwd_rows<S_TANH, F32>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((act_bwd_rows<S_TANH, F32, ODD>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -275,16 +263,11 @@ extern "C" MVIT_API int mvit_act_bwd(const void* dy, int dy_f32, const void* pre
   const int runs = run_count(M, N);
   if (M > 0) {
     const SlopeArgs a = {dy, (const bf16_t*)pre, (bf16_t*)dz, dbias ? (float*)scratch : nullptr, ld_dz, M, N, run_rows(M, N), act};
-    if (N % 8 == 0 && aligned16(dy) && aligned16(pre)) {
-      const dim3 grid((N + 255) / 256, runs);
-      dy_f32 ? launch_rows_bwd<true>(a, grid, s) : launch_rows_bwd<false>(a, grid, s);
-    } else {
-      const dim3 grid((unsigned)(((dz ? ld_dz : N) + 255) / 256), runs);
-      if (dy_f32)
-        hipLaunchKernelGGL((act_bwd_elements<true>), grid, dim3(256), 0, s, a);
-      else
-        hipLaunchKernelGGL((act_bwd_elements<false>), grid, dim3(256), 0, s, a);
-    }
+    const dim3 grid((N + 255) / 256, runs);
+    if (N % 8 == 0 && aligned16(dy) && aligned16(pre))
+      dy_f32 ? launch_rows_bwd<true, false>(a, grid, s) : launch_rows_bwd<false, false>(a, grid, s);
+    else
+      dy_f32 ? launch_rows_bwd<true, true>(a, grid, s) : launch_rows_bwd<false, true>(a, grid, s);
     if (const int rc = MVIT_LAUNCH_CHECK()) return rc;
   }
   return dbias ? launch_sum_parts((const float*)scratch, dbias, runs, N, dbias_f32, s) : MVIT_OK;

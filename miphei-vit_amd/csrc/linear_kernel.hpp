@@ -46,7 +46,9 @@ struct Args {
 // What a tile kernel is compiled for besides its operands.  The epilogue is unrolled over the accumulators: with every activation and
 // output in one kernel it was 9800 instructions, more than the instruction cache holds, and cost 3 us a tile instead of 1.
 enum Act { A_CLIP, A_SILU, A_TANH, A_ERF, A_ANY };
-template <bool OUT32, int ACT, bool VEC>   // VEC: rows of y, pre and res start on 16 bytes and N % 8 == 0; else by elements
+// VEC: rows of y, pre and res start on 16 bytes and N % 8 == 0; else pieces go to odd addresses (global memory takes 16-byte accesses at any)
+// and a row's last one by elements
+template <bool OUT32, int ACT, bool VEC>
 struct End {
   static constexpr bool out32 = OUT32, vec = VEC;
   static constexpr int act = ACT;
@@ -109,58 +111,81 @@ struct Columns {
 // The residual's piece, raw: loaded ahead of use, because a load that is waited for behind stores waits for these too
 template <class E>
 __device__ __forceinline__ uint4 residual_piece(const Args& p, int row, int col) {
-  if (!E::vec || !p.res || row >= p.M || col >= p.N) return make_uint4(0, 0, 0, 0);
-  return *(const uint4*)((const char*)p.res + ((size_t)row * p.ldr + col) * (E::out32 ? 4 : 2));
+  uint4 u = make_uint4(0, 0, 0, 0);
+  if (!p.res || row >= p.M || col >= p.N) return u;
+  const char* at = (const char*)p.res + ((size_t)row * p.ldr + col) * (E::out32 ? 4 : 2);
+  if constexpr (E::vec) return *(const uint4*)at;
+  if (p.N - col >= (E::out32 ? 4 : 8)) {
+    __builtin_memcpy(&u, at, 16);
+  } else if constexpr (E::out32) {
+    u.x = ((const uint32_t*)at)[0];
+    if (p.N - col > 1) u.y = ((const uint32_t*)at)[1];
+    if (p.N - col > 2) u.z = ((const uint32_t*)at)[2];
+  } else {
+    const bf16_t* h = (const bf16_t*)at;
+    auto two = [&](int e) __attribute__((always_inline)) {
+      return (e < p.N - col ? (uint32_t)h[e] : 0u) | (e + 1 < p.N - col ? (uint32_t)h[e + 1] << 16 : 0u);
+    };
+    u = make_uint4(two(0), two(2), two(4), two(6));
+  }
+  return u;
+}
+// BYTES of bits to `at`, the first `left` of 4-byte (WORDS) or 2-byte values of them where that is fewer
+template <class E, bool WORDS, int BYTES>
+__device__ __forceinline__ void put(void* at, const uint32_t (&u)[BYTES / 4], int left) {
+  if constexpr (E::vec) {
+    if constexpr (BYTES == 16)
+      *(uint4*)at = make_uint4(u[0], u[1], u[2], u[3]);
+    else
+      *(uint2*)at = make_uint2(u[0], u[1]);
+  } else if (left >= BYTES / (WORDS ? 4 : 2)) {
+    __builtin_memcpy(at, u, BYTES);
+  } else {
+#pragma unroll
+    for (int e = 0; e < BYTES / (WORDS ? 4 : 2); ++e)
+      if (e < left) {
+        if constexpr (WORDS)
+          ((uint32_t*)at)[e] = u[e];
+        else
+          ((bf16_t*)at)[e] = (bf16_t)(e & 1 ? u[e / 2] >> 16 : u[e / 2]);
+      }
+  }
 }
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
 }
 
-// The end of a piece but for its store: v (products, times their row's scale) -> the bits of y (E::vec), or all of it (not E::vec)
+// The end of a piece but for its store: v (products, times their row's scale) -> the bits of y
 template <bool OP8, class E, int W>
 __device__ __forceinline__ uint4 finish(const Args& p, float (&v)[W], int row, int col, const Columns<OP8, W>& c, const uint4& res) {
   static_assert(W == (E::out32 ? 4 : 8), "16 bytes of y");
 #pragma unroll
   for (int e = 0; e < W; ++e) v[e] = OP8 ? __builtin_fmaf(v[e], c.s[e], c.b[e]) : v[e] + c.b[e];
-  if constexpr (E::vec) {
-    if (!OP8 && p.pre && row < p.M && col < p.N) {
-      bf16_t* o = (bf16_t*)p.pre + (size_t)row * p.N + col;
-      if constexpr (W == 8)
-        *(uint4*)o = pack8(v);
-      else
-        *(uint2*)o = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
-    }
+  if (!OP8 && p.pre && row < p.M && col < p.N) {
+    uint32_t u[W / 2];
 #pragma unroll
-    for (int e = 0; e < W; ++e) v[e] = activated<E::act>(p, v[e]);
-    if constexpr (W == 4) {
-      if (p.res) v[0] += __uint_as_float(res.x), v[1] += __uint_as_float(res.y), v[2] += __uint_as_float(res.z), v[3] += __uint_as_float(res.w);
-      return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    } else {
-      if (p.res) {
-        v[0] += lo16f(res.x), v[1] += hi16f(res.x), v[2] += lo16f(res.y), v[3] += hi16f(res.y);
-        v[4] += lo16f(res.z), v[5] += hi16f(res.z), v[6] += lo16f(res.w), v[7] += hi16f(res.w);
-      }
-      return pack8(v);
-    }
+    for (int e = 0; e < W / 2; ++e) u[e] = pack2bf(v[2 * e], v[2 * e + 1]);
+    put<E, false, W * 2>((bf16_t*)p.pre + (size_t)row * p.N + col, u, p.N - col);
+  }
+#pragma unroll
+  for (int e = 0; e < W; ++e) v[e] = activated<E::act>(p, v[e]);
+  if constexpr (W == 4) {
+    if (p.res) v[0] += __uint_as_float(res.x), v[1] += __uint_as_float(res.y), v[2] += __uint_as_float(res.z), v[3] += __uint_as_float(res.w);
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
   } else {
-    const size_t o = (size_t)row * p.N + col, r = (size_t)row * p.ldr + col;
-#pragma unroll
-    for (int e = 0; e < W; ++e)
-      if (row < p.M && col + e < p.N) {
-        if (!OP8 && p.pre) ((bf16_t*)p.pre)[o + e] = f2bf(v[e]);
-        float u = activated<E::act>(p, v[e]);
-        if (p.res) u += value_of(p.res, r + e, E::out32);
-        if constexpr (E::out32)
-          ((float*)p.y)[o + e] = u;
-        else
-          ((bf16_t*)p.y)[o + e] = f2bf(u);
-      }
-    return make_uint4(0, 0, 0, 0);
+    if (p.res) {
+      v[0] += lo16f(res.x), v[1] += hi16f(res.x), v[2] += lo16f(res.y), v[3] += hi16f(res.y);
+      v[4] += lo16f(res.z), v[5] += hi16f(res.z), v[6] += lo16f(res.w), v[7] += hi16f(res.w);
+    }
+    return pack8(v);
   }
 }
 template <class E>
 __device__ __forceinline__ void store_piece(const Args& p, int row, int col, const uint4& u) {
-  if (E::vec && row < p.M && col < p.N) *(uint4*)((char*)p.y + ((size_t)row * p.N + col) * (E::out32 ? 4 : 2)) = u;
+  if (row < p.M && col < p.N) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    put<E, E::out32, 16>((char*)p.y + ((size_t)row * p.N + col) * (E::out32 ? 4 : 2), w, p.N - col);
+  }
 }
 
 // 16 e4m3 values -> two fragments of 8 16-bit ones (order kept; exact)
@@ -526,7 +551,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
           out[q] = finish<OP8, E, W>(p, o, row, col_of(q), cols[q], res[i & 1][q]);
           if constexpr (!WIDE) store_piece<E>(p, row, col_of(q), out[q]);
         }
-        if constexpr (WIDE && E::vec) {
+        if constexpr (WIDE) {
           // two lanes of a row, 32 bytes a store: trade pieces between rows r and r + 16, so that four lanes have 64 bytes of one row
 #pragma unroll
           for (int q = 0; q < NP; q += 2) {

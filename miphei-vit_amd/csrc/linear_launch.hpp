@@ -78,20 +78,23 @@ int dispatch_grad(const Args& a, int tile, hipStream_t s) {
   }
 }
 
-template <int MODE, bool OUT32>
-int dispatch(const Args& a, bool vec, hipStream_t s) {
-  if (!vec) return by_size<MODE, End<OUT32, A_ANY, false>>(a, s);
+template <int MODE, bool OUT32, bool VEC>
+int by_activation(const Args& a, hipStream_t s) {
   switch (a.act) {
     case MVIT_ACT_NONE:
     case MVIT_ACT_RELU:
-      return by_size<MODE, End<OUT32, A_CLIP, true>>(a, s);
+      return by_size<MODE, End<OUT32, A_CLIP, VEC>>(a, s);
     case MVIT_ACT_GELU:
-      return by_size<MODE, End<OUT32, A_ERF, true>>(a, s);
+      return by_size<MODE, End<OUT32, A_ERF, VEC>>(a, s);
     case MVIT_ACT_SILU:
-      return by_size<MODE, End<OUT32, A_SILU, true>>(a, s);
+      return by_size<MODE, End<OUT32, A_SILU, VEC>>(a, s);
     default:
-      return by_size<MODE, End<OUT32, A_TANH, true>>(a, s);
+      return by_size<MODE, End<OUT32, A_TANH, VEC>>(a, s);
   }
+}
+template <int MODE, bool OUT32>
+int dispatch(const Args& a, bool vec, hipStream_t s) {
+  return vec ? by_activation<MODE, OUT32, true>(a, s) : by_activation<MODE, OUT32, false>(a, s);
 }
 
 }  // namespace mvit_linear

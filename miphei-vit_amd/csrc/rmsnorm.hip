@@ -9,7 +9,9 @@
 // are formed, and is written once.
 //  * A row belongs to TPR = 64 threads (one wave: no barrier) or to a block (fewer registers and loads a thread: for wide rows, and for
 //    few, whose latency counts).
-//  * Each thread holds NV pieces of VEC values; VEC = 8 (16-byte loads) where D, the row strides and the addresses allow it, else 1.
+//  * Each thread holds NV pieces of 8 values (16-byte loads); where D, a row stride or an address is odd the loads go to odd addresses and a
+//    row's last piece goes by elements (ODD), us with elements before and so: 8 bits
+//    of an f32 stream [16623, 1053] 106 / 46, [2032, 7956] 257 / 40
 //  * Rows are walked with a grid stride, so that w is loaded once per thread and not once per row.
 // Measured against a 1 GiB copy's 5.05 TB/s (one MI355X): f32 stream of [21056, 1536] forward 75 us (388 MB, 5.2 TB/s), backward with
 // d w 96 us (517 MB, 5.4 TB/s); 16-bit stream to 8 bits [20816, 1536] 37 us (6.0 TB/s); quantisation [21056, 4096] 43 us (6.0 TB/s).
@@ -25,48 +27,61 @@ enum { T16 = 0, F32 = 1, NONE = 2, F8 = 3 };
 
 constexpr float E4M3_MAX = 448.f, AMAX_MIN = 1e-30f;
 
-// VEC values from element `i` of a 16-bit or f32 array
-template <int T, int VEC>
-__device__ __forceinline__ void load_vec(const void* p, size_t i, float* v) {
-  if constexpr (T == T16) {
-    if constexpr (VEC == 8) {
-      const uint4 u = *(const uint4*)((const bf16_t*)p + i);
-      v[0] = lo16f(u.x), v[1] = hi16f(u.x), v[2] = lo16f(u.y), v[3] = hi16f(u.y);
-      v[4] = lo16f(u.z), v[5] = hi16f(u.z), v[6] = lo16f(u.w), v[7] = hi16f(u.w);
-    } else {
-      v[0] = bf2f(((const bf16_t*)p)[i]);
-    }
+// 8 values from element `i` of a 16-bit or f32 array (f32: 8 from 4-byte, 16-bit: from 2-byte addresses where ODD; global memory takes
+// 16-byte accesses at any address), of which the last `left` .. 8 lie behind the row where ODD: not touched, and zeros.
+constexpr int VEC = 8;
+template <bool ODD, class V>
+__device__ __forceinline__ V load_raw(const void* p) {
+  V u;
+  if constexpr (ODD)
+    __builtin_memcpy(&u, p, sizeof(V));
+  else
+    u = *(const V*)p;
+  return u;
+}
+template <bool ODD, class V>
+__device__ __forceinline__ void store_raw(void* p, const V& u) {
+  if constexpr (ODD)
+    __builtin_memcpy(p, &u, sizeof(V));
+  else
+    *(V*)p = u;
+}
+template <int T, bool ODD>
+__device__ __forceinline__ void load_vec(const void* p, size_t i, int left, float* v) {
+  if (ODD && left < VEC) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = e >= left ? 0.f : T == T16 ? bf2f(((const bf16_t*)p)[i + e]) : ((const float*)p)[i + e];
+  } else if constexpr (T == T16) {
+    const uint4 u = load_raw<ODD, uint4>((const bf16_t*)p + i);
+    v[0] = lo16f(u.x), v[1] = hi16f(u.x), v[2] = lo16f(u.y), v[3] = hi16f(u.y);
+    v[4] = lo16f(u.z), v[5] = hi16f(u.z), v[6] = lo16f(u.w), v[7] = hi16f(u.w);
   } else {
-    if constexpr (VEC == 8) {
-      const float4 a = *(const float4*)((const float*)p + i), b = *(const float4*)((const float*)p + i + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      v[0] = ((const float*)p)[i];
-    }
+    const float4 a = load_raw<ODD, float4>((const float*)p + i), b = load_raw<ODD, float4>((const float*)p + i + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   }
 }
-template <int T, int VEC>
-__device__ __forceinline__ void store_vec(void* p, size_t i, const float* v) {
-  if constexpr (T == T16) {
-    if constexpr (VEC == 8)
-      *(uint4*)((bf16_t*)p + i) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
-    else
-      ((bf16_t*)p)[i] = f2bf(v[0]);
+template <int T, bool ODD>
+__device__ __forceinline__ void store_vec(void* p, size_t i, int left, const float* v) {
+  if (ODD && left < VEC) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (e < left) {
+        if constexpr (T == T16)
+          ((bf16_t*)p)[i + e] = f2bf(v[e]);
+        else if constexpr (T == F32)
+          ((float*)p)[i + e] = v[e];
+        else
+          ((uint8_t*)p)[i + e] = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[e], v[e], 0, false) & 0xff);
+      }
+  } else if constexpr (T == T16) {
+    store_raw<ODD>((bf16_t*)p + i, make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])));
   } else if constexpr (T == F32) {
-    if constexpr (VEC == 8) {
-      *(float4*)((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
-      *(float4*)((float*)p + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      ((float*)p)[i] = v[0];
-    }
+    store_raw<ODD>((float*)p + i, make_float4(v[0], v[1], v[2], v[3]));
+    store_raw<ODD>((float*)p + i + 4, make_float4(v[4], v[5], v[6], v[7]));
   } else {
-    if constexpr (VEC == 8) {
-      int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
-      a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true), b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], b, true);
-      *(int2*)((uint8_t*)p + i) = make_int2(a, b);
-    } else {
-      ((uint8_t*)p)[i] = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[0], 0, false) & 0xff);
-    }
+    int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true), b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], b, true);
+    store_raw<ODD>((uint8_t*)p + i, make_int2(a, b));
   }
 }
 // the value as it reads back from the stream's own type (16-bit streams are normed as they are stored)
@@ -124,7 +139,7 @@ struct RowArgs {
 };
 
 // NORM = false: y is x itself (the quantisation alone)
-template <int TPR, int NV, int VEC, int XT, int RT, int YT, bool NORM>
+template <int TPR, int NV, bool ODD, int XT, int RT, int YT, bool NORM>
 __global__ __launch_bounds__(256) void rms_fwd(const RowArgs p) {
   constexpr int RPB = 256 / TPR;
   __shared__ float lds[2 * 4];
@@ -137,9 +152,9 @@ __global__ __launch_bounds__(256) void rms_fwd(const RowArgs p) {
       const int c = (v * TPR + t) * VEC;
       if (c < p.D) {
         if (p.w_f32)
-          load_vec<F32, VEC>(p.w, c, w[v]);
+          load_vec<F32, ODD>(p.w, c, p.D - c, w[v]);
         else
-          load_vec<T16, VEC>(p.w, c, w[v]);
+          load_vec<T16, ODD>(p.w, c, p.D - c, w[v]);
       }
     }
   }
@@ -152,7 +167,7 @@ __global__ __launch_bounds__(256) void rms_fwd(const RowArgs p) {
       const int c = (v * TPR + t) * VEC;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) a[v][e] = 0.f;
-      if (c < p.D) load_vec<XT, VEC>(p.x, xo + c, a[v]);
+      if (c < p.D) load_vec<XT, ODD>(p.x, xo + c, p.D - c, a[v]);
     }
     if constexpr (RT != NONE) {
 #pragma unroll
@@ -160,10 +175,10 @@ __global__ __launch_bounds__(256) void rms_fwd(const RowArgs p) {
         const int c = (v * TPR + t) * VEC;
         if (c < p.D) {
           float r[VEC];
-          load_vec<RT, VEC>(p.res, ro + c, r);
+          load_vec<RT, ODD>(p.res, ro + c, p.D - c, r);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) a[v][e] = as_stored<RT>(a[v][e] + r[e]);
-          store_vec<RT, VEC>(p.h, o + c, a[v]);
+          store_vec<RT, ODD>(p.h, o + c, p.D - c, a[v]);
         }
       }
     }
@@ -179,7 +194,7 @@ __global__ __launch_bounds__(256) void rms_fwd(const RowArgs p) {
       for (int v = 0; v < NV; ++v) {
         const int c = (v * TPR + t) * VEC;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) a[v][e] = c < p.D ? a[v][e] * r * w[v][e] : 0.f;
+        for (int e = 0; e < VEC; ++e) a[v][e] = c + (ODD ? e : 0) < p.D ? a[v][e] * r * w[v][e] : 0.f;
       }
     }
     if constexpr (YT == F8) {
@@ -207,7 +222,7 @@ __global__ __launch_bounds__(256) void rms_fwd(const RowArgs p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * TPR + t) * VEC;
-      if (c < p.D) store_vec<YT, VEC>(p.y, o + c, a[v]);
+      if (c < p.D) store_vec<YT, ODD>(p.y, o + c, p.D - c, a[v]);
     }
   }
 }
@@ -221,7 +236,7 @@ struct BwdArgs {
 };
 
 // XT: the type of dy and dx; HT: the type of h, dh and dres.  Blocks of NT threads, a row to a wave (TPR = 64) or to the block (TPR = NT).
-template <int NT, int TPR, int NV, int VEC, int XT, int HT>
+template <int NT, int TPR, int NV, bool ODD, int XT, int HT>
 __global__ __launch_bounds__(NT) void rms_bwd(const BwdArgs p) {
   constexpr int RPB = NT / TPR;
   static_assert(RPB == 1 || TPR == 64, "rows that share a barrier would have to end together");
@@ -236,9 +251,9 @@ __global__ __launch_bounds__(NT) void rms_bwd(const BwdArgs p) {
     for (int e = 0; e < VEC; ++e) w[v][e] = acc[v][e] = 0.f;
     if (c < p.D) {
       if (p.w_f32)
-        load_vec<F32, VEC>(p.w, c, w[v]);
+        load_vec<F32, ODD>(p.w, c, p.D - c, w[v]);
       else
-        load_vec<T16, VEC>(p.w, c, w[v]);
+        load_vec<T16, ODD>(p.w, c, p.D - c, w[v]);
     }
   }
   const float inv_d = 1.f / (float)p.D;
@@ -252,8 +267,8 @@ __global__ __launch_bounds__(NT) void rms_bwd(const BwdArgs p) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) g[v][e] = h[v][e] = 0.f;
       if (c < p.D) {
-        load_vec<HT, VEC>(p.h, o + c, h[v]);
-        load_vec<XT, VEC>(p.dy, o + c, g[v]);
+        load_vec<HT, ODD>(p.h, o + c, p.D - c, h[v]);
+        load_vec<XT, ODD>(p.dy, o + c, p.D - c, g[v]);
       }
     }
     float dot = 0.f;
@@ -274,11 +289,11 @@ __global__ __launch_bounds__(NT) void rms_bwd(const BwdArgs p) {
         float d[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[e] = 0.f;
-        if (p.dh) load_vec<HT, VEC>(p.dh, o + c, d);
+        if (p.dh) load_vec<HT, ODD>(p.dh, o + c, p.D - c, d);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[e] += r * (g[v][e] - h[v][e] * mean);
-        if (p.dx) store_vec<XT, VEC>(p.dx, o + c, d);
-        if (p.dres) store_vec<HT, VEC>(p.dres, o + c, d);
+        if (p.dx) store_vec<XT, ODD>(p.dx, o + c, p.D - c, d);
+        if (p.dres) store_vec<HT, ODD>(p.dres, o + c, p.D - c, d);
       }
     }
   }
@@ -294,7 +309,8 @@ __global__ __launch_bounds__(NT) void rms_bwd(const BwdArgs p) {
           const int c = (v * TPR + t) * VEC;
           if (c < p.D)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) lds[c + e] += acc[v][e];
+            for (int e = 0; e < VEC; ++e)
+              if (!ODD || c + e < p.D) lds[c + e] += acc[v][e];
         }
       }
       __syncthreads();
@@ -304,7 +320,7 @@ __global__ __launch_bounds__(NT) void rms_bwd(const BwdArgs p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * TPR + t) * VEC;
-      if (c < p.D) store_vec<F32, VEC>(out, c, acc[v]);
+      if (c < p.D) store_vec<F32, ODD>(out, c, p.D - c, acc[v]);
     }
   }
 }
@@ -313,37 +329,35 @@ constexpr int MAX_D = 16384, MAX_M = 1 << 30;   // (row numbers run past M by a 
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int TPR, int NV, int VEC, int XT, int RT, int YT, bool NORM>
+template <int TPR, int NV, bool ODD, int XT, int RT, int YT, bool NORM>
 int launch_fwd(const RowArgs& a, hipStream_t s) {
   const int rpb = 256 / TPR;
   // rounds of the grid stride: [20816, 1536] bf16 to 8 bits 40 us with 8 blocks a CU, 37 with 16, 39 with as many as there are rows for
   const long long need = ((long long)a.M + rpb - 1) / rpb, most = (long long)mvit_num_cus() * 16;
-  hipLaunchKernelGGL((rms_fwd<TPR, NV, VEC, XT, RT, YT, NORM>), dim3((unsigned)(need < most ? need : most)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((rms_fwd<TPR, NV, ODD, XT, RT, YT, NORM>), dim3((unsigned)(need < most ? need : most)), dim3(256), 0, s, a);
   return MVIT_LAUNCH_CHECK();
 }
 
-template <int XT, int RT, int YT, bool NORM>
-int fwd_layout(const RowArgs& a, bool vec, hipStream_t s) {
+template <bool ODD, int XT, int RT, int YT, bool NORM>
+int fwd_layout(const RowArgs& a, hipStream_t s) {
   const int D = a.D;
-  if (vec) {
-    // a wave a row, or 256 threads (f32 stream to 8 bits, us): rows of 512: 1024 of them 3.1 / 3.8, 8192 9.1 / 12.1; of 1024: 256 3.4 / 3.2,
-    // 1024 4.1 / 4.3, 8192 15.7 / 16.5; of 1536: 256 4.1 / 3.4, 2048 7.6 / 6.9, 4096 12.0 / 13.2; of 4096: 64 6.9 / 3.7,
-    // 8192 83 / 75
-    if (D <= 512) return launch_fwd<64, 1, 8, XT, RT, YT, NORM>(a, s);
-    if (D <= 2048 && a.M >= (D <= 1024 ? 4 : 12) * mvit_num_cus()) {
-      if (D <= 1024) return launch_fwd<64, 2, 8, XT, RT, YT, NORM>(a, s);
-      if (D <= 1536) return launch_fwd<64, 3, 8, XT, RT, YT, NORM>(a, s);
-      return launch_fwd<64, 4, 8, XT, RT, YT, NORM>(a, s);
-    }
-    if (D <= 2048) return launch_fwd<256, 1, 8, XT, RT, YT, NORM>(a, s);
-    if (D <= 4096) return launch_fwd<256, 2, 8, XT, RT, YT, NORM>(a, s);
-    if (D <= 8192) return launch_fwd<256, 4, 8, XT, RT, YT, NORM>(a, s);
-    return launch_fwd<256, 8, 8, XT, RT, YT, NORM>(a, s);
+  // a wave a row, or 256 threads (f32 stream to 8 bits, us): rows of 512: 1024 of them 3.1 / 3.8, 8192 9.1 / 12.1; of 1024: 256 3.4 / 3.2,
+  // 1024 4.1 / 4.3, 8192 15.7 / 16.5; of 1536: 256 4.1 / 3.4, 2048 7.6 / 6.9, 4096 12.0 / 13.2; of 4096: 64 6.9 / 3.7,
+  // 8192 83 / 75
+  if (D <= 512) return launch_fwd<64, 1, ODD, XT, RT, YT, NORM>(a, s);
+  if (D <= 2048 && a.M >= (D <= 1024 ? 4 : 12) * mvit_num_cus()) {
+    if (D <= 1024) return launch_fwd<64, 2, ODD, XT, RT, YT, NORM>(a, s);
+    if (D <= 1536) return launch_fwd<64, 3, ODD, XT, RT, YT, NORM>(a, s);
+    return launch_fwd<64, 4, ODD, XT, RT, YT, NORM>(a, s);
   }
-  if (D <= 512) return launch_fwd<64, 8, 1, XT, RT, YT, NORM>(a, s);
-  if (D <= 1024) return launch_fwd<64, 16, 1, XT, RT, YT, NORM>(a, s);
-  if (D <= 4096) return launch_fwd<256, 16, 1, XT, RT, YT, NORM>(a, s);
-  return launch_fwd<256, 64, 1, XT, RT, YT, NORM>(a, s);
+  if (D <= 2048) return launch_fwd<256, 1, ODD, XT, RT, YT, NORM>(a, s);
+  if (D <= 4096) return launch_fwd<256, 2, ODD, XT, RT, YT, NORM>(a, s);
+  if (D <= 8192) return launch_fwd<256, 4, ODD, XT, RT, YT, NORM>(a, s);
+  return launch_fwd<256, 8, ODD, XT, RT, YT, NORM>(a, s);
+}
+template <int XT, int RT, int YT, bool NORM>
+int fwd_layout(const RowArgs& a, bool even, hipStream_t s) {
+  return even ? fwd_layout<false, XT, RT, YT, NORM>(a, s) : fwd_layout<true, XT, RT, YT, NORM>(a, s);
 }
 
 // vector loads: every row of every operand starts on 16 bytes (8 for the e4m3 output, whose rows are D bytes)
@@ -364,33 +378,31 @@ int bwd_blocks(int M, int nt) {
   return (int)(M < most ? M : most);
 }
 
-template <int NT, int TPR, int NV, int VEC, int XT, int HT>
+template <int NT, int TPR, int NV, bool ODD, int XT, int HT>
 int launch_bwd(const BwdArgs& a, int& grid, hipStream_t s) {
   const size_t lds = TPR == 64 ? (size_t)a.D * 4 : 64;
   constexpr int RPB = NT / TPR;
   grid = bwd_blocks((a.M + RPB - 1) / RPB, NT);
-  hipLaunchKernelGGL((rms_bwd<NT, TPR, NV, VEC, XT, HT>), dim3(grid), dim3(NT), lds, s, a);
+  hipLaunchKernelGGL((rms_bwd<NT, TPR, NV, ODD, XT, HT>), dim3(grid), dim3(NT), lds, s, a);
   return MVIT_LAUNCH_CHECK();
 }
 
-template <int XT, int HT>
-int bwd_layout(const BwdArgs& a, bool vec, int& grid, hipStream_t s) {
+template <bool ODD, int XT, int HT>
+int bwd_layout(const BwdArgs& a, int& grid, hipStream_t s) {
   const int D = a.D;
-  if (vec) {
-    // f32 stream, with d w, us.  A wave a row or a block: rows of 1024: 1024 of them 9.6 / 8.1, 4096 17.5 / 17.7, 8192 26 / 28, 21056 69 / 87;
-    // of 1536: 21056 107 / 105; of 2048: 140 / 127.  A row to 256 threads or to 512: of 1536: 1024 11.1 / 9.0 (twice the partial sums of
-    // d w), 8192 35 / 34, 21056 96 / 105; of 2048: 131 / 126
-    if (D <= 512) return launch_bwd<512, 64, 1, 8, XT, HT>(a, grid, s);
-    if (D <= 1024 && a.M >= 16 * mvit_num_cus()) return launch_bwd<512, 64, 2, 8, XT, HT>(a, grid, s);
-    if (D <= 1536 && a.M >= 32 * mvit_num_cus()) return launch_bwd<256, 256, 1, 8, XT, HT>(a, grid, s);
-    if (D <= 4096) return launch_bwd<512, 512, 1, 8, XT, HT>(a, grid, s);
-    if (D <= 8192) return launch_bwd<512, 512, 2, 8, XT, HT>(a, grid, s);
-    return launch_bwd<512, 512, 4, 8, XT, HT>(a, grid, s);
-  }
-  if (D <= 512) return launch_bwd<512, 64, 8, 1, XT, HT>(a, grid, s);
-  if (D <= 1024) return launch_bwd<512, 64, 16, 1, XT, HT>(a, grid, s);
-  if (D <= 4096) return launch_bwd<512, 512, 8, 1, XT, HT>(a, grid, s);
-  return launch_bwd<512, 512, 32, 1, XT, HT>(a, grid, s);
+  // f32 stream, with d w, us.  A wave a row or a block: rows of 1024: 1024 of them 9.6 / 8.1, 4096 17.5 / 17.7, 8192 26 / 28, 21056 69 / 87;
+  // of 1536: 21056 107 / 105; of 2048: 140 / 127.  A row to 256 threads or to 512: of 1536: 1024 11.1 / 9.0 (twice the partial sums of
+  // d w), 8192 35 / 34, 21056 96 / 105; of 2048: 131 / 126
+  if (D <= 512) return launch_bwd<512, 64, 1, ODD, XT, HT>(a, grid, s);
+  if (D <= 1024 && a.M >= 16 * mvit_num_cus()) return launch_bwd<512, 64, 2, ODD, XT, HT>(a, grid, s);
+  if (D <= 1920 && a.M >= 32 * mvit_num_cus()) return launch_bwd<256, 256, 1, ODD, XT, HT>(a, grid, s);
+  if (D <= 4096) return launch_bwd<512, 512, 1, ODD, XT, HT>(a, grid, s);
+  if (D <= 8192) return launch_bwd<512, 512, 2, ODD, XT, HT>(a, grid, s);
+  return launch_bwd<512, 512, 4, ODD, XT, HT>(a, grid, s);
+}
+template <int XT, int HT>
+int bwd_layout(const BwdArgs& a, bool even, int& grid, hipStream_t s) {
+  return even ? bwd_layout<false, XT, HT>(a, grid, s) : bwd_layout<true, XT, HT>(a, grid, s);
 }
 
 }  // namespace
