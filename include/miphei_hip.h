@@ -207,13 +207,17 @@ MVIT_API int mvit_rotary(const mvit_rotary_args* args, mvit_stream_t stream);
  * receives the value in front of the activation for the backward pass.  mvit_linear_fp8: e4m3 x, W, the product times
  * x_scale(f32)[m] * w_scale(f32)[n]; no pre.  bias [N] f32 or 16-bit, may be NULL.  y dense, f32 or 16-bit; res (may be NULL) has y's type
  * and its own row stride ldr.  ldx, ldw, ldr in elements.  x, W rows start on 16 bytes and K is a multiple of 16 bytes (8 or 16 values);
- * K and the row strides of x and W are at most 2^23 bytes.  M up to 2^30, N up to 2^24, of any size. */
+ * K and the row strides of x and W are at most 2^23 bytes.  M up to 2^30, N up to 2^24, of any size.  scratch (may be
+ * NULL: slower): mvit_linear_scratch_bytes(M, N, bytes of a row of K) bytes, on 16 bytes, for the products of parts of a long K where there are few
+ * rows or columns (added in order; none where that is 0). */
 enum mvit_activation { MVIT_ACT_NONE = 0, MVIT_ACT_RELU = 1, MVIT_ACT_SILU = 2, MVIT_ACT_GELU = 3, MVIT_ACT_GELU_TANH = 4 };
 typedef struct mvit_linear_args {
   const void* x; const void* w; const void* bias; const void* res; void* y; void* pre; const float* x_scale; const float* w_scale;
   long long ldx, ldw, ldr;
   int M, N, K, act, bias_f32, y_f32;
+  void* scratch; long long scratch_bytes;
 } mvit_linear_args;
+MVIT_API long long mvit_linear_scratch_bytes(int M, int N, long long k_bytes);
 MVIT_API int mvit_linear_act(const mvit_linear_args* args, mvit_stream_t stream);
 MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_stream_t stream);
 /* The products of its backward pass, 16-bit, f32 accumulation, of operands as they lie in memory: x_rows = 0: y[M,N] = x[M,K] W[K,N] (dx = dz W,

@@ -68,7 +68,8 @@ class RotaryArgs(C.Structure):
 class LinearArgs(C.Structure):
     _fields_ = [("x", vp), ("w", vp), ("bias", vp), ("res", vp), ("y", vp), ("pre", vp), ("x_scale", vp), ("w_scale", vp),
                 ("ldx", ll), ("ldw", ll), ("ldr", ll),
-                ("M", ci), ("N", ci), ("K", ci), ("act", ci), ("bias_f32", ci), ("y_f32", ci)]
+                ("M", ci), ("N", ci), ("K", ci), ("act", ci), ("bias_f32", ci), ("y_f32", ci),
+                ("scratch", vp), ("scratch_bytes", ll)]
 
 
 # name -> argtypes (restype is always int); mirrors include/miphei_hip.h
@@ -138,6 +139,7 @@ SIGNATURES = {
     "mvit_linear_act": [C.POINTER(LinearArgs), vp],
     "mvit_linear_fp8": [C.POINTER(LinearArgs), vp],
     "mvit_act_bwd": [vp, ci, vp, ci, vp, ll, vp, ci, vp, ci, ci, vp],
+    "mvit_linear_scratch_bytes": [ci, ci, ll],
     "mvit_linear_grad": [vp, ci, vp, ll, vp],
     "mvit_linear_grad_scratch_bytes": [ci, ci, ci],
     "mvit_act_bwd_scratch_bytes": [ci, ci],

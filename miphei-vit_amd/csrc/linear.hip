@@ -9,11 +9,15 @@ namespace mvit_linear {
 template <int MODE, bool OUT32>
 int dispatch(const Args& a, bool vec, hipStream_t s);   // linear_launch.hpp
 template <int MODE>
+int dispatch_parts(const Args& a, bool vec, int kind, hipStream_t s);
+template <int MODE>
 int dispatch_grad(const Args& a, int tile, hipStream_t s);
 extern template int dispatch<H16, false>(const Args&, bool, hipStream_t);
 extern template int dispatch<H16, true>(const Args&, bool, hipStream_t);
 extern template int dispatch<F8, false>(const Args&, bool, hipStream_t);
 extern template int dispatch<F8X, true>(const Args&, bool, hipStream_t);
+extern template int dispatch_parts<H16>(const Args&, bool, int, hipStream_t);
+extern template int dispatch_parts<F8X>(const Args&, bool, int, hipStream_t);
 extern template int dispatch_grad<DX>(const Args&, int, hipStream_t);
 extern template int dispatch_grad<DW>(const Args&, int, hipStream_t);
 }  // namespace mvit_linear
@@ -37,18 +41,124 @@ int check(const mvit_linear_args* g, int es, Args& a, bool& vec) {
   if (g->res && g->ldr < g->N) return MVIT_EINVAL;
   const int ye = g->y_f32 ? 4 : 2;
   a = {(const char*)g->x, (const char*)g->w, g->bias, g->res, g->y, g->pre, g->x_scale, g->w_scale, g->res ? g->ldr : 0, (unsigned)lx, (unsigned)lw,
-       g->M, g->N, (int)kb, g->act, g->bias_f32, g->act == MVIT_ACT_RELU ? 0.f : -INFINITY, 0, 0, 1, nullptr};
+       g->M, g->N, (int)kb, g->act, g->bias_f32, g->act == MVIT_ACT_RELU ? 0.f : -INFINITY, 0, 1 << 20, 1, nullptr};
   vec = g->N % 8 == 0 && aligned16(g->y) && aligned16(g->pre) && aligned16(g->res) && (!g->res || g->ldr * ye % 16 == 0);
   return 0;
 }
 
+// Few tiles or few columns and a long K: K in parts, whose f32 products a second launch adds in order and finishes.  By what it costs, in
+// tenths of a microsecond: 40 for a round of blocks and for each of its K tiles of 128 bytes 10 and 4 with tiles of 128 x 128 and 64 x 64 (7 and 3
+// with one block a CU), 22 for every 32 of them by rows; 50 for the second launch and 8 bytes an output and part at 5 TB/s.  Taken where it
+// saves a seventh.  us without and with, W cold: bf16 [1, 16384] x
+// [512, 16384] 22 / 10, [64, 7792] x [2558, 7792] 59 / 28, the same in e4m3 34 / 19, [37, 2560] x [2044, 2560] 13 / 12
+struct Parts {
+  int kind, splits, kper;
+};
+Parts plan_parts(int M, int N, long long kb) {
+  const int cus = mvit_num_cus(), nk = (int)((kb + 127) / 128);
+  Parts best = {0, 1, 1 << 20};
+  if (nk < 8) return best;
+  const bool rows = M <= 16 || (M <= 32 && N <= 16 * cus);
+  double whole = 1e300, least = 1e300;
+  for (int kind = rows ? 0 : 2; kind <= (rows ? 0 : 3); ++kind) {
+    const int b = kind == 0 ? 16 : kind == 2 ? 128 : 64;
+    const long long tiles = (kind == 0 ? 1 : ((long long)M + b - 1) / b) * ((N + b - 1) / b);
+    const int slots = 2 * cus;
+    if (tiles > slots) return {0, 1, 1 << 20};
+    for (int want = 1; want <= 16 && tiles * want <= slots && nk >= 4 * want; ++want) {
+      const int kper = (nk + want - 1) / want, s = (nk + kper - 1) / kper;
+      double c = 40. + (kind == 0 ? 22. * ((kper + 31) / 32) : (double)kper * (kind == 2 ? (tiles * s <= cus ? 7 : 10) : (tiles * s <= cus ? 3 : 4)));
+      if (want == 1) {
+        whole = c < whole ? c : whole;
+        continue;
+      }
+      c += 50. + (double)s * M * N * (8. / 5e5);
+      if (s > 1 && c < least) least = c, best = {kind, s, kper};
+    }
+  }
+  return least * 7 < whole * 6 ? best : Parts{0, 1, 1 << 20};
+}
+long long parts_bytes(const Parts& p, int M, int N) { return p.splits > 1 ? (long long)p.splits * M * N * 4 : 0; }
+
+// y = res + act(sum of the parts + bias), 4 columns a thread
+template <bool OUT32>
+__global__ __launch_bounds__(256) void finish_parts(const Args p, const float* part, int splits) {
+  using E = End<OUT32, A_ANY, false>;
+  const int pieces = (p.N + 3) / 4;
+  const long long n = (long long)p.M * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const int row = (int)(i / pieces), col = (int)(i - (long long)row * pieces) * 4, left = p.N - col;
+    float v[4] = {};
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float* at = part + ((size_t)k * p.M + row) * p.N + col;
+      if (left >= 4) {
+        float u[4];
+        __builtin_memcpy(u, at, 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += u[e];
+      } else {
+        for (int e = 0; e < left; ++e) v[e] += at[e];
+      }
+    }
+    const size_t o = (size_t)row * p.N + col, r = (size_t)row * p.ldr + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left && p.bias) v[e] += value_of(p.bias, col + e, p.bias_f32);
+    if (p.pre) {
+      const uint32_t u[2] = {pack2bf(v[0], v[1]), pack2bf(v[2], v[3])};
+      put<E, false, 8>((bf16_t*)p.pre + o, u, left);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = activated<A_ANY>(p, v[e]);
+      if (e < left && p.res) v[e] += value_of(p.res, r + e, OUT32);
+    }
+    if constexpr (OUT32) {
+      const uint32_t u[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      put<E, true, 16>((float*)p.y + o, u, left);
+    } else {
+      const uint32_t u[2] = {pack2bf(v[0], v[1]), pack2bf(v[2], v[3])};
+      put<E, false, 8>((bf16_t*)p.y + o, u, left);
+    }
+  }
+}
+
+// MODE: the kernels whose f32 outputs are not rounded before they are added
+template <int MODE>
+int in_parts(const mvit_linear_args* g, const Args& a, const Parts& plan, hipStream_t s) {
+  Args b = a;
+  b.y = g->scratch, b.bias = b.res = nullptr, b.pre = nullptr, b.act = MVIT_ACT_NONE, b.act_lo = -INFINITY, b.kper = plan.kper, b.splits = plan.splits;
+  if (const int rc = dispatch_parts<MODE>(b, a.N % 8 == 0, plan.kind, s)) return rc;
+  const long long blocks = ((long long)a.M * ((a.N + 3) / 4) + 255) / 256, most = (long long)mvit_num_cus() * 16;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  if (g->y_f32)
+    hipLaunchKernelGGL((finish_parts<true>), grid, dim3(256), 0, s, a, (const float*)g->scratch, plan.splits);
+  else
+    hipLaunchKernelGGL((finish_parts<false>), grid, dim3(256), 0, s, a, (const float*)g->scratch, plan.splits);
+  return MVIT_LAUNCH_CHECK();
+}
+// in parts where that pays and there is room for them
+bool parts_fit(const mvit_linear_args* g, const Args& a, Parts& plan) {
+  if (!g->scratch || !aligned16(g->scratch)) return false;
+  plan = plan_parts(a.M, a.N, a.kb);
+  return plan.splits > 1 && g->scratch_bytes >= parts_bytes(plan, a.M, a.N);
+}
+
 }  // namespace
+
+extern "C" MVIT_API long long mvit_linear_scratch_bytes(int M, int N, long long k_bytes) {
+  if (M <= 0 || M > MAX_M || N <= 0 || N > MAX_N || k_bytes <= 0 || k_bytes > (1 << 23)) return 0;
+  return parts_bytes(plan_parts(M, N, k_bytes), M, N);
+}
 
 extern "C" MVIT_API int mvit_linear_act(const mvit_linear_args* args, mvit_stream_t stream) {
   MVIT_CLEAR_ERROR();
   Args a;
   bool vec;
   if (const int rc = check(args, 2, a, vec)) return rc < 0 ? rc : MVIT_OK;
+  Parts plan;
+  if (parts_fit(args, a, plan)) return in_parts<H16>(args, a, plan, (hipStream_t)stream);
   return args->y_f32 ? dispatch<H16, true>(a, vec, (hipStream_t)stream) : dispatch<H16, false>(a, vec, (hipStream_t)stream);
 }
 
@@ -58,6 +168,8 @@ extern "C" MVIT_API int mvit_linear_fp8(const mvit_linear_args* args, mvit_strea
   bool vec;
   if (const int rc = check(args, 1, a, vec)) return rc < 0 ? rc : MVIT_OK;
   if (!a.xs || !a.ws || a.pre) return MVIT_EINVAL;
+  Parts plan;
+  if (parts_fit(args, a, plan)) return in_parts<F8X>(args, a, plan, (hipStream_t)stream);
   return args->y_f32 ? dispatch<F8X, true>(a, vec, (hipStream_t)stream) : dispatch<F8, false>(a, vec, (hipStream_t)stream);
 }
 

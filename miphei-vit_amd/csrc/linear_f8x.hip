@@ -2,3 +2,4 @@
 #include "linear_launch.hpp"
 
 template int mvit_linear::dispatch<mvit_linear::F8X, true>(const mvit_linear::Args&, bool, hipStream_t);
+template int mvit_linear::dispatch_parts<mvit_linear::F8X>(const mvit_linear::Args&, bool, int, hipStream_t);

@@ -38,9 +38,9 @@ struct Args {
   int M, N, kb;      // kb: bytes of a row of x and W
   int act, bias_f32;
   float act_lo;   // -inf, or 0 for relu
-  // DX, DW: rows of the operands whose rows are K; K tiles of a split and splits; their products f32 [splits][M][N] where there is more than one
-  int krows, kper, splits;
-  float* part;
+  int krows;         // DX, DW: rows of the operands whose rows are K
+  int kper, splits;  // K tiles of a part of K, and parts; their products f32 [splits][M][N] where there is more than one:
+  float* part;       // DX, DW: here, else in y (f32)
 };
 
 // What a tile kernel is compiled for besides its operands.  The epilogue is unrolled over the accumulators: with every activation and
@@ -181,10 +181,10 @@ __device__ __forceinline__ uint4 finish(const Args& p, float (&v)[W], int row, i
   }
 }
 template <class E>
-__device__ __forceinline__ void store_piece(const Args& p, int row, int col, const uint4& u) {
+__device__ __forceinline__ void store_piece(const Args& p, int part, int row, int col, const uint4& u) {   // of part `part` of K
   if (row < p.M && col < p.N) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    put<E, E::out32, 16>((char*)p.y + ((size_t)row * p.N + col) * (E::out32 ? 4 : 2), w, p.N - col);
+    put<E, E::out32, 16>((char*)p.y + (((size_t)part * p.M + row) * p.N + col) * (E::out32 ? 4 : 2), w, p.N - col);
   }
 }
 
@@ -280,15 +280,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
   const int wm = wave / WN, wn = wave % WN;
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, nt = tm * tn;
   const int nk = (p.kb + BKB - 1) / BKB;
-  // DX, DW: number v is split v / nt of tile v % nt; the K tiles [first, end) of a number
-  const int nv = T::WR ? nt * p.splits : nt;
-  auto first_k = [&](int v) __attribute__((always_inline)) { return T::WR ? v / nt * p.kper : 0; };
-  auto end_k = [&](int v) __attribute__((always_inline)) { return T::WR ? min(nk, (v / nt + 1) * p.kper) : nk; };
+  // K in parts: number v is part v / nt of tile v % nt, K tiles [first, end)
+  constexpr bool PARTS = T::WR || (E::out32 && E::act == A_CLIP);
+  const int nv = PARTS ? nt * p.splits : nt;
+  auto first_k = [&](int v) __attribute__((always_inline)) { return PARTS ? v / nt * p.kper : 0; };
+  auto end_k = [&](int v) __attribute__((always_inline)) { return PARTS ? min(nk, (v / nt + 1) * p.kper) : nk; };
 
   // tile number -> place: blocks go to the eight XCDs in turn, so the numbers of one XCD are put on one contiguous run of tiles, and runs
   // go down 8 rows of tiles before the next column: the blocks that share an L2 share rows of x and of W
   auto place = [&](int v, int& m0, int& n0) __attribute__((always_inline)) {
-    if constexpr (T::WR) v %= nt;
+    if constexpr (PARTS) v %= nt;
     const int q = nt >> 3, r = nt & 7, xcd = v & 7;
     const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (v >> 3);
     const int per = 8 * tn, g0 = id / per * 8, gsz = min(tm - g0, 8), in = id % per;
@@ -499,13 +500,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
           const acc_t &c0 = acc[i][j], &c1 = acc[i][j + 1];
           const auto lo = __builtin_amdgcn_permlane16_swap(pack2bf(c0[0], c0[1]), pack2bf(c1[0], c1[1]), false, false);
           const auto hi = __builtin_amdgcn_permlane16_swap(pack2bf(c0[2], c0[3]), pack2bf(c1[2], c1[3]), false, false);
-          store_piece<E>(p, m0 + wm * T::WTM + i * 16 + fr, n0 + wn * T::WTN + (j + (fh & 1)) * 16 + (fh >> 1) * 8, make_uint4(lo[0], hi[0], lo[1], hi[1]));
+          store_piece<E>(p, 0, m0 + wm * T::WTM + i * 16 + fr, n0 + wn * T::WTN + (j + (fh & 1)) * 16 + (fh >> 1) * 8, make_uint4(lo[0], hi[0], lo[1], hi[1]));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       constexpr int W = E::out32 ? 4 : 8, NP = T::TN * AR / W;   // pieces of a lane in one row of fragments
-      const int row0 = m0 + wm * T::WTM + fr, col0 = n0 + wn * T::WTN;
+      const int row0 = m0 + wm * T::WTM + fr, col0 = n0 + wn * T::WTN, part = PARTS ? v / nt : 0;
       auto col_of = [&](int q) __attribute__((always_inline)) {
         return col0 + (PAIRED ? q * 32 + fh * 8 : WIDE ? (q >> 1) * 32 + (q & 1) * 16 + fh * 8 : q * 16 + fh * 4);
       };
@@ -549,7 +550,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
           for (int e = 0; e < W; ++e)
             o[e] = (WIDE ? acc[i][q >> 1][(q & 1) * 8 + e] : PAIRED ? acc[i][q * 2 + (e >> 2)][e & 3] : acc[i][q][e & 3]) * (OP8 ? rs[i] : 1.f);
           out[q] = finish<OP8, E, W>(p, o, row, col_of(q), cols[q], res[i & 1][q]);
-          if constexpr (!WIDE) store_piece<E>(p, row, col_of(q), out[q]);
+          if constexpr (!WIDE) store_piece<E>(p, part, row, col_of(q), out[q]);
         }
         if constexpr (WIDE) {
           // two lanes of a row, 32 bytes a store: trade pieces between rows r and r + 16, so that four lanes have 64 bytes of one row
@@ -562,8 +563,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile(const Args p) {
               a[e] = s[0], b[e] = s[1];
             }
             const int r = row - fr + (lane & 15), c = col0 + (q >> 1) * 32 + ((lane >> 4) & 1) * 16 + (lane >> 5) * 8;
-            store_piece<E>(p, r, c, out[q]);
-            store_piece<E>(p, r + 16, c, out[q + 1]);
+            store_piece<E>(p, part, r, c, out[q]);
+            store_piece<E>(p, part, r + 16, c, out[q + 1]);
           }
         }
         __builtin_amdgcn_sched_barrier(0);   // (rows of fragments pulled together cost registers that are not there)
@@ -594,15 +595,15 @@ __global__ __launch_bounds__(512) void linear_rows(const Args p) {
   f32x4 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  const int np = (p.kb + 127) / 128;
-  for (int k0 = wave; k0 < np; k0 += NWV * U) {
+  const int part_k = blockIdx.y, np = min((p.kb + 127) / 128, (part_k + 1) * p.kper);   // this block's part of K: pieces [kper part_k, np)
+  for (int k0 = part_k * p.kper + wave; k0 < np; k0 += NWV * U) {
     i32x4 b[U][2], a[U][MT][2];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int k = (k0 + u * NWV) * 128 + fh * 32 + c * 16;
-        const bool ok = k < p.kb;
+        const bool ok = k < p.kb && k0 + u * NWV < np;
         b[u][c] = __builtin_amdgcn_raw_buffer_load_b128(rw, ok ? wo + k : OOB, 0, 0);
 #pragma unroll
         for (int m = 0; m < MT; ++m) a[u][m][c] = __builtin_amdgcn_raw_buffer_load_b128(rx, ok ? xo[m] + k : OOB, 0, 0);
@@ -646,7 +647,7 @@ __global__ __launch_bounds__(512) void linear_rows(const Args p) {
       for (int k = 1; k < NWV; ++k) v[e] += part[k][row][c0 + e];
       if constexpr (OP8) v[e] *= p.xs[row];
     }
-    store_piece<E>(p, row, col, finish<OP8, E, W>(p, v, row, col, cols, res));
+    store_piece<E>(p, part_k, row, col, finish<OP8, E, W>(p, v, row, col, cols, res));
   }
 }
 

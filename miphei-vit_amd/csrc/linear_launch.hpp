@@ -8,7 +8,7 @@ namespace mvit_linear {
 template <int MODE, class E, int BM, int BN, int WM, int WN, int NST>
 int launch_tile(const Args& a, hipStream_t s) {
   using T = Tile<MODE, BM, BN, WM, WN, NST>;
-  const long long nt = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN) * (T::WR ? a.splits : 1);
+  const long long nt = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN) * a.splits;
   if (nt > 0x7fffffff) return MVIT_EINVAL;
   static mvit_per_device_size raised;
   const auto fn = linear_tile<MODE, E, BM, BN, WM, WN, NST>;
@@ -20,7 +20,7 @@ int launch_tile(const Args& a, hipStream_t s) {
 
 template <bool OP8, class E, int MT>
 int launch_rows(const Args& a, hipStream_t s) {
-  hipLaunchKernelGGL((linear_rows<OP8, E, MT>), dim3((a.N + 15) / 16), dim3(512), 0, s, a);
+  hipLaunchKernelGGL((linear_rows<OP8, E, MT>), dim3((a.N + 15) / 16, a.splits), dim3(512), 0, s, a);
   return MVIT_LAUNCH_CHECK();
 }
 
@@ -91,6 +91,18 @@ int by_activation(const Args& a, hipStream_t s) {
     default:
       return by_size<MODE, End<OUT32, A_TANH, VEC>>(a, s);
   }
+}
+// The products of parts of K, f32 (plan_parts in linear.hip): kind 0 by rows, else tiles of 128 x 128 (2) or 64 x 64 (3)
+template <int MODE, bool VEC>
+int parts_of(const Args& a, int kind, hipStream_t s) {
+  using Any = End<true, A_ANY, VEC>;
+  using Sum = End<true, A_CLIP, VEC>;
+  if (kind == 0) return a.M <= 16 ? launch_rows<MODE != H16, Any, 1>(a, s) : launch_rows<MODE != H16, Any, 2>(a, s);
+  return kind == 2 ? launch_tile<MODE, Sum, 128, 128, 2, 2, 2>(a, s) : launch_tile<MODE, Sum, 64, 64, 2, 2, 4>(a, s);
+}
+template <int MODE>
+int dispatch_parts(const Args& a, bool vec, int kind, hipStream_t s) {
+  return vec ? parts_of<MODE, true>(a, kind, s) : parts_of<MODE, false>(a, kind, s);
 }
 template <int MODE, bool OUT32>
 int dispatch(const Args& a, bool vec, hipStream_t s) {

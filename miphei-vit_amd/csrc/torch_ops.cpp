@@ -46,6 +46,7 @@ struct Lib {
   MVIT_FN(mvit_linear_fp8);
   MVIT_FN(mvit_act_bwd_scratch_bytes);
   MVIT_FN(mvit_act_bwd);
+  MVIT_FN(mvit_linear_scratch_bytes);
   MVIT_FN(mvit_linear_grad_scratch_bytes);
   MVIT_FN(mvit_linear_grad);
 #undef MVIT_FN
@@ -404,6 +405,9 @@ void product(const Lib& l, const Tensor& x, const Tensor& w, const OptTensor& bi
   a.x = x.const_data_ptr(), a.w = w.const_data_ptr(), a.bias = ptr(bias), a.res = ptr(res), a.y = y.mutable_data_ptr(), a.pre = pre;
   a.x_scale = xs, a.w_scale = ws, a.ldx = ld(x), a.ldw = ld(w), a.ldr = res ? ld(*res) : 0;
   a.M = (int)M, a.N = (int)N, a.K = (int)x.size(1), a.act = act, a.bias_f32 = f32(bias), a.y_f32 = f32(y);
+  a.scratch_bytes = l.mvit_linear_scratch_bytes(a.M, a.N, x.size(1) * x.element_size());
+  const Tensor s = a.scratch_bytes ? scratch(y, a.scratch_bytes) : Tensor();
+  if (a.scratch_bytes) a.scratch = s.mutable_data_ptr();
   if (xs)
     ok(l.mvit_linear_fp8(&a, st), "mvit_linear_fp8");
   else
@@ -713,6 +717,7 @@ extern "C" __attribute__((visibility("default"))) const char* mvit_torch_bind(co
     MVIT_FN(mvit_linear_fp8);
     MVIT_FN(mvit_act_bwd_scratch_bytes);
     MVIT_FN(mvit_act_bwd);
+    MVIT_FN(mvit_linear_scratch_bytes);
     MVIT_FN(mvit_linear_grad_scratch_bytes);
     MVIT_FN(mvit_linear_grad);
 #undef MVIT_FN

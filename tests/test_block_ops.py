@@ -1185,3 +1185,43 @@ def test_linear_act_gradients_of_odd_upstream_layouts(N, act):
     row = dy[:1].expand(M, N)
     for u, v in zip(torch.autograd.grad(y, (x, w, b), row, retain_graph=True), torch.autograd.grad(y, (x, w, b), row.contiguous())):
         assert torch.equal(u, v)
+
+
+LONG_K = [(1, 16384, 512), (1, 16384, 509), (16, 32768, 70), (17, 32768, 136), (30, 16384, 45), (37, 2560, 2044), (64, 7792, 2558), (100, 8192, 64), (33, 4096, 33)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("res", ["none", "half", "f32"])
+@pytest.mark.parametrize("M,K,N", LONG_K)
+def test_linear_of_a_long_k(M, K, N, res):
+    """few rows and a long K, taken in parts: with a bias, every activation, residuals with strides, the kept pre-activation; twice the same"""
+    ops, g = T(), gen(M + K + N)
+    dtype = HALF[(M + N) % 2]
+    act = ACTS[(M + len(res)) % 5]
+    rt = {"none": None, "half": dtype, "f32": torch.float32}[res]
+    x, w, b, r = linear_case(g, M, K, N, dtype, rt, bool(N % 2))
+    if r is not None:
+        wide = torch.zeros(M, N + 3, device="cuda", dtype=rt)
+        wide[:, 1:N + 1] = r
+        r = wide[:, 1:N + 1]
+    z = x.double() @ w.double().t() + b.double()
+    mag = x.double().abs() @ w.double().abs().t() + b.double().abs()
+    rd = torch.zeros_like(z) if r is None else r.double()
+    y = ops.linear_act(x, w, b, r, act)
+    close(y, act_oracle(z, act)[0] + rd, 1.2 * mag + rd.abs(), "y")
+    assert torch.equal(y, ops.linear_act(x, w, b, r, act))
+    out, pre = torch.ops.mvit.linear_act_forward(x, w, b, r, act, True)
+    close(pre, z, mag, "pre")
+    assert torch.equal(out, y)
+    xs, ws = (t.float().abs().amax(-1) / 448 for t in (x, w))          # (rows longer than quantize_fp8 takes)
+    xq, wq = ((t.float() / s[:, None]).to(torch.float8_e4m3fn) for t, s in ((x, xs), (w, ws)))
+    xd, wd = xq.double() * xs.double()[:, None], wq.double() * ws.double()[:, None]
+    z, mag = xd @ wd.t() + b.double(), xd.abs() @ wd.abs().t() + b.double().abs()
+    close(ops.linear_fp8(xq, xs, wq, ws, b, r, act, dtype), act_oracle(z, act)[0] + rd, 1.2 * mag + rd.abs(), "fp8", F32 if res == "f32" else F8)
+
+
+def test_room_for_parts():
+    from miphei_vit_amd import _lib
+    lib = _lib.lib()
+    assert lib.mvit_linear_scratch_bytes(1, 512, 32768) > 0 == lib.mvit_linear_scratch_bytes(1, 1536, 3072) == lib.mvit_linear_scratch_bytes(5264, 4096, 3072)
+    assert lib.mvit_linear_scratch_bytes(0, 512, 32768) == lib.mvit_linear_scratch_bytes(1, 512, 1 << 24) == 0
