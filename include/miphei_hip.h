@@ -170,8 +170,8 @@ MVIT_API int mvit_attention_bwd(const void* qkv, const void* out, const void* ou
 /* Root-mean-square norm of a residual stream.  h = x + res (kept in res's type; what is normed is h as it is stored),
  * y = h / sqrt(mean(h^2) + eps) * w, rstd(f32)[M] (optional) = 1 / sqrt(...) for the backward pass.  *_f32 != 0: that operand is f32,
  * else 16-bit; row strides ldx, ldr in elements, h and y are dense [M, D].  res = NULL: h is x and is not written.
- * x 16-bit: res 16-bit or f32, y 16-bit.  x f32: res f32, y 16-bit or f32.  1 <= D <= 16384, M <= 2^30, any D and any alignment (16-byte loads
- * where D % 8 == 0 and all rows start on 16 bytes). */
+ * x 16-bit: res 16-bit or f32, y 16-bit.  x f32: res f32, y 16-bit or f32.  1 <= D <= 16384, M <= 2^30, any D and any alignment (fastest where
+ * D % 8 == 0 and all rows start on 16 bytes). */
 MVIT_API int mvit_rmsnorm_fwd(const void* x, int x_f32, long long ldx, const void* res, int res_f32, long long ldr, const void* w,
                               int w_f32, void* h, void* y, int y_f32, float* rstd, int M, int D, float eps, mvit_stream_t stream);
 /* The same with y in 8 bits: scale(f32)[M] = max(max |y|, 1e-30) / 448, q(e4m3)[M, D] = y / scale rounded to nearest even.  A row with

@@ -9,9 +9,9 @@
 // are formed, and is written once.
 //  * A row belongs to TPR = 64 threads (one wave: no barrier) or to a block (fewer registers and loads a thread: for wide rows, and for
 //    few, whose latency counts).
-//  * Each thread holds NV pieces of 8 values (16-byte loads); where D, a row stride or an address is odd the loads go to odd addresses and a
-//    row's last piece goes by elements (ODD), us with elements before and so: 8 bits
-//    of an f32 stream [16623, 1053] 106 / 46, [2032, 7956] 257 / 40
+//  * Each thread holds NV pieces of 8 values (16-byte loads).  Where D is no multiple of 8, or a row starts off 16 bytes (ODD), they go to odd
+//    addresses and a row's last piece goes by elements; with all of it by elements an f32 stream of [16623, 1053] to 8 bits took 106 us
+//    instead of 46, of [2032, 7956] 257 instead of 40.
 //  * Rows are walked with a grid stride, so that w is loaded once per thread and not once per row.
 // Measured against a 1 GiB copy's 5.05 TB/s (one MI355X): f32 stream of [21056, 1536] forward 75 us (388 MB, 5.2 TB/s), backward with
 // d w 96 us (517 MB, 5.4 TB/s); 16-bit stream to 8 bits [20816, 1536] 37 us (6.0 TB/s); quantisation [21056, 4096] 43 us (6.0 TB/s).
@@ -360,7 +360,7 @@ int fwd_layout(const RowArgs& a, bool even, hipStream_t s) {
   return even ? fwd_layout<false, XT, RT, YT, NORM>(a, s) : fwd_layout<true, XT, RT, YT, NORM>(a, s);
 }
 
-// vector loads: every row of every operand starts on 16 bytes (8 for the e4m3 output, whose rows are D bytes)
+// every row of every operand starts on 16 bytes (8 for the e4m3 output, whose rows are D bytes)
 bool vec_ok(const RowArgs& a) {
   return a.D % 8 == 0 && a.ldx % 8 == 0 && (!a.res || a.ldr % 8 == 0) && aligned16(a.x) && aligned16(a.res) && aligned16(a.h) && aligned16(a.y) &&
          aligned16(a.w);
