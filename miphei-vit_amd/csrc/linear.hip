@@ -48,9 +48,9 @@ int check(const mvit_linear_args* g, int es, Args& a, bool& vec) {
 
 // Few tiles or few columns and a long K: K in parts, whose f32 products a second launch adds in order and finishes.  By what it costs, in
 // tenths of a microsecond: 40 for a round of blocks and for each of its K tiles of 128 bytes 10 and 4 with tiles of 128 x 128 and 64 x 64 (7 and 3
-// with one block a CU), 22 for every 32 of them by rows; 50 for the second launch and 8 bytes an output and part at 5 TB/s.  Taken where it
-// saves a seventh.  us without and with, W cold: bf16 [1, 16384] x
-// [512, 16384] 22 / 10, [64, 7792] x [2558, 7792] 59 / 28, the same in e4m3 34 / 19, [37, 2560] x [2044, 2560] 13 / 12
+// with one block a CU), 22 for every 32 of them by rows; 50 for the second launch and 8 bytes an output and part at 5 TB/s.  Taken where that
+// says a quarter less (at a seventh, [134, 2352] x [395, 2352] lost 1 us).  us without and with: bf16 [1, 16384] x [512, 16384] 22 / 10,
+// [64, 7792] x [2558, 7792] 35 / 21, the same in e4m3 20 / 16, [66, 6784] x [146, 6784] 25 / 14, [37, 2560] x [2044, 2560] 11.4 / 9.0
 struct Parts {
   int kind, splits, kper;
 };
@@ -76,44 +76,59 @@ Parts plan_parts(int M, int N, long long kb) {
       if (s > 1 && c < least) least = c, best = {kind, s, kper};
     }
   }
-  return least * 7 < whole * 6 ? best : Parts{0, 1, 1 << 20};
+  return least < whole * 0.73 ? best : Parts{0, 1, 1 << 20};
 }
 long long parts_bytes(const Parts& p, int M, int N) { return p.splits > 1 ? (long long)p.splits * M * N * 4 : 0; }
 
-// y = res + act(sum of the parts + bias), 4 columns a thread
+// Sum of `splits` groups of 4 values, `stride` apart, in order; eight of them on their way at a time (f32, at any 4-byte address)
+__device__ __forceinline__ f32x4 sum_of_parts(const float* at, size_t stride, int splits) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < splits; k += 8) {
+    f32x4 u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) __builtin_memcpy(&u[j], at + (size_t)min(k + j, splits - 1) * stride, 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < splits) s += u[j];
+  }
+  return s;
+}
+
+// y = res + act(sum of the parts + bias), 4 columns a thread, 64 threads by 4 rows a block
 template <bool OUT32>
 __global__ __launch_bounds__(256) void finish_parts(const Args p, const float* part, int splits) {
   using E = End<OUT32, A_ANY, false>;
-  const int pieces = (p.N + 3) / 4;
-  const long long n = (long long)p.M * pieces;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const int row = (int)(i / pieces), col = (int)(i - (long long)row * pieces) * 4, left = p.N - col;
-    float v[4] = {};
-#pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      const float* at = part + ((size_t)k * p.M + row) * p.N + col;
-      if (left >= 4) {
-        float u[4];
-        __builtin_memcpy(u, at, 16);
+  const int col = (blockIdx.x * 64 + threadIdx.x) * 4, left = p.N - col;
+  if (left <= 0) return;
+  float bias[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += u[e];
-      } else {
-        for (int e = 0; e < left; ++e) v[e] += at[e];
-      }
+  for (int e = 0; e < 4; ++e) bias[e] = p.bias && e < left ? value_of(p.bias, col + e, p.bias_f32) : 0.f;
+  for (int row = blockIdx.y * 4 + threadIdx.y; row < p.M; row += gridDim.y * 4) {
+    float v[4] = {}, res[4] = {};
+    const float* at = part + (size_t)row * p.N + col;
+    if (p.res)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) res[e] = value_of(p.res, (size_t)row * p.ldr + col + e, OUT32);
+    if (left >= 4) {
+      const f32x4 s = sum_of_parts(at, (size_t)p.M * p.N, splits);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = s[e];
+    } else {
+      for (int k = 0; k < splits; ++k)
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < left) v[e] += at[(size_t)k * p.M * p.N + e];
     }
-    const size_t o = (size_t)row * p.N + col, r = (size_t)row * p.ldr + col;
+    const size_t o = (size_t)row * p.N + col;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < left && p.bias) v[e] += value_of(p.bias, col + e, p.bias_f32);
+    for (int e = 0; e < 4; ++e) v[e] += bias[e];
     if (p.pre) {
       const uint32_t u[2] = {pack2bf(v[0], v[1]), pack2bf(v[2], v[3])};
       put<E, false, 8>((bf16_t*)p.pre + o, u, left);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = activated<A_ANY>(p, v[e]);
-      if (e < left && p.res) v[e] += value_of(p.res, r + e, OUT32);
-    }
+    for (int e = 0; e < 4; ++e) v[e] = activated<A_ANY>(p, v[e]) + res[e];
     if constexpr (OUT32) {
       const uint32_t u[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
       put<E, true, 16>((float*)p.y + o, u, left);
@@ -130,12 +145,12 @@ int in_parts(const mvit_linear_args* g, const Args& a, const Parts& plan, hipStr
   Args b = a;
   b.y = g->scratch, b.bias = b.res = nullptr, b.pre = nullptr, b.act = MVIT_ACT_NONE, b.act_lo = -INFINITY, b.kper = plan.kper, b.splits = plan.splits;
   if (const int rc = dispatch_parts<MODE>(b, a.N % 8 == 0, plan.kind, s)) return rc;
-  const long long blocks = ((long long)a.M * ((a.N + 3) / 4) + 255) / 256, most = (long long)mvit_num_cus() * 16;
-  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  const int row_blocks = (a.M + 3) / 4;
+  const dim3 grid((a.N + 255) / 256, row_blocks < 4096 ? row_blocks : 4096);
   if (g->y_f32)
-    hipLaunchKernelGGL((finish_parts<true>), grid, dim3(256), 0, s, a, (const float*)g->scratch, plan.splits);
+    hipLaunchKernelGGL((finish_parts<true>), grid, dim3(64, 4), 0, s, a, (const float*)g->scratch, plan.splits);
   else
-    hipLaunchKernelGGL((finish_parts<false>), grid, dim3(256), 0, s, a, (const float*)g->scratch, plan.splits);
+    hipLaunchKernelGGL((finish_parts<false>), grid, dim3(64, 4), 0, s, a, (const float*)g->scratch, plan.splits);
   return MVIT_LAUNCH_CHECK();
 }
 // in parts where that pays and there is room for them
@@ -211,9 +226,7 @@ long long split_bytes(const Plan& p, int M, int N) { return p.splits > 1 ? (long
 // 4 outputs a thread
 __global__ __launch_bounds__(256) void sum_splits(const float* part, bf16_t* y, int splits, long long n4) {
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
-    f32x4 s = *(const f32x4*)(part + i * 4);
-#pragma unroll 4
-    for (int k = 1; k < splits; ++k) s += *(const f32x4*)(part + (k * n4 + i) * 4);
+    const f32x4 s = sum_of_parts(part + i * 4, (size_t)n4 * 4, splits);
     *(uint2*)(y + i * 4) = make_uint2(pack2bf(s[0], s[1]), pack2bf(s[2], s[3]));
   }
 }
