@@ -7,9 +7,9 @@
 // and every measurement of round 5 says the loop is paced by the bytes a CU moves per flop, not by the matrix pipe: per K tile the
 // eight 64x64 waves read 128 KB of fragments from LDS (each A row block twice, each B column block four times) beside the 48 KB the
 // DMA writes.  A 128x64 sub-tile reads (128 + 64) x 128 B = 24 KB per wave, 96 KB per K tile (-25 %), and 8 instead of 12 waves meet
-// in the K-tile barrier.  The price is one MFMA stream per SIMD (no partner wave to fill its bubbles) -- which is why the vendor's
-// 256x128 kernel has this shape and why this file exists as a measured alternative, selected per problem by the dispatcher
-// (mvit_gemm::ws4_supported; MVIT_GEMM_WS4 in the dbg library).
+// in the K-tile barrier.  The price is one MFMA stream per SIMD (no partner wave to fill its bubbles), and it is the larger: proj 26.2
+// against 24.2 us, qkv 72.9 against 69.5, fc2 61.0 against 58.6.  Kept as a measured alternative in the dbg library only, selected per
+// problem by the dispatcher (mvit_gemm::ws4_supported; MVIT_GEMM_WS4).
 #include <type_traits>
 #include "common.hpp"
 #include "../../include/miphei_hip.h"
