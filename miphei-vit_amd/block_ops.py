@@ -7,6 +7,9 @@ functions below are their entry points, re-exported by ``torch_ops``.  CUDA (ROC
 the tensors are (fp16 runs in libmiphei_hip_f16.so), never a mixture; the work goes to the tensors' device, on its current stream.  Wrong
 arguments raise ValueError.
 
+Their gradients are those of a backward pass, once.  Forward-mode tangents and functional gradient transforms (torch.func.grad, vjp, jvp) are
+refused by all of them, not dropped; torch.vmap runs those without a gradient an entry at a time.
+
 All of them can be captured into a graph, forward and backward; as with any backward pass, let no eager graph over the same leaves live
 while one is captured (delete its outputs first): its accumulation nodes belong to the eager stream.
 

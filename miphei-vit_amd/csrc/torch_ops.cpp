@@ -86,10 +86,22 @@ void same_place(const char* op, const Tensor& x, const OptTensor& y) {
   REQUIRE(!y || y->device() == x.device(), op, "tensors on ", x.device(), " and ", y->device());
 }
 
-void no_grad(const char* op, std::initializer_list<OptTensor> ts) {
-  if (!at::GradMode::is_enabled()) return;
+// A derivative is never dropped: what carries a forward-mode tangent (torch.no_grad() does not stop those) is refused, and so is, by operators
+// without a gradient, what requires one.  Asked in the autograd kernels, where functional transforms have their tensors still wrapped.
+bool has_tangent(const OptTensor& t) { return t && t->defined() && t->_fw_grad(/*level=*/0).defined(); }
+void no_tangent(const char* op, std::initializer_list<OptTensor> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const auto& t : ts) TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), "mvit::", op, " has no forward-mode derivative");
+}
+bool wants_grad(std::initializer_list<OptTensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
   for (const auto& t : ts)
-    TORCH_CHECK(!t || !t->requires_grad(), "mvit::", op, " has no gradient: call it under torch.no_grad() or on detached tensors");
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+void no_grad(const char* op, std::initializer_list<OptTensor> ts) {
+  no_tangent(op, ts);
+  TORCH_CHECK(!wants_grad(ts), "mvit::", op, " has no gradient: call it under torch.no_grad() or on detached tensors");
 }
 
 constexpr int64_t ROWS_MAX = 1 << 30;
@@ -222,7 +234,6 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_backward_meta(const Tensor&, const O
 }
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps) {
-  no_grad("rms_norm_fp8", {x, residual, weight});
   const HalfType h = norm_check("rms_norm_fp8", x, residual, weight, std::nullopt);
   c10::DeviceGuard guard(x.device());
   NormOut o = norm_out(x, residual, at::kFloat8_e4m3fn);
@@ -247,7 +258,6 @@ HalfType quantize_check(const Tensor& x) {
   return h;
 }
 std::tuple<Tensor, Tensor> quantize_fp8(const Tensor& x) {
-  no_grad("quantize_fp8", {x});
   const HalfType h = quantize_check(x);
   c10::DeviceGuard guard(x.device());
   NormOut o = norm_out(x, std::nullopt, at::kFloat8_e4m3fn);
@@ -350,7 +360,6 @@ void rotary_check_(const Tensor& x) {
 }
 void rotary_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix,
              bool interleaved) {
-  no_grad("rotary_", {x, positions, inv_freq});
   const HalfType h = rotary_check("rotary_", x, positions, inv_freq, sections, rotate_heads, num_prefix);
   rotary_check_(x);
   c10::DeviceGuard guard(x.device());
@@ -508,7 +517,6 @@ int linear_fp8_check(const Tensor& x, const Tensor& x_scale, const Tensor& weigh
 }
 Tensor linear_fp8(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& w_scale, const OptTensor& bias, const OptTensor& residual,
                   c10::string_view act, ScalarType out_dtype) {
-  no_grad("linear_fp8", {x_scale, w_scale, bias, residual});
   HalfType h{"linear_fp8"};
   const int code = linear_fp8_check(x, x_scale, weight, w_scale, bias, residual, act, out_dtype, h);
   c10::DeviceGuard guard(x.device());
@@ -554,12 +562,6 @@ const auto& linear_backward_op() {
   return h;
 }
 
-bool wants_grad(std::initializer_list<OptTensor> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const auto& t : ts)
-    if (t && t->requires_grad()) return true;
-  return false;
-}
 OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
@@ -597,6 +599,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 };
 std::tuple<Tensor, Tensor, Tensor> rms_norm_forward_autograd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps,
                                                              std::optional<ScalarType> out_dtype) {
+  no_tangent("rms_norm", {x, residual, weight});
   if (wants_grad({x, residual, weight})) {
     auto o = RmsNorm::apply(x, residual, weight, eps, out_dtype);
     return {o[0], o[1], o[2]};
@@ -629,6 +632,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 };
 Tensor rotary_forward_autograd(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads,
                                int64_t num_prefix, bool interleaved, bool inverse) {
+  no_tangent("rotary", {x, positions, inv_freq});
   TORCH_CHECK(!wants_grad({positions, inv_freq}), "mvit::rotary has no gradient of positions and inv_freq: detach them");
   if (wants_grad({x})) return Rotary::apply(x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved, inverse);
   at::AutoDispatchBelowAutograd below;
@@ -672,6 +676,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 };
 std::tuple<Tensor, Tensor> linear_act_forward_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                                                        c10::string_view act, bool save_pre) {
+  no_tangent("linear_act", {x, weight, bias, residual});
   if (wants_grad({x, weight, bias, residual})) {
     auto o = LinearAct::apply(x, weight, bias, residual, std::string(act));
     return {o[0], o[1]};
@@ -684,15 +689,45 @@ std::tuple<Tensor, Tensor> linear_act_forward_autograd(const Tensor& x, const Te
 std::tuple<Tensor, Tensor, Tensor> rms_norm_backward_autograd(const Tensor& dy, const OptTensor& dh, const Tensor& h, const Tensor& weight,
                                                               const Tensor& rstd, ScalarType x_dtype, bool need_x, bool need_residual,
                                                               bool need_weight) {
+  no_tangent("rms_norm_backward", {dy, dh, h, weight});
   TORCH_CHECK(!wants_grad({dy, dh, h, weight}), "mvit::rms_norm is differentiable once");
   at::AutoDispatchBelowAutograd below;
   return rms_backward_op().call(dy, dh, h, weight, rstd, x_dtype, need_x, need_residual, need_weight);
 }
 std::tuple<Tensor, Tensor, Tensor> linear_act_backward_autograd(const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& pre,
                                                                 c10::string_view act, bool need_x, bool need_w, bool need_b, ScalarType bias_dtype) {
+  no_tangent("linear_act_backward", {dy, x, weight});
   TORCH_CHECK(!wants_grad({dy, x, weight}), "mvit::linear_act is differentiable once");
   at::AutoDispatchBelowAutograd below;
   return linear_backward_op().call(dy, x, weight, pre, act, need_x, need_w, need_b, bias_dtype);
+}
+
+// the operators without a gradient
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8_autograd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps) {
+  static const auto h = op<decltype(rms_norm_fp8)>("mvit::rms_norm_fp8");
+  no_grad("rms_norm_fp8", {x, residual, weight});
+  at::AutoDispatchBelowAutograd below;
+  return h.call(x, residual, weight, eps);
+}
+std::tuple<Tensor, Tensor> quantize_fp8_autograd(const Tensor& x) {
+  static const auto h = op<decltype(quantize_fp8)>("mvit::quantize_fp8");
+  no_grad("quantize_fp8", {x});
+  at::AutoDispatchBelowAutograd below;
+  return h.call(x);
+}
+void rotary_autograd_(Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, int64_t rotate_heads, int64_t num_prefix,
+                      bool interleaved) {
+  static const auto h = op<decltype(rotary_)>("mvit::rotary_");
+  no_grad("rotary_", {x, positions, inv_freq});
+  at::AutoDispatchBelowAutograd below;
+  h.call(x, positions, inv_freq, sections, rotate_heads, num_prefix, interleaved);
+}
+Tensor linear_fp8_autograd(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& w_scale, const OptTensor& bias,
+                           const OptTensor& residual, c10::string_view act, ScalarType out_dtype) {
+  static const auto h = op<decltype(linear_fp8)>("mvit::linear_fp8");
+  no_grad("linear_fp8", {x, x_scale, weight, w_scale, bias, residual});
+  at::AutoDispatchBelowAutograd below;
+  return h.call(x, x_scale, weight, w_scale, bias, residual, act, out_dtype);
 }
 
 }  // namespace
@@ -770,5 +805,8 @@ TORCH_LIBRARY_IMPL(mvit, Autograd, m) {
   m.impl("rotary_forward", rotary_forward_autograd);
   m.impl("linear_act_forward", linear_act_forward_autograd);
   m.impl("linear_act_backward", linear_act_backward_autograd);
-  for (const char* name : {"rms_norm_fp8", "quantize_fp8", "rotary_", "linear_fp8"}) m.impl(name, torch::CppFunction::makeFallthrough());
+  m.impl("rms_norm_fp8", rms_norm_fp8_autograd);
+  m.impl("quantize_fp8", quantize_fp8_autograd);
+  m.impl("rotary_", rotary_autograd_);
+  m.impl("linear_fp8", linear_fp8_autograd);
 }

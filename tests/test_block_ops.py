@@ -1225,3 +1225,73 @@ def test_room_for_parts():
     lib = _lib.lib()
     assert lib.mvit_linear_scratch_bytes(1, 512, 32768) > 0 == lib.mvit_linear_scratch_bytes(1, 1536, 2 * 1536) == lib.mvit_linear_scratch_bytes(5264, 4096, 2 * 1536)
     assert lib.mvit_linear_scratch_bytes(0, 512, 32768) == lib.mvit_linear_scratch_bytes(1, 512, 1 << 24) == 0
+
+
+# ------------------------------------------------------------------ derivatives of other kinds
+def derivative_calls(device):
+    """name -> (function of one tensor, that tensor); shapes only where the device is meta"""
+    ops, f32, f8 = T(), torch.float32, torch.float8_e4m3fn
+    make = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
+    w, p, fr = make(64, dtype=f32), make(4, 1, dtype=torch.int32), make(8, dtype=f32)
+    x, lw, q, wq = make(4, 64), make(32, 64), make(4, 64, dtype=f8), make(32, 64, dtype=f8)
+    s, ws = make(4, dtype=f32), make(32, dtype=f32)
+    return {
+        "rms_norm": (lambda x: ops.rms_norm(x, w), x), "rms_norm weight": (lambda w: ops.rms_norm(x, w), w),
+        "add_rms_norm residual": (lambda r: ops.add_rms_norm(x, r, w)[1], x), "linear_act": (lambda x: ops.linear_act(x, lw), x),
+        "linear_act weight": (lambda lw: ops.linear_act(x, lw), lw), "linear_act bias": (lambda b: ops.linear_act(x, lw, b), ws),
+        "linear_act residual": (lambda r: ops.linear_act(x, lw, None, r), make(4, 32)), "rotary": (lambda x: ops.rotary(x, p, fr, [8]), make(1, 4, 2, 16)),
+        "rotary frequencies": (lambda fr: ops.rotary(make(1, 4, 2, 16), p, fr, [8]), fr),
+        "rotary_": (lambda x: ops.rotary_(x, p, fr, [8]), make(1, 4, 2, 16)), "quantize_fp8": (lambda x: ops.quantize_fp8(x)[1], x),
+        "rms_norm_fp8": (lambda x: ops.rms_norm_fp8(x, w)[1], x), "add_rms_norm_fp8": (lambda x: ops.add_rms_norm_fp8(x, x, w)[2], x),
+        "linear_fp8 scale": (lambda s: ops.linear_fp8(q, s, wq, ws), s), "linear_fp8 bias": (lambda b: ops.linear_fp8(q, s, wq, ws, b), ws),
+        "linear_fp8 residual": (lambda r: ops.linear_fp8(q, s, wq, ws, None, r), make(4, 32)),
+    }
+
+
+DERIVATIVES = ["rms_norm", "rms_norm weight", "add_rms_norm residual", "linear_act", "linear_act weight", "linear_act bias", "linear_act residual",
+               "rotary", "rotary frequencies", "rotary_", "quantize_fp8", "rms_norm_fp8", "add_rms_norm_fp8", "linear_fp8 scale", "linear_fp8 bias",
+               "linear_fp8 residual"]
+
+
+def refuses_other_derivatives(f, x):
+    from torch.autograd import forward_ad
+    for grad in (True, False):                      # (torch.no_grad() is about the backward pass)
+        with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                f(forward_ad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+        torch.func.jvp(f, (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError, match="no gradient|functorch"):
+        torch.func.grad(lambda x: f(x).float().sum())(x)
+    f(x.clone())
+
+
+@pytest.mark.parametrize("name", DERIVATIVES)
+def test_derivatives_that_there_are_not_are_refused(name):
+    """forward mode and functional transforms: refused, never a tangent or gradient of zeros"""
+    refuses_other_derivatives(*derivative_calls("meta")[name])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", DERIVATIVES)
+def test_derivatives_that_there_are_not_are_refused_on_the_gpu(name):
+    refuses_other_derivatives(*derivative_calls("cuda")[name])
+
+
+def test_8_bit_operands_that_require_a_gradient_are_refused():
+    ops, f32, f8 = T(), torch.float32, torch.float8_e4m3fn
+    q, wq, s, ws = (torch.empty(*n, dtype=t, device="meta") for n, t in (((4, 64), f8), ((32, 64), f8), ((4,), f32), ((32,), f32)))
+    for a, b in ((q.detach().requires_grad_(), wq), (q, wq.detach().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.linear_fp8(a, s, b, ws)
+        with torch.no_grad():
+            ops.linear_fp8(a, s, b, ws)
+
+
+@pytest.mark.gpu
+def test_mapped_over_a_batch():
+    """torch.vmap of the operators without gradients: each entry as its own call gives it"""
+    ops, g = T(), gen(61)
+    x, w, lw = randn(g, 3, 4, 64, dtype=torch.bfloat16), randn(g, 64), randn(g, 32, 64, dtype=torch.bfloat16)
+    for f in (lambda x: ops.rms_norm(x, w), lambda x: ops.linear_act(x, lw, None, None, "silu"), lambda x: ops.quantize_fp8(x)[1]):
+        assert torch.equal(torch.vmap(f)(x), torch.stack([f(v) for v in x]))
