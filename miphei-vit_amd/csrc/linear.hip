@@ -50,7 +50,9 @@ int check(const mvit_linear_args* g, int es, Args& a, bool& vec) {
 // tenths of a microsecond: 40 for a round of blocks and for each of its K tiles of 128 bytes 10 and 4 with tiles of 128 x 128 and 64 x 64 (7 and 3
 // with one block a CU), 22 for every 32 of them by rows; 50 for the second launch and 8 bytes an output and part at 5 TB/s.  Taken where that
 // says a quarter less (at a seventh, [134, 2352] x [395, 2352] lost 1 us).  us without and with: bf16 [1, 16384] x [512, 16384] 22 / 10,
-// [64, 7792] x [2558, 7792] 35 / 21, the same in e4m3 20 / 16, [66, 6784] x [146, 6784] 25 / 14, [37, 2560] x [2044, 2560] 11.4 / 9.0
+// [64, 7792] x [2558, 7792] 35 / 21, the same in e4m3 20 / 16, [66, 6784] x [146, 6784] 25 / 14, [37, 2560] x [2044, 2560] 11.4 / 9.0,
+// [513, 14336] x [4096, 14336] 138 / 74, [1400, 8192] x [1536, 8192] 77 / 48.  e4m3 with a 16-bit y leaves the e4m3 instructions for it and gains the least:
+// [513, 14336] x [4096, 14336] 71 / 71, onto an f32 stream 104 / 72
 struct Parts {
   int kind, splits, kper;
 };
@@ -64,7 +66,7 @@ Parts plan_parts(int M, int N, long long kb) {
     const int b = kind == 0 ? 16 : kind == 2 ? 128 : 64;
     const long long tiles = (kind == 0 ? 1 : ((long long)M + b - 1) / b) * ((N + b - 1) / b);
     const int slots = 2 * cus;
-    if (tiles > slots) return {0, 1, 1 << 20};
+    if (tiles > slots) continue;   // (no room for parts here; and by_size forms nothing whole of them where 128 x 128 tiles are one a CU at most)
     for (int want = 1; want <= 16 && tiles * want <= slots && nk >= 4 * want; ++want) {
       const int kper = (nk + want - 1) / want, s = (nk + kper - 1) / kper;
       double c = 40. + (kind == 0 ? 22. * ((kper + 31) / 32) : (double)kper * (kind == 2 ? (tiles * s <= cus ? 7 : 10) : (tiles * s <= cus ? 3 : 4)));

@@ -1295,3 +1295,39 @@ def test_mapped_over_a_batch():
     x, w, lw = randn(g, 3, 4, 64, dtype=torch.bfloat16), randn(g, 64), randn(g, 32, 64, dtype=torch.bfloat16)
     for f in (lambda x: ops.rms_norm(x, w), lambda x: ops.linear_act(x, lw, None, None, "silu"), lambda x: ops.quantize_fp8(x)[1]):
         assert torch.equal(torch.vmap(f)(x), torch.stack([f(v) for v in x]))
+
+
+# ------------------------------------------------------------------ K in parts of large tiles
+# 64 x 64 tiles that leave no room for parts, 128 x 128 tiles that do; ragged ones, and the first row behind the border
+LARGE_PARTS = [(513, 14336, 4096), (1400, 8192, 1536), (1297, 8200, 1607)]
+
+
+@pytest.mark.parametrize("M,K,N", LARGE_PARTS + [(2048, 8192, 1152), (1025, 16384, 2048)])
+def test_room_for_parts_of_large_tiles(M, K, N):
+    from miphei_vit_amd import _lib
+    lib = _lib.lib()
+    assert lib.mvit_linear_scratch_bytes(M, N, 2 * K) == 3 * M * N * 4      # 132 to 165 tiles for 256 CUs: three parts make two blocks a CU of most of them
+    assert lib.mvit_linear_scratch_bytes(5264, 4096, 2 * 1536) == lib.mvit_linear_scratch_bytes(1301, 1536, 2 * 4096) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("res", ["none", "half", "f32"])
+@pytest.mark.parametrize("M,K,N", LARGE_PARTS)
+def test_linear_of_a_long_k_in_large_tiles(M, K, N, res):
+    """16-bit operands of any K that they take; e4m3 operands of the next multiple of 16"""
+    ops, g = T(), gen(M + K + N)
+    dtype, act = HALF[(M + N) % 2], ACTS[(M + len(res)) % 5]
+    rt = {"none": None, "half": dtype, "f32": torch.float32}[res]
+    x, w, b, r = linear_case(g, M, K, N, dtype, rt, bool(N % 2))
+    rd = 0 if r is None else r.double()
+
+    def check(y, xd, wd, f32=F32):
+        z, mag = xd @ wd.t() + b.double(), xd.abs() @ wd.abs().t() + b.double().abs()
+        close(y, act_oracle(z, act)[0] + rd, 1.2 * mag + (0 if r is None else rd.abs()), "y", f32)
+    y = ops.linear_act(x, w, b, r, act)
+    check(y, x.double(), w.double())
+    assert torch.equal(y, ops.linear_act(x, w, b, r, act))
+    x, w = (torch.nn.functional.pad(t, (0, -K % 16)) for t in (x, w))
+    xs, ws = (t.float().abs().amax(-1) / 448 for t in (x, w))          # (rows longer than quantize_fp8 takes)
+    xq, wq = ((t.float() / s[:, None]).to(torch.float8_e4m3fn) for t, s in ((x, xs), (w, ws)))
+    check(ops.linear_fp8(xq, xs, wq, ws, b, r, act, dtype), xq.double() * xs.double()[:, None], wq.double() * ws.double()[:, None], F32 if res == "f32" else F8)
