@@ -641,11 +641,11 @@ Tensor rotary_forward_autograd(const Tensor& x, const Tensor& positions, const T
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
-                               std::string act) {
+                               std::string act, bool save_pre) {
     // (the K axis of dW = dz^T x)
     REQUIRE(!weight.requires_grad() || x.sym_numel() <= weight.sym_size(1) * (1 << 29), "linear_act", "more than 2^29 rows of x with a gradient of weight");
     at::AutoDispatchBelowAutograd below;
-    const bool keep = act != "none" && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
+    const bool keep = save_pre || (act != "none" && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad())));
     auto [y, pre] = linear_forward_op().call(x, weight, bias, residual, act, keep);
     ctx->save_for_backward({x, weight, pre});
     ctx->saved_data["act"] = act;
@@ -657,7 +657,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     return {y, pre};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    variable_list out(5);
+    variable_list out(6);
     if (!g[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const bool bias = ctx->saved_data["bias"].toBool(), res = ctx->saved_data["residual"].toBool();
@@ -678,7 +678,7 @@ std::tuple<Tensor, Tensor> linear_act_forward_autograd(const Tensor& x, const Te
                                                        c10::string_view act, bool save_pre) {
   no_tangent("linear_act", {x, weight, bias, residual});
   if (wants_grad({x, weight, bias, residual})) {
-    auto o = LinearAct::apply(x, weight, bias, residual, std::string(act));
+    auto o = LinearAct::apply(x, weight, bias, residual, std::string(act), save_pre);
     return {o[0], o[1]};
   }
   at::AutoDispatchBelowAutograd below;

@@ -1331,3 +1331,28 @@ def test_linear_of_a_long_k_in_large_tiles(M, K, N, res):
     xs, ws = (t.float().abs().amax(-1) / 448 for t in (x, w))          # (rows longer than quantize_fp8 takes)
     xq, wq = ((t.float() / s[:, None]).to(torch.float8_e4m3fn) for t, s in ((x, xs), (w, ws)))
     check(ops.linear_fp8(xq, xs, wq, ws, b, r, act, dtype), xq.double() * xs.double()[:, None], wq.double() * ws.double()[:, None], F32 if res == "f32" else F8)
+
+
+# ------------------------------------------------------------------ the value in front of the activation
+def pre_of_all_modes(device):
+    g = torch.Generator(device=device).manual_seed(62) if device == "cuda" else None
+    make = (lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()) if g else (lambda *s: torch.empty(*s, device=device, dtype=torch.bfloat16))  # noqa: E731
+    for act in ("none", "gelu"):
+        for wants in ((), (0,), (1,), (2,), (3,), (0, 1, 2, 3)):
+            args = [t.requires_grad_(k in wants) for k, t in enumerate((make(5, 64), make(24, 64), make(24), make(5, 24)))]
+            yield act, wants, args, torch.ops.mvit.linear_act_forward(*args, act, True)
+
+
+def test_pre_activation_is_given_where_it_is_asked_for():
+    for act, wants, _, (y, pre) in pre_of_all_modes("meta"):
+        assert pre.shape == y.shape == (5, 24), (act, wants)
+        assert y.requires_grad == bool(wants) and not pre.requires_grad
+
+
+@pytest.mark.gpu
+def test_pre_activation_is_given_where_it_is_asked_for_on_the_gpu():
+    for act, wants, (x, w, b, r), (y, pre) in pre_of_all_modes("cuda"):
+        x, w, b = (t.detach().double() for t in (x, w, b))
+        close(pre, x @ w.t() + b, x.abs() @ w.abs().t() + b.abs(), f"{act} {wants}")
+        if wants:
+            y.backward(torch.ones_like(y))
