@@ -392,10 +392,12 @@ int bwd_layout(const BwdArgs& a, int& grid, hipStream_t s) {
   const int D = a.D;
   // f32 stream, with d w, us.  A wave a row or a block: rows of 1024: 1024 of them 9.6 / 8.1, 4096 17.5 / 17.7, 8192 26 / 28, 21056 69 / 87;
   // of 1536: 21056 107 / 105; of 2048: 140 / 127.  A row to 256 threads or to 512: of 1536: 1024 11.1 / 9.0 (twice the partial sums of
-  // d w), 8192 35 / 34, 21056 96 / 105; of 2048: 131 / 126
+  // d w), 8192 35 / 34, 21056 96 / 105; of 2048: 131 / 126.  Rows that leave most of 512 threads without a piece go to 256 sooner: of 520: 2000 10.7 /
+  // 10.7, 4000 12.2 / 15.0; of 768: 4000 13.5 / 15.3; of 1053 (odd): 1000 13.3 / 11.1, 4000 22.8 / 28.0, 8000 36 / 49; of 1280: 2000 12.4 / 11.6,
+  // 4000 18.0 / 18.2
   if (D <= 512) return launch_bwd<512, 64, 1, ODD, XT, HT>(a, grid, s);
   if (D <= 1024 && a.M >= 16 * mvit_num_cus()) return launch_bwd<512, 64, 2, ODD, XT, HT>(a, grid, s);
-  if (D <= 1920 && a.M >= 32 * mvit_num_cus()) return launch_bwd<256, 256, 1, ODD, XT, HT>(a, grid, s);
+  if (D <= 1920 && a.M >= (D <= 1280 ? 8 : 32) * mvit_num_cus()) return launch_bwd<256, 256, 1, ODD, XT, HT>(a, grid, s);
   if (D <= 4096) return launch_bwd<512, 512, 1, ODD, XT, HT>(a, grid, s);
   if (D <= 8192) return launch_bwd<512, 512, 2, ODD, XT, HT>(a, grid, s);
   return launch_bwd<512, 512, 4, ODD, XT, HT>(a, grid, s);

@@ -1356,3 +1356,11 @@ def test_pre_activation_is_given_where_it_is_asked_for_on_the_gpu():
         close(pre, x @ w.t() + b, x.abs() @ w.abs().t() + b.abs(), f"{act} {wants}")
         if wants:
             y.backward(torch.ones_like(y))
+
+
+# ------------------------------------------------------------------ the norm's backward pass: widths between the layouts' borders, types
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16)], ids=str)
+@pytest.mark.parametrize("M,D", [(2047, 520), (2049, 520), (4100, 768), (4095, 1053), (2050, 1280), (2050, 1281), (8200, 1100)])
+def test_rms_norm_between_the_layouts(M, D, types):
+    test_rms_norm_forward_backward(M, D, types)
