@@ -1364,3 +1364,97 @@ def test_pre_activation_is_given_where_it_is_asked_for_on_the_gpu():
 @pytest.mark.parametrize("M,D", [(2047, 520), (2049, 520), (4100, 768), (4095, 1053), (2050, 1280), (2050, 1281), (8200, 1100)])
 def test_rms_norm_between_the_layouts(M, D, types):
     test_rms_norm_forward_backward(M, D, types)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("res", [False, True])
+@pytest.mark.parametrize("out", HALF)
+@pytest.mark.parametrize("M,D", [(1, 1), (5, 512), (1037, 520), (70, 1531), (40, 4096), (9, 8192), (2, 16383), (4097, 64)])
+def test_rms_norm_of_an_f32_stream_with_a_16_bit_output(M, D, out, res):
+    """the second norm of a block: dy in 16 bits, everything else in f32"""
+    ops, g = T(), gen(M * 13 + D)
+    x, w = randn(g, M, D).requires_grad_(), (1 + 0.2 * randn(g, D)).requires_grad_()
+    dy = randn(g, M, D, dtype=out)
+    if res:
+        r, dh = randn(g, M, D, scale=3).requires_grad_(), randn(g, M, D)
+        y, h = ops.add_rms_norm(x, r, w, 1e-5, out_dtype=out)
+        close(h.detach(), x.detach().double() + r.detach().double(), x.detach().double().abs() + r.detach().double().abs(), "h")
+        dx, dr, dw = torch.autograd.grad((y, h), (x, r, w), (dy, dh))
+        assert torch.equal(dx, dr)
+    else:
+        y, h, dh = ops.rms_norm(x, w, 1e-5, out_dtype=out), x, None
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert y.dtype == out and dx.dtype == dw.dtype == torch.float32
+    hd, wd, dyd = h.detach().double(), w.detach().double(), dy.double()
+    want, rstd = norm_oracle(hd, wd, 1e-5)
+    close(y.detach(), want, want.abs(), "y")
+    xhat, wdy = hd * rstd, wd * dyd
+    base = 0 if dh is None else dh.double()
+    close(dx, base + rstd * (wdy - xhat * (wdy * xhat).mean(-1, keepdim=True)),
+          (0 if dh is None else dh.double().abs()) + rstd * (wdy.abs() + xhat.abs() * (wdy * xhat).abs().mean(-1, keepdim=True)), "dx")
+    close(dw, (dyd * xhat).sum(0), (dyd * xhat).abs().sum(0), "dweight")
+
+
+# ------------------------------------------------------------------ what stood in the tests above without being asked
+@pytest.mark.parametrize("sections", [[], [0], [0, 0]], ids=str)
+def test_rotary_without_sections_is_refused(sections):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = T()
+    with FakeTensorMode():
+        x, n = fake(2, 7, 6, 16), len(sections)
+        for f in (ops.rotary, ops.rotary_):
+            with pytest.raises(ValueError, match="sections"):
+                f(x, fake(7, n, dtype=torch.int32), fake(0, dtype=torch.float32), sections)
+
+
+def test_a_varying_number_of_rows_stays_one():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
+    ops, mode = T(), FakeTensorMode(shape_env=ShapeEnv())
+    x = mode.from_tensor(torch.empty(6, 64, dtype=torch.bfloat16, device="meta"),
+                         symbolic_context=StatelessSymbolicContext(dynamic_sizes=[DimDynamic.DYNAMIC, DimDynamic.STATIC]))
+    with mode:
+        y, h = ops.add_rms_norm(x, x.float(), torch.empty(64, device="meta"))
+        q, s = ops.quantize_fp8(y)
+        z = ops.linear_act(x, torch.empty(48, 64, device="meta", dtype=torch.bfloat16))
+    for t in (y, h, q, s, z):
+        assert isinstance(t.shape[0], torch.SymInt), t.shape      # (a plain int here would be a size that the trace has fixed)
+
+
+@pytest.mark.gpu
+def test_serving_block_in_8_bits_against_64_bits():
+    """attention's half of a block in 8 bits, each step against 64 bits on what it was given, and all of it against the unquantised block.
+
+    The whole: e4m3 with a scale a row is off by at most 2^-4 of a value above its normal range, uniformly spread in its step: on the average of
+    values 2^-4 / sqrt 3 relative at the bottom of a binade, half of that at its top, 0.027 of a tensor's norm (2^-4 / sqrt 3 * 0.75).  A product of
+    two such operands, of random signs, is off by 0.027 sqrt 2 = 0.038 of its norm.  q, k and v carry it; the softmax averages v over 41 keys, their
+    errors with it, and turns the scores' error, 0.038 sqrt 2 of scores of unit size, into as much of its weights, uncorrelated with v: 0.038 + 0.054 in
+    quadrature 0.066.  The projection quantises twice more (0.038): 0.076 of the branch's norm.  Three times that bounds it."""
+    ops = T()
+    x, branch, p, pos, freq, B, N, H, prefix = block_inputs()
+    D = x.shape[-1]
+    Dh = D // H
+    wq, ws = ops.quantize_fp8(p["wqkv"])
+    oq, os_ = ops.quantize_fp8(p["wo"])
+    with torch.no_grad():
+        q, s, h = ops.add_rms_norm_fp8(branch, x, p["n"])
+        qkv = ops.linear_fp8(q, s, wq, ws, p["bqkv"])
+        before = qkv.clone()
+        ops.rotary_(qkv.view(B, N, 3 * H, Dh), pos, freq, [8, 8], 2 * H, prefix)
+        a = ops.attention(qkv, H)
+        y = ops.linear_fp8(*ops.quantize_fp8(a), oq, os_, p["bo"], h)
+    close(qkv.view(B, N, 3 * H, Dh), *rotary_oracle(before.view(B, N, 3 * H, Dh), pos, freq, [8, 8], 2 * H, prefix, False), "rotary_")
+    # attention of the same 16-bit q | k | v: the weights (for the second product) and the result are rounded to bf16, 2^-8 of the weights times |v| each
+    z = qkv.double().view(B, N, 3, H, Dh).permute(2, 0, 3, 1, 4)
+    weights = torch.softmax(z[0] @ z[1].transpose(2, 3) * Dh ** -0.5, -1)
+    want, mag = ((weights @ v).transpose(1, 2).reshape(B, N, D) for v in (z[2], z[2].abs()))
+    assert bool(((a.double() - want).abs() <= (2 * 2.0 ** -8 + F32) * mag).all())
+    # the unquantised half in 64 bits
+    pd = {k: v.double() for k, v in p.items()}
+    hd = x.double() + branch.double()
+    u = (norm_oracle(hd, pd["n"], 1e-6)[0] @ pd["wqkv"].t() + pd["bqkv"]).view(B, N, 3 * H, Dh)
+    u = rotary_oracle(u, pos, freq, [8, 8], 2 * H, prefix, False)[0].view(B, N, 3, H, Dh).permute(2, 0, 3, 1, 4)
+    out = (torch.softmax(u[0] @ u[1].transpose(2, 3) * Dh ** -0.5, -1) @ u[2]).transpose(1, 2).reshape(B, N, D) @ pd["wo"].t()
+    assert float(h.double().sub(hd).norm()) <= 2.0 ** -24 * float(hd.norm())
+    got = y.double() - h.double() - pd["bo"]
+    assert rel(got, out) < 3 * 0.076, rel(got, out)
