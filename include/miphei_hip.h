@@ -203,9 +203,12 @@ typedef struct mvit_rotary_args {
 } mvit_rotary_args;
 MVIT_API int mvit_rotary(const mvit_rotary_args* args, mvit_stream_t stream);
 
-/* y[M,N] = res + act(x[M,K] W[N,K]^T + bias), f32 accumulation.  mvit_linear_act: 16-bit x, W; pre (optional, 16-bit, dense [M,N])
- * receives the value in front of the activation for the backward pass.  mvit_linear_fp8: e4m3 x, W, the product times
- * x_scale(f32)[m] * w_scale(f32)[n]; no pre.  bias [N] f32 or 16-bit, may be NULL.  y dense, f32 or 16-bit; res (may be NULL) has y's type
+/* y[M,N] = res + act(x[M,K] W[N,K]^T + bias).  mvit_linear_act: 16-bit x, W, f32 accumulation; pre (optional, 16-bit whatever y's type, dense
+ * [M,N]) receives the value in front of the activation for the backward pass.  mvit_linear_fp8: e4m3 x, W, the product times
+ * x_scale(f32)[m] * w_scale(f32)[n]; no pre.  With an f32 y its products are formed on the 16-bit instructions (operands widened, exact) and added in
+ * f32.  With a 16-bit y the e4m3 instructions may form them: they add neighbouring products with 13 bits below the largest of those, so that a sum
+ * is off by up to 2^-13 of the sum of the products' magnitudes, below half a step of fp16 (2^-11) and of bf16 (2^-8) of them; which of the two it is goes by
+ * M, N and K, and so may a row's last bits.  bias [N] f32 or 16-bit, may be NULL.  y dense, f32 or 16-bit; res (may be NULL) has y's type
  * and its own row stride ldr.  ldx, ldw, ldr in elements.  x, W rows start on 16 bytes and K is a multiple of 16 bytes (8 or 16 values);
  * K and the row strides of x and W are at most 2^23 bytes.  M up to 2^30, N up to 2^24, of any size.  scratch (may be
  * NULL: slower): mvit_linear_scratch_bytes(M, N, bytes of a row of K) bytes, on 16 bytes, for the products of parts of a long K where there are few

@@ -1,5 +1,5 @@
 // y = residual + act((x W^T) [* x_scale[m] * w_scale[n]] + bias) on the matrix cores: x [M, K], W [N, K], both K-contiguous, 16-bit
-// operands (bf16; fp16 under MVIT_F16) or e4m3 with a scale for each row of either.  f32 accumulation throughout.
+// operands (bf16; fp16 under MVIT_F16) or e4m3 with a scale for each row of either.  f32 accumulation, but for what mode F8 does (below).
 //
 // Everything below counts K in BYTES: a 128-byte row piece is 64 16-bit or 128 8-bit values, and the matrix instructions take equal time
 // for equal bytes (v_mfma_f32_16x16x32 and the twice as wide v_mfma_f32_32x32x64_f8f6f4), so that one pipeline serves both.
@@ -161,6 +161,8 @@ __device__ __forceinline__ uint4 finish(const Args& p, float (&v)[W], int row, i
   static_assert(W == (E::out32 ? 4 : 8), "16 bytes of y");
 #pragma unroll
   for (int e = 0; e < W; ++e) v[e] = OP8 ? __builtin_fmaf(v[e], c.s[e], c.b[e]) : v[e] + c.b[e];
+  // (kept in 16 bits also beside an f32 y: what comes of it, dz, is rounded to the operands' 16 bits for the matrix instructions anyway, and f32 would
+  // double what the forward pass writes and the backward pass reads again)
   if (!OP8 && p.pre && row < p.M && col < p.N) {
     uint32_t u[W / 2];
 #pragma unroll

@@ -13,8 +13,9 @@
 //    addresses and a row's last piece goes by elements; with all of it by elements an f32 stream of [16623, 1053] to 8 bits took 106 us
 //    instead of 46, of [2032, 7956] 257 instead of 40.
 //  * Rows are walked with a grid stride, so that w is loaded once per thread and not once per row.
-// Measured against a 1 GiB copy's 5.05 TB/s (one MI355X): f32 stream of [21056, 1536] forward 75 us (388 MB, 5.2 TB/s), backward with
-// d w 96 us (517 MB, 5.4 TB/s); 16-bit stream to 8 bits [20816, 1536] 37 us (6.0 TB/s); quantisation [21056, 4096] 43 us (6.0 TB/s).
+// Measured against a 1 GiB copy's 5.05 TB/s (one MI355X, kernels by themselves): f32 stream of [21056, 1536] forward 71 us (388 MB, 5.5 TB/s), backward
+// 97 us (517 MB, 5.3 TB/s) and 5 for d w's partial sums; 16-bit stream to 8 bits [20816, 1536] 34 us (6.6 TB/s); quantisation [21056, 4096] 39 us
+// (6.6 TB/s).  Among other calls a pass takes some 10 us more, in 8 bits 43 and 48.
 // Sums and statistics are f32; sums over the rows (d w) go row by row in registers, over the waves of a block in LDS, over the blocks
 // through a [blocks][D] f32 workspace that a second launch adds up: a fixed order, no atomics, bit-identical from run to run.
 #include "column_sums.hpp"

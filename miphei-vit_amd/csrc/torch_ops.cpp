@@ -213,7 +213,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_backward(const Tensor& dy, const Opt
   c10::DeviceGuard guard(h.device());
   NormBwd o = norm_bwd_out(h, weight, x_dtype, need_x, need_residual, need_weight);
   const int64_t d = h.size(-1), m = h.numel() / d;
-  // the kernel's dx has dy's type: the gradient of a 16-bit output of an f32 x is widened first
+  // the kernel's dx has dy's type: the gradient of a 16-bit output of an f32 x is widened first (a pass of its own, some 30 us of 99 at [21056, 1536])
   const Tensor h2 = h.contiguous(), dy2 = dy.to(x_dtype).contiguous(), w = weight.contiguous();
   const OptTensor dh2 = dh ? OptTensor(dh->to(h.scalar_type()).contiguous()) : std::nullopt;
   HalfType half{"rms_norm"};

@@ -12,7 +12,8 @@ foundation_models.py:53-57``), ``WeightedMSELoss`` (``/root/reference/src/loss.p
     torch.ops.mvit.weighted_mse(pred, target, w, lam)  WeightedMSELoss.forward     -> mvit_wmse_fwd_bwd
 
 The further operators of a transformer block (RMS norm of a residual stream, rotary positions, linear with activation and residual, 8-bit
-forms) are defined in ``block_ops`` and re-exported here.
+forms) are defined in ``block_ops`` and re-exported here.  Of the two linear layers, ``linear`` takes f32 masters and rounds them itself, as under
+autocast; ``linear_act`` takes 16-bit tensors as they are and has the faster backward pass.
 
 Arithmetic is the reference's bf16-mixed mode: bf16 operands, f32 accumulation, f32 LayerNorm statistics.  Every op has a fake
 (meta) implementation, so FakeTensor tracing / torch.compile shape propagation work, and an autograd formula built on the
